@@ -1,0 +1,827 @@
+// Embedding rows by index, times a scale, and the gradient of that lookup.
+//
+//   forward   out[t, :] = scale * table[index[t], :]
+//   backward  dtable[v, :] (+)= scale * sum over t with index[t] == v of grad[t, :]
+//
+// Both are bound by HBM: the forward reads each looked-up row and writes each output row once, the
+// backward reads each incoming row once and writes each table row once.
+//
+// The backward is one cooperative kernel without floating-point atomics, so the result is the same in
+// every run:
+//   1. a stable radix sort of (index, position) pairs: least significant digit first, at most 9 bits
+//      a pass (the least number of passes, bits shared evenly).  Each sorting block owns a contiguous
+//      range of tokens; a pass is its digit histogram, a scan of every digit's counts over the blocks,
+//      and the scatter, where a warp ranks 32 keys at a time by matching equal digits.  One block
+//      sorts alone, without grid barriers, when it holds all tokens.
+//   2. segment sums over equal shares of the sorted list (not of the table: a row looked up by half
+//      of the tokens is shared by as many workers as its tokens deserve).  A worker is a group of 8,
+//      16 or 32 lanes with 16-byte vectors side by side on a row; it keeps one fp32 sum per column in
+//      registers, four or eight rows in flight.  Runs inside a share are written at once; a run that crosses a
+//      border leaves its part in the workspace.
+//   3. the parts of each crossing run, added in order.
+// An index outside [0, rows) yields a row of zeros, takes no gradient and sets the sticky error word;
+// tokens with the padding index take no gradient.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "pbg_common.cuh"
+
+namespace pbg {
+
+enum { EMB_F32 = 0, EMB_BF16 = 1, EMB_F16 = 2 };
+constexpr int EMB_THREADS = 512;
+constexpr int EMB_WARPS = EMB_THREADS / 32;
+constexpr int EMB_BINS = 512;        // 9-bit digits
+constexpr int EMB_MAX_KPT = 8;       // keys a thread ranks per tile
+constexpr int EMB_MIN_SHARE = 16;    // sorted tokens a worker takes at least
+constexpr int EMB_SERIAL_PARTS = 16; // parts of a run that one worker adds
+constexpr uint32_t EMB_WAIT_TRIES = 1u << 24;
+
+template <typename T>
+__device__ __forceinline__ float emb_float(T v) {
+    if constexpr (std::is_same<T, float>::value) return v;
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __bfloat162float(v);
+    else return __half2float(v);
+}
+
+template <typename T>
+__device__ __forceinline__ T emb_zero() {
+    if constexpr (std::is_same<T, float>::value) return 0.0f;
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __ushort_as_bfloat16(0);
+    else return __ushort_as_half(0);
+}
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC > 16 ? 16 : sizeof(T) * VEC) EmbVec {
+    T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void emb_load(const T* p, float* f) {
+    const EmbVec<T, VEC> x = *reinterpret_cast<const EmbVec<T, VEC>*>(p);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = emb_float(x.v[i]);
+}
+
+// VEC values rounded once to the output's type and stored; `type` is uniform over the launch.
+template <int VEC>
+__device__ __forceinline__ void emb_store(void* base, int64_t at, int type, const float* f) {
+    if (type == EMB_F32) {
+        constexpr int W = VEC > 4 ? 4 : VEC;
+#pragma unroll
+        for (int q = 0; q < VEC / W; ++q) {
+            EmbVec<float, W> x;
+#pragma unroll
+            for (int i = 0; i < W; ++i) x.v[i] = f[q * W + i];
+            reinterpret_cast<EmbVec<float, W>*>(static_cast<float*>(base) + at)[q] = x;
+        }
+    } else if (type == EMB_BF16) {
+        EmbVec<__nv_bfloat16, VEC> x;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x.v[i] = __float2bfloat16_rn(f[i]);
+        *reinterpret_cast<EmbVec<__nv_bfloat16, VEC>*>(static_cast<__nv_bfloat16*>(base) + at) = x;
+    } else {
+        EmbVec<__half, VEC> x;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) x.v[i] = __float2half_rn(f[i]);
+        *reinterpret_cast<EmbVec<__half, VEC>*>(static_cast<__half*>(base) + at) = x;
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void emb_load_typed(const void* base, int64_t at, int type, float* f) {
+    if (type == EMB_F32) {
+        constexpr int W = VEC > 4 ? 4 : VEC;
+#pragma unroll
+        for (int q = 0; q < VEC / W; ++q) emb_load<float, W>(static_cast<const float*>(base) + at + q * W, f + q * W);
+    } else if (type == EMB_BF16) {
+        emb_load<__nv_bfloat16, VEC>(static_cast<const __nv_bfloat16*>(base) + at, f);
+    } else {
+        emb_load<__half, VEC>(static_cast<const __half*>(base) + at, f);
+    }
+}
+
+__device__ __forceinline__ int64_t emb_index(const void* index, int wide, int64_t t) {
+    return wide ? __ldg(static_cast<const long long*>(index) + t) : (int64_t)__ldg(static_cast<const int*>(index) + t);
+}
+
+// ---------------------------------------------------------------- forward
+
+struct EmbArgs {
+    int64_t tokens, rows, width, ldt;
+    const void* index;
+    int index64;
+    const void* table;
+    void* out;
+    int out_type;
+    int log_lanes;  // lanes side by side on one row
+    float scale;
+    uint32_t* error;
+};
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) embedding_kernel(EmbArgs E) {
+    const int lanes = 1 << E.log_lanes;
+    const int lane = threadIdx.x & (lanes - 1);
+    const int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> E.log_lanes;
+    const int64_t step = ((int64_t)gridDim.x * 256) >> E.log_lanes;
+    const T* table = static_cast<const T*>(E.table);
+    for (int64_t t = first; t < E.tokens; t += step) {
+        const int64_t i = emb_index(E.index, E.index64, t);
+        const bool live = i >= 0 && i < E.rows;
+        if (!live && lane == 0) *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
+        const T* src = table + (live ? i : 0) * E.ldt;
+        for (int64_t c0 = (int64_t)lane * VEC; c0 < E.width; c0 += (int64_t)lanes * VEC * 4) {
+            float f[4][VEC];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t c = c0 + (int64_t)u * lanes * VEC;
+                if (live && c < E.width) {
+                    emb_load<T, VEC>(src + c, f[u]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) f[u][k] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t c = c0 + (int64_t)u * lanes * VEC;
+                if (c < E.width) {
+                    if (live) {
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) f[u][k] *= E.scale;
+                    }
+                    emb_store<VEC>(E.out, t * E.width + c, E.out_type, f[u]);
+                }
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- backward
+
+struct EmbGradArgs {
+    int64_t tokens, rows, width, ldg, ldo;
+    const void* grad;
+    const void* index;
+    int index64;
+    int64_t padding;     // -1: none
+    void* out;
+    int out_type, accumulate;
+    float scale;
+    uint32_t* error;
+    // plan
+    int passes, bits;    // radix passes and digit bits
+    int parts, kpt;      // sorting blocks, keys per thread and tile
+    int64_t part_tokens; // tokens a sorting block owns
+    int lanes;           // lanes of a worker
+    int tiles;           // column tiles of lanes * VEC
+    int64_t share;       // sorted tokens of one worker's task
+    int64_t shares;
+    int zero_first;      // the whole table zeroed beside the sort; else its absent rows after it
+    // workspace
+    uint32_t* barrier;
+    uint32_t* counts;    // [bins][parts], then their scans
+    uint32_t* totals;    // [bins]
+    uint32_t* key[2];
+    int32_t* pos[2];
+    float* part_sums;    // [shares][2][width]
+};
+
+// Arrivals counted in one word; the kernel is launched cooperatively, so every block runs.  A wait
+// that runs out records 2 in the error word and lets its block go on to the end of the kernel
+// without touching the output.
+__device__ __forceinline__ bool emb_grid_sync(const EmbGradArgs& E, uint32_t& target) {
+    if (gridDim.x == 1) {
+        __syncthreads();
+        return true;
+    }
+    __shared__ int ok_s;
+    target += gridDim.x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        uint32_t seen = atomicAdd(E.barrier, 1u) + 1u;
+        uint32_t i = 0;
+        while ((int32_t)(seen - target) < 0 && i < EMB_WAIT_TRIES) {
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(E.barrier) : "memory");
+            ++i;
+        }
+        const int ok = (int32_t)(seen - target) >= 0;
+        if (!ok) atomicExch(E.error, 2u);
+        __threadfence();
+        ok_s = ok;
+    }
+    __syncthreads();
+    return ok_s != 0;
+}
+
+// token t's sort key: its row, or `rows` (sorted last, no gradient) for the padding index and for an
+// index outside the table
+__device__ __forceinline__ uint32_t emb_key(const EmbGradArgs& E, int64_t t) {
+    const int64_t i = emb_index(E.index, E.index64, t);
+    if (i < 0 || i >= E.rows) {
+        *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
+        return (uint32_t)E.rows;
+    }
+    return i == E.padding ? (uint32_t)E.rows : (uint32_t)i;
+}
+
+struct EmbSortShared {
+    uint32_t base[EMB_BINS];                  // next position of each digit for this block
+    uint16_t warp_count[EMB_WARPS][EMB_BINS];
+    uint32_t scan[EMB_WARPS];
+};
+
+// exclusive scan over the block's 512 threads
+__device__ __forceinline__ uint32_t emb_block_scan(uint32_t v, uint32_t* warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int w = 0; w < warp; ++w) before += warp_sums[w];
+    __syncthreads();
+    return before + x - v;
+}
+
+// one radix pass of the calling block's range; false when a grid barrier gave up
+__device__ bool emb_radix_pass(const EmbGradArgs& E, int pass, uint32_t& target, EmbSortShared& S) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int shift = pass * E.bits, bins = 1 << E.bits;
+    const uint32_t mask = (uint32_t)bins - 1u;
+    const bool sorting = (int)blockIdx.x < E.parts;
+    const int64_t lo = (int64_t)blockIdx.x * E.part_tokens;
+    const int64_t hi = sorting ? (lo + E.part_tokens < E.tokens ? lo + E.part_tokens : E.tokens) : lo;
+    const uint32_t* src_key = E.key[(pass & 1) ^ 1];
+    const int32_t* src_pos = E.pos[(pass & 1) ^ 1];
+    if (sorting) {
+        for (int b = threadIdx.x; b < bins; b += EMB_THREADS) S.base[b] = 0;
+        __syncthreads();
+        for (int64_t t0 = lo; t0 < hi; t0 += EMB_THREADS) {
+            const int64_t t = t0 + threadIdx.x;
+            const bool live = t < hi;
+            const uint32_t digit = live ? (((pass ? __ldcg(src_key + t) : emb_key(E, t)) >> shift) & mask) : EMB_BINS;
+            const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+            if (live && (peers & ((1u << lane) - 1u)) == 0) atomicAdd(&S.base[digit], (uint32_t)__popc(peers));
+        }
+        __syncthreads();
+    }
+    if (E.parts == 1) {  // the block's own counts are the totals
+        if (sorting) {
+            const uint32_t v = threadIdx.x < bins ? S.base[threadIdx.x] : 0;
+            const uint32_t x = emb_block_scan(v, S.scan);
+            if (threadIdx.x < bins) S.base[threadIdx.x] = x;
+            __syncthreads();
+        }
+    } else {
+        if (sorting)
+            for (int b = threadIdx.x; b < bins; b += EMB_THREADS) E.counts[(int64_t)b * E.parts + blockIdx.x] = S.base[b];
+        if (!emb_grid_sync(E, target)) return false;
+        for (int b = blockIdx.x * EMB_WARPS + warp; b < bins; b += gridDim.x * EMB_WARPS) {
+            uint32_t run = 0;
+            for (int p0 = 0; p0 < E.parts; p0 += 32) {
+                const int p = p0 + lane;
+                const uint32_t v = p < E.parts ? __ldcg(E.counts + (int64_t)b * E.parts + p) : 0;
+                uint32_t x = v;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+                    if (lane >= o) x += y;
+                }
+                if (p < E.parts) E.counts[(int64_t)b * E.parts + p] = run + x - v;
+                run += __shfl_sync(0xffffffffu, x, 31);
+            }
+            if (lane == 0) E.totals[b] = run;
+        }
+        if (!emb_grid_sync(E, target)) return false;
+        if (sorting) {
+            const uint32_t v = threadIdx.x < bins ? __ldcg(E.totals + threadIdx.x) : 0;
+            const uint32_t x = emb_block_scan(v, S.scan);
+            if (threadIdx.x < bins) S.base[threadIdx.x] = x + __ldcg(E.counts + (int64_t)threadIdx.x * E.parts + blockIdx.x);
+            __syncthreads();
+        }
+    }
+    if (sorting) {
+        uint32_t* dst_key = E.key[pass & 1];
+        int32_t* dst_pos = E.pos[pass & 1];
+        const int64_t tile = (int64_t)EMB_THREADS * E.kpt;
+        for (int64_t t0 = lo; t0 < hi; t0 += tile) {
+            for (int b = lane; b < bins; b += 32) S.warp_count[warp][b] = 0;
+            __syncwarp();
+            uint32_t key[EMB_MAX_KPT];
+            int32_t pos[EMB_MAX_KPT];
+            uint16_t rank[EMB_MAX_KPT];
+            const int64_t w0 = t0 + (int64_t)warp * 32 * E.kpt;  // a warp's keys are consecutive
+#pragma unroll
+            for (int k = 0; k < EMB_MAX_KPT; ++k) {
+                const int64_t t = w0 + k * 32 + lane;
+                const bool live = k < E.kpt && t < hi;
+                key[k] = live ? (pass ? __ldcg(src_key + t) : emb_key(E, t)) : 0;
+                pos[k] = live ? (pass ? __ldcg(src_pos + t) : (int32_t)t) : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < EMB_MAX_KPT; ++k) {
+                if (k < E.kpt) {
+                    const uint32_t digit = pos[k] >= 0 ? ((key[k] >> shift) & mask) : EMB_BINS;
+                    const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+                    const uint32_t below = peers & ((1u << lane) - 1u);
+                    const uint16_t old = digit < EMB_BINS ? S.warp_count[warp][digit] : 0;
+                    __syncwarp();
+                    if (digit < EMB_BINS && below == 0) S.warp_count[warp][digit] = (uint16_t)(old + __popc(peers));
+                    __syncwarp();
+                    rank[k] = (uint16_t)(old + __popc(below));
+                }
+            }
+            __syncthreads();
+            uint32_t next = 0;
+            if (threadIdx.x < bins) {  // counts of the warps before, per digit
+                uint32_t run = 0;
+                for (int w = 0; w < EMB_WARPS; ++w) {
+                    const uint16_t c = S.warp_count[w][threadIdx.x];
+                    S.warp_count[w][threadIdx.x] = (uint16_t)run;
+                    run += c;
+                }
+                next = run;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < EMB_MAX_KPT; ++k) {
+                if (k < E.kpt && pos[k] >= 0) {
+                    const uint32_t digit = (key[k] >> shift) & mask;
+                    const uint32_t at = S.base[digit] + S.warp_count[warp][digit] + rank[k];
+                    dst_key[at] = key[k];
+                    dst_pos[at] = pos[k];
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x < bins) S.base[threadIdx.x] += next;
+            __syncthreads();
+        }
+    }
+    return emb_grid_sync(E, target);
+}
+
+__device__ __forceinline__ int64_t emb_lower_bound(const uint32_t* key, int64_t n, uint32_t v) {
+    int64_t lo = 0;
+    while (n > 0) {
+        const int64_t half = n >> 1;
+        if (__ldcg(key + lo + half) < v) {
+            lo += half + 1;
+            n -= half + 1;
+        } else {
+            n = half;
+        }
+    }
+    return lo;
+}
+
+// a finished row: rounded once, or added to what the table's gradient holds and rounded once
+template <int VEC>
+__device__ __forceinline__ void emb_finish(const EmbGradArgs& E, uint32_t row, int64_t c, float* sum) {
+    const int64_t at = (int64_t)row * E.ldo + c;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] *= E.scale;
+    if (E.accumulate) {
+        float old[VEC];
+        emb_load_typed<VEC>(E.out, at, E.out_type, old);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] += old[i];
+    }
+    emb_store<VEC>(E.out, at, E.out_type, sum);
+}
+
+template <int VEC>
+__device__ __forceinline__ void emb_part(float* part_sums, int64_t share, int slot, int64_t width, int64_t c,
+                                         const float* sum) {
+    emb_store<VEC>(part_sums, (share * 2 + slot) * width + c, EMB_F32, sum);
+}
+
+template <int VEC>
+__device__ __forceinline__ void emb_zero_row(const EmbGradArgs& E, int64_t row, int lane, int lanes) {
+    float zero[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) zero[i] = 0.0f;
+    for (int64_t c = (int64_t)lane * VEC; c < E.width; c += (int64_t)lanes * VEC)
+        emb_store<VEC>(E.out, row * E.ldo + c, E.out_type, zero);
+}
+
+__device__ __forceinline__ uint32_t emb_last_key(const EmbGradArgs& E, const uint32_t* key, int64_t share) {
+    const int64_t end = (share + 1) * E.share;
+    return __ldcg(key + (end < E.tokens ? end : E.tokens) - 1);
+}
+
+// parts of the run that starts in `share` and goes on past its end; 0 where there is none
+__device__ __forceinline__ int64_t emb_run_parts(const EmbGradArgs& E, const uint32_t* key, int64_t share) {
+    const int64_t begin = share * E.share, end = begin + E.share;
+    if (end >= E.tokens) return 0;
+    const uint32_t run = __ldcg(key + end - 1), next = __ldcg(key + end);
+    const uint32_t before = begin > 0 ? __ldcg(key + begin - 1) : 0xffffffffu;
+    if (run >= (uint32_t)E.rows || next != run || before == run) return 0;
+    // its last share: few steps when it ends in the next one, as most do
+    int64_t last = share + 1;
+    if (end + E.share < E.tokens && __ldcg(key + end + E.share) == run)
+        last = (emb_lower_bound(key, E.tokens, run + 1u) - 1) / E.share;
+    return last - share + 1;
+}
+
+// parts [i0, i1) of the run that starts in `share`: part 0 is that share's tail, part i the head of the
+// i-th share after it
+template <int VEC>
+__device__ __forceinline__ void emb_sum_parts(const EmbGradArgs& E, int64_t share, int64_t c, int64_t i0, int64_t i1,
+                                              float* sum) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
+    for (int64_t i = i0; i < i1; i += 4) {
+        float x[4][VEC];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i + u < i1) {
+                const float* p = E.part_sums + ((share + i + u) * 2 + (i + u == 0 ? 1 : 0)) * E.width + c;
+                if constexpr (VEC >= 4) {
+#pragma unroll
+                    for (int q = 0; q < VEC / 4; ++q) {
+                        const float4 f = __ldcg(reinterpret_cast<const float4*>(p) + q);
+                        x[u][4 * q] = f.x, x[u][4 * q + 1] = f.y, x[u][4 * q + 2] = f.z, x[u][4 * q + 3] = f.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) x[u][k] = __ldcg(p + k);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) x[u][k] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] += (x[0][k] + x[1][k]) + (x[2][k] + x[3][k]);
+    }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbGradArgs E) {
+    __shared__ EmbSortShared S;
+    const int lane32 = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * EMB_WARPS;
+    const int64_t gwarp = (int64_t)blockIdx.x * EMB_WARPS + (threadIdx.x >> 5);
+    uint32_t target = 0;
+
+    if (E.zero_first && !(E.parts < (int)gridDim.x && (int)blockIdx.x < E.parts)) {
+        // the blocks that do not sort zero the table meanwhile (all of them where every block sorts)
+        const int64_t skip = E.parts < (int)gridDim.x ? (int64_t)E.parts * EMB_WARPS : 0;
+        for (int64_t r = gwarp - skip; r < E.rows; r += warps - skip) emb_zero_row<VEC>(E, r, lane32, 32);
+    }
+    for (int pass = 0; pass < E.passes; ++pass)
+        if (!emb_radix_pass(E, pass, target, S)) return;
+    const uint32_t* key = E.key[(E.passes & 1) ^ 1];
+    const int32_t* pos = E.pos[(E.passes & 1) ^ 1];
+    const uint32_t rows = (uint32_t)E.rows;
+
+    // ------------------------------------------------ segment sums
+    constexpr int U = sizeof(T) * VEC == 16 ? 4 : 8;  // rows in flight per worker: 64 KB or less an SM
+    const int lanes = E.lanes, lane = threadIdx.x & (lanes - 1);
+    const int64_t workers = warps * (32 / lanes);
+    const int64_t worker = ((int64_t)blockIdx.x * EMB_THREADS + threadIdx.x) / lanes;
+    const uint32_t group_mask = lanes == 32 ? 0xffffffffu : (((1u << lanes) - 1u) << (lane32 & ~(lanes - 1)));
+    const T* grad = static_cast<const T*>(E.grad);
+    const int64_t tasks = E.shares * E.tiles;
+    for (int64_t task = worker; task < tasks; task += workers) {
+        const int64_t share = task % E.shares;
+        const int64_t c = (task / E.shares) * ((int64_t)lanes * VEC) + (int64_t)lane * VEC;
+        const bool in = c < E.width;
+        const int64_t begin = share * E.share;
+        const int64_t end = begin + E.share < E.tokens ? begin + E.share : E.tokens;
+        uint32_t run = __ldcg(key + begin);
+        bool head = begin > 0 && __ldcg(key + begin - 1) == run;  // the run started in an earlier share
+        float sum[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+        for (int64_t e0 = begin; e0 < end; e0 += U) {
+            // lane j of the worker fetches entry j
+            const int64_t mine = e0 + (lane & (U - 1));
+            const uint32_t my_key = mine < end ? __ldcg(key + mine) : rows;
+            const int32_t my_pos = mine < end ? __ldcg(pos + mine) : 0;
+            const int n = end - e0 < U ? (int)(end - e0) : U;
+            EmbVec<T, VEC> x[U];  // as loaded: converted where they are added
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const uint32_t k = __shfl_sync(group_mask, my_key, j, lanes);
+                const int64_t p = __shfl_sync(group_mask, my_pos, j, lanes);
+                if (in && k < rows) {
+                    x[j] = *reinterpret_cast<const EmbVec<T, VEC>*>(grad + p * E.ldg + c);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) x[j].v[i] = emb_zero<T>();
+                }
+            }
+            const uint32_t first = __shfl_sync(group_mask, my_key, 0, lanes);
+            const uint32_t last = __shfl_sync(group_mask, my_key, U - 1, lanes);
+            if (n == U && first == run && last == run) {  // all of the same run: a tree
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    float four[U / 4];
+#pragma unroll
+                    for (int q = 0; q < U / 4; ++q)
+                        four[q] = (emb_float(x[4 * q].v[i]) + emb_float(x[4 * q + 1].v[i])) +
+                                  (emb_float(x[4 * q + 2].v[i]) + emb_float(x[4 * q + 3].v[i]));
+                    sum[i] += U == 8 ? four[0] + four[U / 4 - 1] : four[0];
+                }
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const uint32_t k = __shfl_sync(group_mask, my_key, j, lanes);
+                if (j < n) {
+                    if (k != run) {
+                        if (in && run < rows) {
+                            if (head) emb_part<VEC>(E.part_sums, share, 0, E.width, c, sum);
+                            else emb_finish<VEC>(E, run, c, sum);
+                        }
+                        run = k;
+                        head = false;
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) sum[i] += emb_float(x[j].v[i]);
+                }
+            }
+        }
+        if (in && run < rows) {
+            const bool on = end < E.tokens && __ldcg(key + end) == run;
+            if (head) emb_part<VEC>(E.part_sums, share, 0, E.width, c, sum);
+            else if (on) emb_part<VEC>(E.part_sums, share, 1, E.width, c, sum);
+            else emb_finish<VEC>(E, run, c, sum);
+        }
+    }
+    // rows that no token has
+    if (!E.accumulate && !E.zero_first) {
+        for (int64_t r0 = gwarp * 32; r0 < E.rows; r0 += warps * 32) {
+            const int64_t r = r0 + lane32;
+            bool absent = false;
+            if (r < E.rows) {
+                const int64_t at = emb_lower_bound(key, E.tokens, (uint32_t)r);
+                absent = at >= E.tokens || __ldcg(key + at) != (uint32_t)r;
+            }
+            uint32_t todo = __ballot_sync(0xffffffffu, absent);
+            while (todo) {
+                const int b = __ffs(todo) - 1;
+                todo &= todo - 1;
+                emb_zero_row<VEC>(E, r0 + b, lane32, 32);
+            }
+        }
+    }
+    if (E.shares <= 1) return;
+    if (!emb_grid_sync(E, target)) return;
+
+    // ------------------------------------------------ runs that cross shares
+    // The worker of the share where such a run starts adds its parts in order; a run of more than
+    // EMB_SERIAL_PARTS parts is left to its whole block, whose workers add a stretch of parts each.
+    __shared__ float fold[EMB_THREADS * VEC];
+    __shared__ int long_count;
+    __shared__ int64_t long_task[EMB_THREADS / 8];
+    const int groups = EMB_THREADS / lanes, group = threadIdx.x / lanes;
+    for (int64_t task0 = worker - group; task0 < tasks; task0 += workers) {
+        if (threadIdx.x == 0) long_count = 0;
+        __syncthreads();
+        int64_t count = 0;
+        if (task0 + group < tasks) {
+            count = emb_run_parts(E, key, (task0 + group) % E.shares);
+            if (count > EMB_SERIAL_PARTS && lane == 0) long_task[atomicAdd(&long_count, 1)] = task0 + group;
+        }
+        if (count > 0 && count <= EMB_SERIAL_PARTS) {
+            const int64_t share = (task0 + group) % E.shares;
+            const int64_t c = ((task0 + group) / E.shares) * ((int64_t)lanes * VEC) + (int64_t)lane * VEC;
+            if (c < E.width) {
+                float sum[VEC];
+                emb_sum_parts<VEC>(E, share, c, 0, count, sum);
+                emb_finish<VEC>(E, emb_last_key(E, key, share), c, sum);
+            }
+        }
+        __syncthreads();
+        for (int i = 0; i < long_count; ++i) {
+            const int64_t share = long_task[i] % E.shares;
+            const int64_t c = (long_task[i] / E.shares) * ((int64_t)lanes * VEC) + (int64_t)lane * VEC;
+            const int64_t parts = emb_run_parts(E, key, share);
+            const int64_t each = (parts + groups - 1) / groups;
+            const int64_t i0 = (int64_t)group * each;
+            float sum[VEC];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] = 0.0f;
+            if (c < E.width && i0 < parts) emb_sum_parts<VEC>(E, share, c, i0, i0 + each < parts ? i0 + each : parts, sum);
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) fold[k * EMB_THREADS + threadIdx.x] = sum[k];
+            __syncthreads();
+            if (group == 0 && c < E.width) {
+                for (int g = 1; g < groups; ++g) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) sum[k] += fold[k * EMB_THREADS + g * lanes + lane];
+                }
+                emb_finish<VEC>(E, emb_last_key(E, key, share), c, sum);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+// elements of a vector access: the widest of 16 bytes that width, strides and addresses allow
+static int emb_vec(int size, int64_t width, int64_t ld, const void* p, int out_size, int64_t ldo, const void* out) {
+    for (int v = 16 / size; v > 1; v /= 2) {
+        const int ob = v * out_size > 16 ? 16 : v * out_size;
+        if (width % v == 0 && ld % v == 0 && ldo % v == 0 && (uintptr_t)p % (v * size) == 0 && (uintptr_t)out % ob == 0)
+            return v;
+    }
+    return 1;
+}
+
+static int emb_size(int type) { return type == EMB_F32 ? 4 : 2; }
+
+template <typename T>
+static void (*emb_forward_kernel(int vec))(EmbArgs) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 8) return embedding_kernel<T, 8>;
+    }
+    return vec == 4 ? embedding_kernel<T, 4> : vec == 2 ? embedding_kernel<T, 2> : embedding_kernel<T, 1>;
+}
+
+template <typename T>
+static void (*emb_backward_kernel(int vec))(EmbGradArgs) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 8) return embedding_backward_kernel<T, 8>;
+    }
+    return vec == 4 ? embedding_backward_kernel<T, 4> : vec == 2 ? embedding_backward_kernel<T, 2> : embedding_backward_kernel<T, 1>;
+}
+
+struct EmbLayout {
+    int64_t barrier, counts, totals, key0, key1, pos0, pos1, parts, bytes;
+};
+
+// The plan and workspace depend on sizes and the vector width alone; the workspace is sized for any
+// vector width (the share count is bounded by the resident workers).
+static void emb_plan(int64_t tokens, int64_t rows, int64_t width, int vec, int grid_max, EmbGradArgs& E, int& grid) {
+    int key_bits = 1;
+    while ((rows >> key_bits) != 0) ++key_bits;  // keys 0 .. rows (absent tokens)
+    E.passes = (key_bits + 8) / 9;
+    E.bits = (key_bits + E.passes - 1) / E.passes;
+    // a worker's lanes: the fewest of 8, 16, 32 that cover a row, 32 for wider rows
+    const int64_t vectors = (width + vec - 1) / vec;
+    E.lanes = vectors <= 8 ? 8 : vectors <= 16 ? 16 : 32;
+    E.tiles = (int)((vectors + E.lanes - 1) / E.lanes);
+    const int64_t per_block = EMB_THREADS / E.lanes;
+    // one task (a share of the tokens, a column tile) for each resident worker
+    const int64_t most_shares = per_block * grid_max / E.tiles > 1 ? per_block * grid_max / E.tiles : 1;
+    const int64_t share = (tokens + most_shares - 1) / most_shares;
+    E.share = share < EMB_MIN_SHARE ? EMB_MIN_SHARE : (share + 7) / 8 * 8;
+    E.shares = (tokens + E.share - 1) / E.share;
+    // sorting blocks: one tile of a key per thread each at first, then more keys per thread; alone up to
+    // four keys per thread, where grid barriers would cost more than the work that they share out
+    if (tokens <= 4 * EMB_THREADS) {
+        E.parts = 1;
+        E.kpt = (int)((tokens + EMB_THREADS - 1) / EMB_THREADS);
+        E.part_tokens = tokens;
+    } else {
+        const int64_t tiles = (tokens + EMB_THREADS - 1) / EMB_THREADS;
+        const int64_t most = grid_max < 148 ? grid_max : 148;
+        int64_t kpt = (tiles + most - 1) / most;
+        E.kpt = (int)(kpt > EMB_MAX_KPT ? EMB_MAX_KPT : kpt);
+        const int64_t whole = (int64_t)EMB_THREADS * E.kpt;
+        const int64_t n = (tokens + whole - 1) / whole;  // tiles of kpt keys per thread
+        const int64_t per = (n + most - 1) / most;
+        E.part_tokens = per * whole;
+        E.parts = (int)((tokens + E.part_tokens - 1) / E.part_tokens);
+    }
+    E.zero_first = !E.accumulate && tokens <= rows / 4;
+    int64_t want = (E.shares * E.tiles + per_block - 1) / per_block;
+    if (want < E.parts) want = E.parts;
+    if (!E.accumulate) {  // blocks for the zeroed rows: 64 KB each
+        const int64_t z = (rows * width * 4) >> 16;
+        if (want < z) want = z;
+    }
+    grid = (int)(want < grid_max ? want : grid_max);
+}
+
+static EmbLayout emb_layout(int64_t tokens, int64_t width, int grid_max) {
+    EmbLayout L;
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    int64_t at = 0;
+    L.barrier = at, at += 256;
+    L.totals = at, at += up(EMB_BINS * 4);
+    L.counts = at, at += up((int64_t)EMB_BINS * 148 * 4);
+    L.key0 = at, at += up(tokens * 4);
+    L.key1 = at, at += up(tokens * 4);
+    L.pos0 = at, at += up(tokens * 4);
+    L.pos1 = at, at += up(tokens * 4);
+    // two rows of sums a share; shares * tiles is at most the resident workers (and one share more), so
+    // their columns are at most 8 per resident thread
+    const int64_t by_tokens = (tokens + EMB_MIN_SHARE - 1) / EMB_MIN_SHARE * width;
+    const int64_t by_threads = (int64_t)grid_max * EMB_THREADS * 8 + 2 * width;
+    L.parts = at, at += up((by_tokens < by_threads ? by_tokens : by_threads) * 2 * 4);
+    L.bytes = at;
+    return L;
+}
+
+// blocks of the backward kernel that one device holds at once
+static int emb_grid_max() { return 2 * sm_count(); }
+
+}  // namespace pbg
+
+using namespace pbg;
+
+extern "C" {
+
+int pbg_embedding(int64_t tokens, int64_t rows, int64_t width, const void* index, int32_t index64, const void* table,
+                  int32_t table_type, int64_t ldt, float scale, void* out, int32_t out_type, uint32_t* error, void* stream) {
+    PBG_REQUIRE(tokens >= 0 && rows >= 0 && width >= 0, "embedding: negative size");
+    PBG_REQUIRE(table_type >= 0 && table_type <= 2 && out_type >= 0 && out_type <= 2, "embedding: unknown type");
+    if (tokens == 0 || width == 0) return 0;
+    PBG_REQUIRE(index && out && error && (table || rows == 0), "embedding: null pointer");
+    PBG_REQUIRE(ldt >= width || rows <= 1, "embedding: table row stride must be >= width");
+    EmbArgs E;
+    E.tokens = tokens, E.rows = rows, E.width = width, E.ldt = ldt;
+    E.index = index, E.index64 = index64, E.table = table, E.out = out, E.out_type = out_type;
+    E.scale = scale, E.error = error;
+    const int vec = emb_vec(emb_size(table_type), width, rows > 1 ? ldt : 0, table, emb_size(out_type), width, out);
+    const int64_t vectors = (width + vec - 1) / vec;
+    // lanes of a row: a vector each up to a warp, then up to four vectors each, at most a block
+    E.log_lanes = 0;
+    while (E.log_lanes < 5 && (1LL << E.log_lanes) < vectors) ++E.log_lanes;
+    while (E.log_lanes < 8 && (4LL << E.log_lanes) < vectors) ++E.log_lanes;
+    const int64_t need = ((tokens << E.log_lanes) + 255) / 256;
+    const int64_t most = (int64_t)sm_count() * 32;
+    void (*kernel)(EmbArgs) = table_type == EMB_F32 ? emb_forward_kernel<float>(vec)
+                              : table_type == EMB_BF16 ? emb_forward_kernel<__nv_bfloat16>(vec)
+                                                       : emb_forward_kernel<__half>(vec);
+    kernel<<<(unsigned)(need < most ? need : most), 256, 0, as_stream(stream)>>>(E);
+    return launch_status("embedding");
+}
+
+int64_t pbg_embedding_backward_workspace(int64_t tokens, int64_t width) {
+    if (tokens < 0 || width < 0) return PBG_EINVAL;
+    return emb_layout(tokens, width, emb_grid_max()).bytes;
+}
+
+int pbg_embedding_backward(int64_t tokens, int64_t rows, int64_t width, const void* grad, int32_t grad_type, int64_t ldg,
+                           const void* index, int32_t index64, int64_t padding, float scale, void* out, int32_t out_type,
+                           int64_t ldo, int32_t accumulate, void* workspace, int64_t workspace_bytes, uint32_t* error,
+                           void* stream) {
+    PBG_REQUIRE(tokens >= 0 && rows >= 0 && width >= 0, "embedding_backward: negative size");
+    PBG_REQUIRE(tokens < (1LL << 31) && rows < (1LL << 31), "embedding_backward: at most 2^31 - 1 tokens and rows");
+    PBG_REQUIRE(grad_type >= 0 && grad_type <= 2 && out_type >= 0 && out_type <= 2, "embedding_backward: unknown type");
+    if (rows == 0 || width == 0) return 0;
+    PBG_REQUIRE(out && error, "embedding_backward: null pointer");
+    PBG_REQUIRE(ldo >= width || rows == 1, "embedding_backward: out row stride must be >= width");
+    PBG_REQUIRE(padding >= -1 && padding < rows, "embedding_backward: the padding index must be a row of the table");
+    cudaStream_t s = as_stream(stream);
+    if (tokens == 0) {
+        if (accumulate) return 0;
+        return cuda_status(cudaMemset2DAsync(out, (size_t)(rows == 1 ? width : ldo) * emb_size(out_type), 0,
+                                             (size_t)width * emb_size(out_type), (size_t)rows, s),
+                           "embedding_backward: zero table");
+    }
+    PBG_REQUIRE(grad && index && workspace, "embedding_backward: null pointer");
+    PBG_REQUIRE(ldg >= width || tokens == 1, "embedding_backward: gradient row stride must be >= width");
+    PBG_REQUIRE((uintptr_t)workspace % 256 == 0, "embedding_backward: workspace must be 256-byte aligned");
+    const int grid_max = emb_grid_max();
+    const EmbLayout L = emb_layout(tokens, width, grid_max);
+    PBG_REQUIRE(workspace_bytes >= L.bytes, "embedding_backward: workspace too small");
+    EmbGradArgs E;
+    E.tokens = tokens, E.rows = rows, E.width = width, E.ldg = ldg, E.ldo = ldo;
+    E.grad = grad, E.index = index, E.index64 = index64, E.padding = padding;
+    E.out = out, E.out_type = out_type, E.accumulate = accumulate, E.scale = scale, E.error = error;
+    const int vec = emb_vec(emb_size(grad_type), width, tokens > 1 ? ldg : 0, grad, emb_size(out_type), rows > 1 ? ldo : 0, out);
+    int grid = 1;
+    emb_plan(tokens, rows, width, vec, grid_max, E, grid);
+    unsigned char* w = static_cast<unsigned char*>(workspace);
+    E.barrier = reinterpret_cast<uint32_t*>(w + L.barrier);
+    E.counts = reinterpret_cast<uint32_t*>(w + L.counts);
+    E.totals = reinterpret_cast<uint32_t*>(w + L.totals);
+    E.key[0] = reinterpret_cast<uint32_t*>(w + L.key0);
+    E.key[1] = reinterpret_cast<uint32_t*>(w + L.key1);
+    E.pos[0] = reinterpret_cast<int32_t*>(w + L.pos0);
+    E.pos[1] = reinterpret_cast<int32_t*>(w + L.pos1);
+    E.part_sums = reinterpret_cast<float*>(w + L.parts);
+    void (*kernel)(EmbGradArgs) = grad_type == EMB_F32 ? emb_backward_kernel<float>(vec)
+                                  : grad_type == EMB_BF16 ? emb_backward_kernel<__nv_bfloat16>(vec)
+                                                          : emb_backward_kernel<__half>(vec);
+    if (grid == 1) {
+        kernel<<<1, EMB_THREADS, 0, s>>>(E);
+        return launch_status("embedding_backward");
+    }
+    int rc = cuda_status(cudaMemsetAsync(E.barrier, 0, 4, s), "embedding_backward: barrier");
+    if (rc) return rc;
+    void* args[] = {&E};
+    return cuda_status(cudaLaunchCooperativeKernel((const void*)kernel, dim3((unsigned)grid), dim3(EMB_THREADS), args, 0, s),
+                       "embedding_backward: cooperative launch");
+}
+
+}  // extern "C"

@@ -154,6 +154,10 @@ SIGNATURES: dict[str, tuple] = {
     "pbg_nvls_signal_bytes": (_I64, []),
     "pbg_nvls_allreduce_sum_f32": (_I32, [_I64, _P, _P, _I64, _I32, _I32, _P, _P]),
     "pbg_nvls_allreduce_sum_f32_grid": (_I32, [_I64, _P, _P, _I64, _I32, _I32, _P, _I32, _P]),
+    "pbg_embedding": (_I32, [_I64, _I64, _I64, _P, _I32, _P, _I32, _I64, ctypes.c_float, _P, _I32, _P, _P]),
+    "pbg_embedding_backward_workspace": (_I64, [_I64, _I64]),
+    "pbg_embedding_backward": (_I32, [_I64, _I64, _I64, _P, _I32, _I64, _P, _I32, _I64, ctypes.c_float, _P, _I32, _I64,
+                                      _I32, _P, _I64, _P, _P]),
     "pbg_adam_partials_size": (_I64, [_I64]),
     "pbg_adam_step": (_I32, [_I64, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P]),
 }

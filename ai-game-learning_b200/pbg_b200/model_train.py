@@ -18,7 +18,9 @@ wrapped in an autograd function whose backward is written for it:
   scores tile by tile on the tensor cores and gives dQ, dK, dV and the gradient
   of each head's score scale (so of the temperature parameter theta);
 - ``_IncidenceCombineFn`` (``pbg_incidence_combine``, the incidence residual's
-  seat sums): ``pbg_incidence_combine_backward``.
+  seat sums): ``pbg_incidence_combine_backward``;
+- ``_EmbeddingFn`` (``pbg_embedding``: rows of a table): ``pbg_embedding_backward``, sums over the
+  tokens sorted by index.
 
 The key bias and mask of the attention and the row mass of the incidence map
 come from the learner rows' ranges, not from parameters, and get no gradient.
@@ -39,6 +41,7 @@ from torch import Tensor
 
 from . import _native as N
 from ._native import NativeError, call, ptr, stream
+from .embedding import embedding, embedding_backward
 from .model import _error_word, attention, linear_ex
 
 
@@ -221,6 +224,26 @@ def incidence_combine_train(source: Tensor, overlap: Tensor, identical_scale: Te
 
     return _IncidenceCombineFn.apply(source.contiguous(), overlap.contiguous(),
                                      identical_scale.detach().float().contiguous())
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale):
+        ctx.save_for_backward(index)
+        ctx.rows, ctx.scale, ctx.dtype = table.shape[0], scale, table.dtype
+        return embedding(table, index, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (index,) = ctx.saved_tensors
+        return embedding_backward(dy, index, ctx.rows, ctx.scale, out_dtype=ctx.dtype), None, None
+
+
+def embedding_train(table: Tensor, index: Tensor, scale: float = 1.0) -> Tensor:
+    """``scale * table[index]`` in the table's type, differentiable in the table: its gradient is the sum
+    of the incoming rows of each index (``pbg_embedding_backward``)."""
+
+    return _EmbeddingFn.apply(table, index, float(scale))
 
 
 def q_scale_of(theta: Tensor) -> Tensor:
