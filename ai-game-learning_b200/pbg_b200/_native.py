@@ -158,6 +158,14 @@ SIGNATURES: dict[str, tuple] = {
     "pbg_embedding_backward_workspace": (_I64, [_I64, _I64]),
     "pbg_embedding_backward": (_I32, [_I64, _I64, _I64, _P, _I32, _I64, _P, _I32, _I64, ctypes.c_float, _P, _I32, _I64,
                                       _I32, _P, _I64, _P, _P]),
+    "pbg_orthogonalize_workspace": (_I64, [_I64, _I64, _I64]),
+    "pbg_orthogonalize": (_I32, [_I64, _I64, _I64, _P, _I32, _P, _I32, _I32, ctypes.c_float, ctypes.c_float, ctypes.c_float,
+                                 ctypes.c_double, _P, _I64, _P, _P]),
+    "pbg_muon_descriptor_bytes": (_I64, []),
+    "pbg_muon_plan_words": (_I64, [_I64]),
+    "pbg_muon_plan": (_I32, [_I64, _P, _P, _P, _P, _P, _P]),
+    "pbg_muon_step": (_I32, [_I64, _P, _P, _P, _P, _P, _P, _I32, _I32, ctypes.c_float, ctypes.c_float, ctypes.c_float,
+                             ctypes.c_double, _P, _I64, _P, _P, _P]),
     "pbg_adam_partials_size": (_I64, [_I64]),
     "pbg_adam_step": (_I32, [_I64, _P, _P, _P, _P, _P, _P, _I32, _P, _P, _P]),
 }

@@ -446,6 +446,36 @@ int pbg_adam_step(int64_t n, float *master, float *grad, float *first, float *se
                   const float *controls, int64_t *step, int32_t decoupled, double *partials,
                   double *report, void *stream);
 
+/* Orthogonalises `batch` contiguous matrices [rows, cols]: X / (|X|_F + eps), then `steps` times
+ * X <- a X + (b G + c G^2) X with G = X X^T on the short side; out contiguous like x.  Types 0 fp32, 1 bf16,
+ * 2 fp16.  fp32 accuracy inside (fp16 pairs on the tensor cores), but for bf16 output of matrices whose
+ * short side is 512 or more (errors of about half the output's rounding).  Coefficients that would let a
+ * singular value grow past 2 are refused; sides up to 65,536.  workspace: 256-byte aligned device memory
+ * of pbg_orthogonalize_workspace bytes, any contents, one per call in flight.  error (device uint32,
+ * sticky): non-zero when a bounded wait gave up. */
+int64_t pbg_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);
+int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void *x, int32_t x_type, void *out,
+                      int32_t out_type, int32_t steps, float a, float b, float c, double eps, void *workspace,
+                      int64_t workspace_bytes, uint32_t *error, void *stream);
+
+/* The transition of the matrices of a flat fp32 master by their orthogonalised momentum:
+ *   m <- mu m + (1 - mu) g / scale,   u = mu m + (1 - mu) g / scale (nesterov) or m,
+ *   w <- w (1 - lr decay) - lr adjust orthogonalize(u).
+ * pbg_muon_plan (host only) lays `count` matrices out: element offset into the flat buffers, rows, columns
+ * and adjust of each (host arrays) -> descriptors (host, count * pbg_muon_descriptor_bytes(), to be copied
+ * to the device) and plan (host, pbg_muon_plan_words(count) words; plan[0] is the workspace's bytes).
+ * pbg_muon_step takes the descriptors on the device and the plan on the host; controls (device fp32[4]):
+ * lr, mu, decay, scale.  Where any direction u is not finite nothing is changed but the matrices' gradients,
+ * which are cleared, and *skipped (device uint32) is 1, else 0. */
+int64_t pbg_muon_descriptor_bytes(void);
+int64_t pbg_muon_plan_words(int64_t count);
+int pbg_muon_plan(int64_t count, const int64_t *offset, const int64_t *rows, const int64_t *cols, const float *adjust,
+                  void *descriptors, int64_t *plan);
+int pbg_muon_step(int64_t count, const void *descriptors, const int64_t *plan, float *grad, float *momentum,
+                  float *master, const float *controls, int32_t nesterov, int32_t steps, float a, float b, float c,
+                  double eps, void *workspace, int64_t workspace_bytes, uint32_t *skipped, uint32_t *error,
+                  void *stream);
+
 /* ------------------------------------------- collision-conditioned sampler */
 
 /* Workspace (device floats) for pbg_posterior_sample_children: the parents'
