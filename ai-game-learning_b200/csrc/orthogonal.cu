@@ -20,7 +20,8 @@
 // output of matrices whose short side is at least ORTHO_SINGLE the symmetric matrices are single fp16
 // numbers (error 2^-12 that does not grow: about 8e-4 of the result's norm, where bf16 rounding alone is
 // 1.7e-3): one pass for A and B, two for X'.  The tensor cores truncate as they accumulate, a bias that
-// grows with the length of the sum, so a sum is taken from tensor memory every ORTHO_CHUNK * 64 terms
+// grows with the length of the sum (sums of 256 terms in three passes left 1.4e-5 of the result at
+// 256 x 1024), so with pairs a sum is taken from tensor memory every 64 terms, the small products first,
 // and added up in fp32 registers.
 //
 // Layout.  X, A and B live in the workspace as 128 x 64 tiles of 16 KB, hi then lo, already in the
@@ -31,20 +32,24 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <math.h>
+
 #include <algorithm>
 
 #include "pbg_common.cuh"
 
 namespace pbg {
 
-constexpr int ORTHO_CHUNK = 4;         // k-blocks of 64 summed in tensor memory
-constexpr int ORTHO_EPI_WARPS = 16;
-constexpr int ORTHO_THREADS = 64 + 32 * ORTHO_EPI_WARPS;
+constexpr int ORTHO_EPI_WARPS = 12;    // four row quarters x three 64-column parts; 16 warps in all leave 128 registers
+constexpr int ORTHO_PRODUCERS = 3;      // warps that issue bulk copies, a third of a stage's each
+constexpr int ORTHO_THREADS = 32 * (1 + ORTHO_PRODUCERS + ORTHO_EPI_WARPS);  // warp 0 issues the products
 constexpr int ORTHO_RING = 192 * 1024;  // operand stages
 constexpr int ORTHO_STAGES = 8;         // at most
 constexpr int ORTHO_BLOCK = 2048;       // an epilogue warp's staging block
-constexpr int ORTHO_SMEM = 1024 + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK;
-constexpr int ORTHO_SPAN = ORTHO_THREADS * 16;  // elements whose squares one block sums
+constexpr int ORTHO_EYE = 2048;         // 16 rows of 128 bytes: (b / c) 2^13 I in fp16 (2^13 I where c is 0), hi, and lo 32 bytes on
+constexpr int ORTHO_SMEM = 1024 + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK + ORTHO_EYE;
+constexpr int ORTHO_FLAT = 256;         // threads of the kernels around the products
+constexpr int ORTHO_SPAN = ORTHO_FLAT * 16;  // elements whose squares one block sums
 constexpr int ORTHO_TILE = 32768;       // bytes of a 128 x 64 tile, hi and lo
 constexpr uint32_t ORTHO_WAIT_TRIES = 1u << 24;
 constexpr float ORTHO_SX = 16384.0f, ORTHO_SA = 8192.0f, ORTHO_SB = 4096.0f;
@@ -85,7 +90,7 @@ struct OrthoArgs {
     unsigned char* tiles;
     uint32_t* barrier;
     uint32_t* error;
-    int phase0, phase1;
+    int aligned;  // vector access to the flat buffers, x and out: 16 bytes at multiples of four elements
 };
 
 // ------------------------------------------------------------ tcgen05, mbarrier and bulk-copy access
@@ -126,22 +131,29 @@ __device__ __forceinline__ void or_bulk_load(uint32_t dst, const void* src, uint
                  : "memory");
 }
 // 128-byte-swizzled operand: K-major (rows of 128 bytes, 8-row atoms 1024 bytes apart), or MN-major (64
-// columns of 8 k-rows an atom, the next k-rows 1024 bytes on, the next 64 columns `lbo` bytes on)
-__device__ __forceinline__ uint64_t or_desc(uint32_t addr, uint32_t lbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
-}
+// columns of 8 k-rows an atom, the next k-rows 1024 bytes on, the next 64 columns `lbo` bytes on).  The low
+// word of the descriptor, whose high word is the same for both.
+__device__ __forceinline__ uint32_t or_desc(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 // kind::f16: fp16 x fp16 -> fp32, M 128, A K-major, B K-major or MN-major
 __device__ __forceinline__ uint32_t or_idesc(int n, int mn_major) {
     return (1u << 4) | ((uint32_t)mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void or_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void or_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29);
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %5};\n\t"
+        "mov.b64 db, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(high)
         : "memory");
+}
+// one lane of a converged warp; the compiler knows that it runs alone and keeps descriptors in uniform registers
+__device__ __forceinline__ bool or_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 __device__ __forceinline__ void or_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -192,8 +204,12 @@ __device__ __forceinline__ int64_t or_find(const OrthoArgs& O, int64_t t, int64_
 
 __host__ __device__ __forceinline__ int or_mb(int m) { return (m + 127) >> 7; }
 __host__ __device__ __forceinline__ int or_b64(int v) { return (v + 63) >> 6; }
-__host__ __device__ __forceinline__ int64_t or_x_bytes(int m, int n) { return (int64_t)or_mb(m) * or_b64(n) * ORTHO_TILE; }
-__host__ __device__ __forceinline__ int64_t or_a_bytes(int m) { return (int64_t)or_mb(m) * 2 * or_mb(m) * ORTHO_TILE; }
+// tiles from one row block to the next, odd: the blocks that read one column of tiles at a time would
+// otherwise meet in a few memory slices where the pitch is a power of two
+__host__ __device__ __forceinline__ int or_pitch_x(int n) { return or_b64(n) | 1; }
+__host__ __device__ __forceinline__ int or_pitch_a(int m) { return 2 * or_mb(m) | 1; }
+__host__ __device__ __forceinline__ int64_t or_x_bytes(int m, int n) { return (int64_t)or_mb(m) * or_pitch_x(n) * ORTHO_TILE; }
+__host__ __device__ __forceinline__ int64_t or_a_bytes(int m) { return (int64_t)or_mb(m) * or_pitch_a(m) * ORTHO_TILE; }
 // symmetric tiles of row block i: from column 128 i on
 __host__ __device__ __forceinline__ int or_sym_row(int m, int i, int bn) { return (or_b64(m) * 64 - i * 128 + bn - 1) / bn; }
 
@@ -226,52 +242,76 @@ __device__ __forceinline__ OrthoDirection or_controls(const OrthoArgs& O) {
     return k;
 }
 
-struct OrthoShared {
-    uint64_t full[ORTHO_STAGES], empty[ORTHO_STAGES], acc_full[2], acc_empty[2], done;
-    double reduce[ORTHO_THREADS / 32];
-    double norm;
-    int64_t norm_of;
-    uint32_t tmem;
-    int ok;
-    volatile int abort_flag;
-};
-
-__device__ __forceinline__ double or_block_sum(double v, OrthoShared& S) {
+// the same sum in every thread, in an order that the block's size alone determines
+__device__ __forceinline__ double or_block_sum(double v) {
+    __shared__ double part[ORTHO_FLAT / 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) S.reduce[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
     double sum = 0.0;
-    for (int w = 0; w < ORTHO_THREADS / 32; ++w) sum += S.reduce[w];
+#pragma unroll
+    for (int w = 0; w < ORTHO_FLAT / 32; ++w) sum += part[w];
     return sum;
 }
 
-// squares of each matrix's direction, a sum per span (fp64: no overflow or underflow at any fp32 scale)
-__device__ void or_phase_squares(const OrthoArgs& O, OrthoShared& S) {
+// eight consecutive elements i .. i + 7, zeros from `live` on
+__device__ __forceinline__ void or_load8(const void* p, int type, int64_t i, bool vector, int live, float* v) {
+    if (vector && live >= 8) {
+        if (type == 0) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
+            const float4 g = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i) + 1);
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w, v[4] = g.x, v[5] = g.y, v[6] = g.z, v[7] = g.w;
+        } else {
+            const uint2 f = __ldcg(reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i));
+            const uint2 g = __ldcg(reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i) + 1);
+            const uint32_t w[4] = {f.x, f.y, g.x, g.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 h = type == 1 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]))
+                                           : __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                v[2 * e] = h.x, v[2 * e + 1] = h.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < live ? or_load(p, type, i + e) : 0.0f;
+    }
+}
+
+// Squares of each matrix's direction, a block and a sum per span (fp64: no overflow or underflow at any
+// fp32 scale).
+__global__ void __launch_bounds__(ORTHO_FLAT) orthogonalize_squares_kernel(const __grid_constant__ OrthoArgs O) {
     const OrthoDirection k = or_controls(O);
-    for (int64_t t = blockIdx.x; t < O.spans; t += gridDim.x) {
-        const OrthoDesc d = or_get(O, or_find(O, t, &OrthoDesc::span0, O.one_span));
-        const int64_t total = (int64_t)d.m * d.n;
-        const int64_t begin = (t - d.span0) * ORTHO_SPAN;
-        const int64_t end = begin + ORTHO_SPAN < total ? begin + ORTHO_SPAN : total;
-        double sum = 0.0;
-        bool bad = false;
-        for (int64_t i = begin + threadIdx.x; i < end; i += ORTHO_THREADS) {
-            float u;
-            if (O.x) {
-                u = or_load(O.x, O.x_type, d.src + i);
-            } else {
-                const float g = O.grad[d.src + i];
-                u = or_direction(k, g, or_momentum(k, g, O.momentum[d.src + i]));
+    const int64_t t = blockIdx.x;
+    const OrthoDesc d = or_get(O, or_find(O, t, &OrthoDesc::span0, O.one_span));
+    const int64_t total = (int64_t)d.m * d.n;
+    const int64_t begin = (t - d.span0) * ORTHO_SPAN;
+    const bool vector = O.aligned && d.src % 4 == 0;
+    double sum = 0.0;
+    bool bad = false;
+    float g[2][8], m[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int64_t i = begin + (h * ORTHO_FLAT + (int)threadIdx.x) * 8;
+        const int live = i < total ? (int)(total - i < 8 ? total - i : 8) : 0;
+        or_load8(O.x ? O.x : O.grad, O.x ? O.x_type : 0, d.src + i, vector, live, g[h]);
+        if (!O.x) or_load8(O.momentum, 0, d.src + i, vector, live, m[h]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float u = g[h][e];
+            if (!O.x) {
+                u = or_direction(k, u, or_momentum(k, u, m[h][e]));
                 bad |= !isfinite(u);
             }
             sum += (double)u * (double)u;
         }
-        if (bad) atomicExch(O.bad, 1u);
-        sum = or_block_sum(sum, S);
-        if (threadIdx.x == 0) O.sums[t] = sum;
-    }
+    if (bad) atomicExch(O.bad, 1u);
+    sum = or_block_sum(sum);
+    if (threadIdx.x == 0) O.sums[t] = sum;
 }
 
 __device__ __forceinline__ void or_split(float v, __half& hi, __half& lo) {
@@ -279,61 +319,75 @@ __device__ __forceinline__ void or_split(float v, __half& hi, __half& lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
-// the normalised direction as tiles of pairs (and the momentum, where there is one)
-__device__ void or_phase_convert(const OrthoArgs& O, OrthoShared& S) {
+// The normalised direction as tiles of pairs, a block per tile (and the momentum, where there is one).  In
+// the transition a direction that is not finite clears the matrices' gradients instead.
+__global__ void __launch_bounds__(ORTHO_FLAT) orthogonalize_convert_kernel(const __grid_constant__ OrthoArgs O) {
     const OrthoDirection k = or_controls(O);
-    if (threadIdx.x == 0) S.norm_of = -1;
-    __syncthreads();
-    for (int64_t t = blockIdx.x; t < O.convs; t += gridDim.x) {
-        const int64_t which = or_find(O, t, &OrthoDesc::conv0, O.one_conv);
-        const OrthoDesc d = or_get(O, which);
-        const int64_t total = (int64_t)d.m * d.n;
-        if (S.norm_of != which) {
-            const int64_t spans = (total + ORTHO_SPAN - 1) / ORTHO_SPAN;
-            double sum = 0.0;
-            for (int64_t i = threadIdx.x; i < spans; i += ORTHO_THREADS) sum += __ldcg(O.sums + d.span0 + i);
-            sum = or_block_sum(sum, S);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                S.norm = sqrt(sum);
-                S.norm_of = which;
-            }
-            __syncthreads();
+    const int64_t t = blockIdx.x;
+    const OrthoDesc d = or_get(O, or_find(O, t, &OrthoDesc::conv0, O.one_conv));
+    const int nb = or_b64(d.n);
+    const int local = (int)(t - d.conv0);
+    const int ti = local / nb, tj = local % nb;
+    const bool clear = !O.x && *O.bad != 0u;
+    double sum = 0.0;
+    const int64_t spans = ((int64_t)d.m * d.n + ORTHO_SPAN - 1) / ORTHO_SPAN;
+    for (int64_t i = threadIdx.x; i < spans; i += ORTHO_FLAT) sum += O.sums[d.span0 + i];
+    const double wide = (double)ORTHO_SX / (sqrt(or_block_sum(sum)) + O.eps);
+    const float scale = (float)wide;
+    const bool plain = scale < 1.0e30f;  // beyond it belongs to a direction of (sub)normal smallness: in fp64 then
+    unsigned char* tile = O.tiles + d.ws + ((int64_t)ti * or_pitch_x(d.n) + tj) * ORTHO_TILE;
+    const bool vector = O.aligned && d.src % 4 == 0 && d.n % 4 == 0;
+    // 1,024 chunks of 8 columns, four a thread.  Lanes run along rows of the stored matrix: 8 chunks of a row,
+    // or (transposed) 32 rows of a chunk.
+#pragma unroll 2
+    for (int q = threadIdx.x; q < 1024; q += ORTHO_FLAT) {
+        const int r = d.tall ? q & 127 : q >> 3, chunk = d.tall ? q >> 7 : q & 7;
+        const int row = ti * 128 + r, col = tj * 64 + chunk * 8;
+        const int live = row < d.m ? (d.n - col < 8 ? d.n - col : 8) : 0;
+        const int64_t i = d.src + (d.tall ? (int64_t)col * d.m + row : (int64_t)row * d.n + col);
+        const int64_t next = d.tall ? d.m : 1;
+        if (clear) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < live) O.grad[i + e * next] = 0.0f;
+            continue;
         }
-        const float scale = (float)((double)ORTHO_SX / (S.norm + O.eps));
-        // a scale beyond fp32 belongs to a direction of (sub)normal smallness: taken in fp64 then
-        const bool plain = scale < 1.0e30f;
-        const double wide = (double)ORTHO_SX / (S.norm + O.eps);
-        const int nb = or_b64(d.n);
-        const int local = (int)(t - d.conv0);
-        const int row0 = (local / nb) * 128, col0 = (local % nb) * 64;
-        unsigned char* tile = O.tiles + d.ws + (int64_t)local * ORTHO_TILE;
-        for (int q = threadIdx.x; q < 1024; q += ORTHO_THREADS) {
-            const int r = q >> 3, chunk = q & 7;
-            const int row = row0 + r, col = col0 + chunk * 8;
-            __align__(16) __half hi[8];
-            __align__(16) __half lo[8];
+        const void* src = O.x ? O.x : O.grad;
+        const int type = O.x ? O.x_type : 0;
+        float g[8], m[8];
+        if (d.tall) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                float u = 0.0f;
-                if (row < d.m && col + e < d.n) {
-                    const int64_t i = d.src + (d.tall ? (int64_t)(col + e) * d.m + row : (int64_t)row * d.n + col + e);
-                    if (O.x) {
-                        u = or_load(O.x, O.x_type, i);
-                    } else {
-                        const float g = O.grad[i];
-                        const float m = or_momentum(k, g, O.momentum[i]);
-                        O.momentum[i] = m;
-                        u = or_direction(k, g, m);
-                    }
-                    u = plain ? u * scale : (float)((double)u * wide);
-                }
-                or_split(u, hi[e], lo[e]);
+                g[e] = e < live ? or_load(src, type, i + e * next) : 0.0f;
+                if (!O.x) m[e] = e < live ? O.momentum[i + e * next] : 0.0f;
             }
-            const int at = r * 128 + ((chunk ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4*>(tile + at) = *reinterpret_cast<uint4*>(hi);
-            *reinterpret_cast<uint4*>(tile + 16384 + at) = *reinterpret_cast<uint4*>(lo);
+        } else {
+            or_load8(src, type, i, vector, live, g);
+            if (!O.x) or_load8(O.momentum, 0, i, vector, live, m);
         }
+        if (!O.x) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m[e] = or_momentum(k, g[e], m[e]);
+                g[e] = or_direction(k, g[e], m[e]);
+            }
+            if (!d.tall && vector && live >= 8) {
+                float4* p = reinterpret_cast<float4*>(O.momentum + i);
+                p[0] = make_float4(m[0], m[1], m[2], m[3]);
+                p[1] = make_float4(m[4], m[5], m[6], m[7]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < live) O.momentum[i + e * next] = m[e];
+            }
+        }
+        __align__(16) __half hi[8];
+        __align__(16) __half lo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) or_split(e < live ? (plain ? g[e] * scale : (float)((double)g[e] * wide)) : 0.0f, hi[e], lo[e]);
+        const int at = r * 128 + ((chunk ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(tile + at) = *reinterpret_cast<uint4*>(hi);
+        *reinterpret_cast<uint4*>(tile + 16384 + at) = *reinterpret_cast<uint4*>(lo);
     }
 }
 
@@ -341,346 +395,286 @@ __device__ void or_phase_convert(const OrthoArgs& O, OrthoShared& S) {
 
 enum { OR_GRAM = 0, OR_SQUARE = 1, OR_UPDATE = 2 };
 
-// one output tile: row block, first column, width, and where its operands lie
+// one output tile: its matrix, row block, first column and width
 struct OrthoTile {
-    OrthoDesc d;
-    int i, c0, width, kblocks;
-    const unsigned char* a;  // tiles of the row operand: k-block kb at a + kb * ORTHO_TILE
-    const unsigned char* b;  // the other operand's tiles
-    int64_t b_row;           // bytes between its row blocks
-    unsigned char *x_next, *amat, *bmat;
+    int which, i, c0, width;
 };
 
-__device__ __forceinline__ OrthoTile or_tile(const OrthoArgs& O, int kind, int step, int64_t t) {
+__device__ __forceinline__ OrthoTile or_tile(const OrthoArgs& O, int kind, int64_t t) {
     OrthoTile T;
     const bool sym = kind != OR_UPDATE;
-    T.d = or_get(O, sym ? or_find(O, t, &OrthoDesc::sym0, O.one_sym) : or_find(O, t, &OrthoDesc::upd0, O.one_upd));
-    const int m64 = or_b64(T.d.m), nb = or_b64(T.d.n), mb = or_mb(T.d.m);
-    const int64_t xb = or_x_bytes(T.d.m, T.d.n), ab = or_a_bytes(T.d.m);
-    unsigned char* base = O.tiles + T.d.ws;
-    unsigned char* x = base + (step & 1 ? xb : 0);
-    T.x_next = base + (step & 1 ? 0 : xb);
-    T.amat = base + 2 * xb;
-    T.bmat = T.amat + ab;
-    int local = (int)(t - (sym ? T.d.sym0 : T.d.upd0));
+    const int64_t w = sym ? or_find(O, t, &OrthoDesc::sym0, O.one_sym) : or_find(O, t, &OrthoDesc::upd0, O.one_upd);
+    T.which = (int)w;
+    const int64_t first = O.list ? (sym ? O.list[w].sym0 : O.list[w].upd0) : w * (sym ? O.one_sym : O.one_upd);
+    const int m = O.list ? O.list[w].m : O.one.m, n = O.list ? O.list[w].n : O.one.n;
+    int local = (int)(t - first);
     if (sym) {
         T.i = 0;
-        for (int n; local >= (n = or_sym_row(T.d.m, T.i, O.bn_sym)); ++T.i) local -= n;
+        for (int r; local >= (r = or_sym_row(m, T.i, O.bn_sym)); ++T.i) local -= r;
         T.c0 = T.i * 128 + local * O.bn_sym;
-        T.width = min(O.bn_sym, m64 * 64 - T.c0);
+        T.width = min(O.bn_sym, or_b64(m) * 64 - T.c0);
     } else {
-        const int across = (nb * 64 + O.bn_upd - 1) / O.bn_upd;
+        const int across = (or_b64(n) * 64 + O.bn_upd - 1) / O.bn_upd;
         T.i = local / across;
         T.c0 = (local % across) * O.bn_upd;
-        T.width = min(O.bn_upd, nb * 64 - T.c0);
-    }
-    if (kind == OR_GRAM) {
-        T.kblocks = nb;
-        T.b_row = (int64_t)nb * ORTHO_TILE;
-        T.a = x + T.i * T.b_row;
-        T.b = x;
-    } else if (kind == OR_SQUARE) {
-        T.kblocks = m64;
-        T.b_row = (int64_t)2 * mb * ORTHO_TILE;
-        T.a = T.amat + T.i * T.b_row;
-        T.b = T.amat;
-    } else {
-        T.kblocks = m64;
-        T.b_row = (int64_t)nb * ORTHO_TILE;
-        T.a = T.bmat + (int64_t)T.i * 2 * mb * ORTHO_TILE;
-        T.b = x;
+        T.width = min(O.bn_upd, or_b64(n) * 64 - T.c0);
     }
     return T;
 }
 
-// A thread's 64 finished values of one row as a 128 x 64 tile's row, hi or lo, by way of the warp's staging
-// block, 16 rows at a time (rows of 128 bytes are contiguous in the tile, so each half is one bulk copy).
-__device__ __forceinline__ void or_store_rows(uint32_t blk, unsigned char* dst, int lane, const float* v, bool low) {
+__device__ __forceinline__ int or_kblocks(const OrthoArgs& O, int kind, const OrthoTile& T) {
+    if (kind == OR_SQUARE && O.c == 0.0f) return T.width >> 6;  // no square: only the tile's own columns of A
+    if (O.list) return kind == OR_GRAM ? or_b64(O.list[T.which].n) : or_b64(O.list[T.which].m);
+    return kind == OR_GRAM ? or_b64(O.one.n) : or_b64(O.one.m);
+}
+
+// where a matrix's tiles lie at a step
+struct OrthoPlace {
+    int64_t x_row, a_row;  // bytes of a row block
+    unsigned char *x, *x_next, *a, *b;
+};
+__device__ __forceinline__ OrthoPlace or_place(const OrthoArgs& O, const OrthoDesc& d, int step) {
+    OrthoPlace L;
+    const int64_t xb = or_x_bytes(d.m, d.n);
+    L.x_row = (int64_t)or_pitch_x(d.n) * ORTHO_TILE;
+    L.a_row = (int64_t)or_pitch_a(d.m) * ORTHO_TILE;
+    unsigned char* base = O.tiles + d.ws;
+    L.x = base + (step & 1 ? xb : 0);
+    L.x_next = base + (step & 1 ? 0 : xb);
+    L.a = base + 2 * xb;
+    L.b = L.a + or_a_bytes(d.m);
+    return L;
+}
+
+// A thread's 64 finished values of one row as a row of a 128 x 64 tile, hi then lo, by way of the warp's
+// staging blocks of 16 rows (rows of 128 bytes are contiguous in the tile, so each block is one bulk copy).
+// `blocks` of them 4 ORTHO_BLOCK apart belong to the warp: those of the warps without columns are used too.
+__device__ __forceinline__ void or_store_rows(uint32_t blk, int blocks, unsigned char* dst, int lane, float* v, int parts) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+#pragma unroll 1
+    for (int round = 0; round < 2 * parts; ++round) {
+        {
+            const bool low = round >= 2;
+            if (round >= blocks) {
+                if (lane == 0) {
+                    if (blocks == 1) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                }
+                __syncwarp();
+            }
+            const uint32_t at = blk + (uint32_t)(round % blocks) * (4u * ORTHO_BLOCK);
+            if ((lane >> 4) == (round & 1)) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
-        if ((lane >> 4) == half) {
+                for (int q = 0; q < 8; ++q) {
+                    uint32_t w[4];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x0 = v[8 * q + 2 * j], x1 = v[8 * q + 2 * j + 1];
-                    __half2 h = __floats2half2_rn(x0, x1);
-                    if (low) {
-                        const float2 f = __half22float2(h);
-                        h = __floats2half2_rn(x0 - f.x, x1 - f.y);
+                    for (int j = 0; j < 4; ++j) {
+                        // opaque, or the conversions of every round would be made and kept before the first
+                        asm volatile("" : "+f"(v[8 * q + 2 * j]), "+f"(v[8 * q + 2 * j + 1]));
+                        const float x0 = v[8 * q + 2 * j], x1 = v[8 * q + 2 * j + 1];
+                        __half2 h = __floats2half2_rn(x0, x1);
+                        if (low) {
+                            const float2 f = __half22float2(h);
+                            h = __floats2half2_rn(x0 - f.x, x1 - f.y);
+                        }
+                        w[j] = *reinterpret_cast<uint32_t*>(&h);
                     }
-                    w[j] = *reinterpret_cast<uint32_t*>(&h);
-                }
-                const uint32_t addr = blk + (uint32_t)(lane & 15) * 128u + (uint32_t)((q ^ (lane & 7)) << 4);
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                             "r"(w[3])
-                             : "memory");
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + half * 2048), "r"(blk),
-                         "r"(2048u)
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        }
-    }
-}
-
-__device__ __forceinline__ void or_write_out(const OrthoArgs& O, const OrthoDesc& d, float lr, float shrink, int64_t i,
-                                             float v) {
-    if (!O.x) {
-        O.master[i] = O.master[i] * shrink - lr * d.adjust * v;
-    } else if (O.out_type == 0) {
-        static_cast<float*>(O.out)[i] = v;
-    } else if (O.out_type == 1) {
-        static_cast<__nv_bfloat16*>(O.out)[i] = __float2bfloat16_rn(v);
-    } else {
-        static_cast<__half*>(O.out)[i] = __float2half_rn(v);
-    }
-}
-
-// what an epilogue warp does with its 32 rows x 64 columns (rows row0 + lane, column block cb of 64)
-__device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, bool last, const OrthoTile& T, int row, int cb,
-                                          uint32_t blk, int lane, float* v) {
-    const int m64 = or_b64(T.d.m), mb = or_mb(T.d.m), nb = or_b64(T.d.n);
-    const int r0 = row - lane;  // multiple of 32
-    if (kind != OR_UPDATE) {
-        unsigned char* dst = kind == OR_GRAM ? T.amat : T.bmat;
-        const int64_t row_bytes = (int64_t)2 * mb * ORTHO_TILE;
-        const bool mirror = cb * 64 >= (T.i + 1) * 128;
-        // the mirrored place of (row, cb * 64 + j): tile row block cb / 2, column block row / 64
-        const int64_t mirror0 = (int64_t)(cb >> 1) * row_bytes + (int64_t)(row >> 6) * ORTHO_TILE;
-        const int mc = row & 63;
-        if (kind == OR_GRAM) {
-#pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] *= ORTHO_SA / (ORTHO_SX * ORTHO_SX);
-        } else {
-            const float fa = O.a * ORTHO_SB, fb = O.b * (ORTHO_SB / ORTHO_SA), fc = O.c * (ORTHO_SB / (ORTHO_SA * ORTHO_SA));
-            const unsigned char* am = T.amat + mirror0;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                // A(col, row) = A(row, col): lanes read along a row
-                const int mr = (cb & 1) * 64 + j;
-                const int at = mr * 128 + (((mc >> 3) ^ (mr & 7)) << 4) + (mc & 7) * 2;
-                float x = 0.0f;  // rows past the last 64-row block are nobody's operand
-                if (row < m64 * 64) x = __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(am + at))));
-                if (O.precise && row < m64 * 64)
-                    x += __half2float(__ushort_as_half(__ldcg(reinterpret_cast<const unsigned short*>(am + 16384 + at))));
-                v[j] = fmaf(fc, v[j], fb * x) + (row == cb * 64 + j ? fa : 0.0f);
-            }
-        }
-        unsigned char* tile = dst + T.i * row_bytes + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
-        or_store_rows(blk, tile, lane, v, false);
-        if (O.precise) or_store_rows(blk, tile + 16384, lane, v, true);
-        if (mirror) {
-            unsigned char* mt = dst + mirror0;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) {
-                const int mr = (cb & 1) * 64 + j;
-                const int at = mr * 128 + (((mc >> 3) ^ (mr & 7)) << 4) + (mc & 7) * 2;
-                __half hi, lo;
-                or_split(v[j], hi, lo);
-                *reinterpret_cast<__half*>(mt + at) = hi;
-                if (O.precise) *reinterpret_cast<__half*>(mt + 16384 + at) = lo;
-            }
-        }
-    } else if (!last) {
-#pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] *= 1.0f / ORTHO_SB;
-        unsigned char* tile = T.x_next + ((int64_t)T.i * nb + cb) * ORTHO_TILE + (r0 & 127) * 128;
-        or_store_rows(blk, tile, lane, v, false);
-        or_store_rows(blk, tile + 16384, lane, v, true);
-    } else {
-        const float lr = O.x ? 0.0f : O.controls[0];
-        const float shrink = O.x ? 1.0f : 1.0f - lr * O.controls[2];
-        if (T.d.tall) {
-            if (row < T.d.m) {
-#pragma unroll
-                for (int j = 0; j < 64; ++j) {
-                    const int col = cb * 64 + j;
-                    if (col < T.d.n)
-                        or_write_out(O, T.d, lr, shrink, T.d.src + (int64_t)col * T.d.m + row, v[j] * (1.0f / (ORTHO_SB * ORTHO_SX)));
-                }
-            }
-        } else {
-            // 32 rows x 16 columns at a time by way of the staging block, so that lanes write along rows
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t addr = blk + (uint32_t)lane * 64u + (uint32_t)((q ^ ((lane >> 1) & 3)) << 4);
-                    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[16 * p + 4 * q]),
-                                 "f"(v[16 * p + 4 * q + 1]), "f"(v[16 * p + 4 * q + 2]), "f"(v[16 * p + 4 * q + 3])
+                    const uint32_t addr = at + (uint32_t)(lane & 15) * 128u + (uint32_t)((q ^ (lane & 7)) << 4);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                                 "r"(w[3])
                                  : "memory");
                 }
-                __syncwarp();
-#pragma unroll
-                for (int it = 0; it < 16; ++it) {
-                    const int rr = it * 2 + (lane >> 4), cc = lane & 15;
-                    float x;
-                    const uint32_t addr =
-                        blk + (uint32_t)rr * 64u + (uint32_t)(((cc >> 2) ^ ((rr >> 1) & 3)) << 4) + (uint32_t)(cc & 3) * 4u;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr) : "memory");
-                    const int col = cb * 64 + p * 16 + cc;
-                    if (r0 + rr < T.d.m && col < T.d.n)
-                        or_write_out(O, T.d, lr, shrink, T.d.src + (int64_t)(r0 + rr) * T.d.n + col, x * (1.0f / (ORTHO_SB * ORTHO_SX)));
-                }
-                __syncwarp();
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::
+                                 "l"(dst + (low ? 16384 : 0) + (round & 1) * 2048), "r"(at), "r"(2048u)
+                             : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
         }
     }
 }
 
-struct OrthoPipe {
-    uint32_t full, empty;  // parity of each stage's next use, a bit a stage
-    uint32_t acc;          // accumulators used
+struct OrthoOut {
+    float lr, shrink;  // of the transition
 };
 
-__device__ void or_phase_product(const OrthoArgs& O, OrthoShared& S, OrthoPipe& P, uint32_t ring, int kind, int step) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
-    const int bn = kind == OR_UPDATE ? O.bn_upd : O.bn_sym;
-    const int pa = O.precise ? 2 : 1, pb = O.precise || kind == OR_UPDATE ? 2 : 1;
-    const uint32_t a_bytes = pa * 16384u, b_part = (uint32_t)bn * 128u;
-    const uint32_t stage_bytes = a_bytes + pb * b_part;
-    const int stages = min(ORTHO_STAGES, (int)(ORTHO_RING / stage_bytes));
-    if (warp == 0) {
-        if (lane == 0) {
-            asm volatile("fence.proxy.async;" ::: "memory");
-            bool ok = true;
-            int s = 0;
-            uint32_t used = 0;
-            for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const OrthoTile T = or_tile(O, kind, step, t);
-                const int pieces = T.width >> 6;
-                for (int kb = 0; kb < T.kblocks; ++kb) {
-                    if (!or_wait(or_smem(&S.empty[s]), ((P.empty >> s) & 1u) ^ 1u, &S.abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    P.empty ^= 1u << s;
-                    used |= 1u << s;
-                    const uint32_t bar = or_smem(&S.full[s]), sa = ring + s * stage_bytes, sb = sa + a_bytes;
-                    or_expect_tx(bar, a_bytes + (uint32_t)(pb * pieces) * 8192u);
-                    or_bulk_load(sa, T.a + (int64_t)kb * ORTHO_TILE, a_bytes, bar);
-                    for (int p = 0; p < pieces; ++p) {
-                        // 64 rows of k-block kb (K-major), or 64 k-rows of a column block (MN-major)
-                        const int cb = (T.c0 >> 6) + p;
-                        const unsigned char* src =
-                            kind == OR_UPDATE ? T.b + (kb >> 1) * T.b_row + (int64_t)cb * ORTHO_TILE + (kb & 1) * 8192
-                                              : T.b + (cb >> 1) * T.b_row + (int64_t)kb * ORTHO_TILE + (cb & 1) * 8192;
-                        or_bulk_load(sb + p * 8192u, src, 8192u, bar);
-                        if (pb == 2) or_bulk_load(sb + b_part + p * 8192u, src + 16384, 8192u, bar);
-                    }
-                    if (++s == stages) s = 0;
-                }
-            }
-            if (!ok) {
-                atomicCAS(O.error, 0u, 1u);
-                S.abort_flag = 1;
-            }
-            if (S.abort_flag) {  // every copy under way lands before the block can end
-                for (int q = 0; q < stages; ++q)
-                    for (uint32_t i = 0; ((used >> q) & 1u) && i < ORTHO_WAIT_TRIES &&
-                                         !or_try_wait(or_smem(&S.full[q]), ((P.empty >> q) & 1u) ^ 1u); ++i) {
-                    }
-            }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = true;
-            int s = 0;
-            const int mn = kind == OR_UPDATE;
-            const uint32_t b_step = mn ? 2048u : 32u, lbo = mn ? 8192u : 16u;
-            for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-                const OrthoTile T = or_tile(O, kind, step, t);
-                const uint32_t idesc = or_idesc(T.width, mn);
-                for (int k0 = 0; ok && k0 < T.kblocks; k0 += ORTHO_CHUNK, ++P.acc) {
-                    const uint32_t b = P.acc & 1u;
-                    if (!or_wait(or_smem(&S.acc_empty[b]), ((P.acc >> 1) & 1u) ^ 1u, &S.abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    or_fence_after();
-                    const uint32_t d = S.tmem + b * 256u;
-                    const int k1 = min(k0 + ORTHO_CHUNK, T.kblocks);
-                    for (int kb = k0; kb < k1; ++kb) {
-                        if (!or_wait(or_smem(&S.full[s]), (P.full >> s) & 1u, &S.abort_flag)) {
-                            ok = false;
-                            break;
-                        }
-                        P.full ^= 1u << s;
-                        or_fence_after();
-                        const uint32_t sa = ring + s * stage_bytes, sb = sa + a_bytes;
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) {
-                            const uint64_t ah = or_desc(sa + ks * 32, 16), bh = or_desc(sb + ks * b_step, lbo);
-                            if (pa == 2) or_mma(d, or_desc(sa + 16384 + ks * 32, 16), bh, idesc, kb > k0 || ks > 0);
-                            if (pb == 2) or_mma(d, ah, or_desc(sb + b_part + ks * b_step, lbo), idesc, kb > k0 || ks > 0 || pa == 2);
-                            or_mma(d, ah, bh, idesc, kb > k0 || ks > 0 || pb == 2);
-                        }
-                        or_commit(or_smem(&S.empty[s]));
-                        if (++s == stages) s = 0;
-                    }
-                    if (ok) or_commit(or_smem(&S.acc_full[b]));
-                }
-            }
-            if (!ok) {
-                atomicCAS(O.error, 0u, 2u);
-                S.abort_flag = 1;
-            }
+// N finished values (4: aligned) at element i of the output, or one into the master
+template <int N>
+__device__ __forceinline__ void or_write_out(const OrthoArgs& O, const OrthoOut& k, int64_t i, float* v) {
+    if (!O.x) {
+        float* p = O.master + i;
+        *p = *p * k.shrink - k.lr * v[0];
+    } else if (O.out_type == 0) {
+        float* p = static_cast<float*>(O.out) + i;
+        if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        else *p = v[0];
+    } else if (O.out_type == 1) {
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(O.out) + i;
+        if constexpr (N == 4) {
+            __nv_bfloat162 w[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
+        } else {
+            *p = __float2bfloat16_rn(v[0]);
         }
     } else {
-        const int e = warp - 2, quad = warp & 3, part = e >> 2;
-        const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * ORTHO_BLOCK;
-        const bool last = kind == OR_UPDATE && step == O.steps - 1;
-        bool ok = true;
-        for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const OrthoTile T = or_tile(O, kind, step, t);
-            const bool mine = part < (T.width >> 6);
-            float v[64];
-#pragma unroll
-            for (int j = 0; j < 64; ++j) v[j] = 0.0f;
-            for (int k0 = 0; k0 < T.kblocks; k0 += ORTHO_CHUNK, ++P.acc) {
-                const uint32_t b = P.acc & 1u;
-                ok = __all_sync(0xffffffffu, or_wait(or_smem(&S.acc_full[b]), (P.acc >> 1) & 1u, &S.abort_flag));
-                if (!ok) break;
-                or_fence_after();
-                if (mine) {
-                    const uint32_t taddr = S.tmem + ((uint32_t)(quad * 32) << 16) + b * 256u + (uint32_t)(part * 64);
-                    or_tmem_add32(taddr, v);
-                    or_tmem_add32(taddr + 32, v + 32);
-                }
-                or_fence_before();
-                or_arrive(or_smem(&S.acc_empty[b]));
-            }
-            if (ok && mine) or_finish(O, kind, last, T, T.i * 128 + quad * 32 + lane, (T.c0 >> 6) + part, blk, lane, v);
+        __half* p = static_cast<__half*>(O.out) + i;
+        if constexpr (N == 4) {
+            __half2 w[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
+        } else {
+            *p = __float2half_rn(v[0]);
         }
-        if (!ok) {
-            if (lane == 0) atomicCAS(O.error, 0u, 3u);
-            S.abort_flag = 1;
-        }
-        // the staging block's copies have been written before anyone reads them
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        __syncwarp();
     }
-    asm volatile("fence.proxy.async;" ::: "memory");
-    __syncthreads();
 }
 
-// All blocks (launched cooperatively, so all run); bounded.
-__device__ bool or_grid_sync(const OrthoArgs& O, OrthoShared& S, uint32_t& target) {
-    target += gridDim.x;
+// the last update: rows of the result to the output or the master
+__device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int row, int cb, uint32_t blk, int lane,
+                                              float* v) {
+    const OrthoDesc d = or_get(O, which);
+    const int r0 = row - lane;
+    OrthoOut k = {0.0f, 1.0f};
+    float scale = 1.0f / (ORTHO_SB * ORTHO_SX);
+    if (!O.x) {
+        k.lr = O.controls[0];
+        k.shrink = 1.0f - k.lr * O.controls[2];
+        k.lr *= d.adjust;
+    }
+#pragma unroll
+    for (int j = 0; j < 64; ++j) v[j] *= scale;
+    if (d.tall) {  // lanes are neighbours in memory
+        const int64_t base = d.src + (int64_t)cb * 64 * d.m + row;
+        const int cols = min(64, d.n - cb * 64);
+        if (row < d.m) {
+            if (!O.x) {
+#pragma unroll
+                for (int j0 = 0; j0 < 64; j0 += 8) {
+                    float w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) w[j] = j0 + j < cols ? O.master[base + (int64_t)(j0 + j) * d.m] : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j0 + j < cols) O.master[base + (int64_t)(j0 + j) * d.m] = w[j] * k.shrink - k.lr * v[j0 + j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 64; ++j)
+                    if (j < cols) or_write_out<1>(O, k, base + (int64_t)j * d.m, v + j);
+            }
+        }
+        return;
+    }
+    // 32 rows x 16 columns at a time by way of the staging block, so that lanes write along rows
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    const bool vector = d.n % 4 == 0 && d.src % 4 == 0 && O.aligned;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t addr = blk + (uint32_t)lane * 64u + (uint32_t)((q ^ ((lane >> 1) & 3)) << 4);
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[16 * p + 4 * q]),
+                         "f"(v[16 * p + 4 * q + 1]), "f"(v[16 * p + 4 * q + 2]), "f"(v[16 * p + 4 * q + 3])
+                         : "memory");
+        }
+        __syncwarp();
+        // four columns a lane, four lanes a row
+        const int col = cb * 64 + p * 16 + (lane & 3) * 4;
+        const int64_t base = d.src + (int64_t)(r0 + (lane >> 2)) * d.n + col;
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+            float x[2][4];
+            float4 w[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int it = pair * 2 + u, rr = it * 8 + (lane >> 2), q = lane & 3;
+                const uint32_t addr = blk + (uint32_t)rr * 64u + (uint32_t)((q ^ ((rr >> 1) & 3)) << 4);
+                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                             : "=f"(x[u][0]), "=f"(x[u][1]), "=f"(x[u][2]), "=f"(x[u][3])
+                             : "r"(addr)
+                             : "memory");
+                if (vector && !O.x && r0 + rr < d.m && col < d.n)
+                    w[u] = *reinterpret_cast<const float4*>(O.master + base + (int64_t)it * 8 * d.n);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int it = pair * 2 + u, rr = it * 8 + (lane >> 2);
+                const int64_t at = base + (int64_t)it * 8 * d.n;
+                if (r0 + rr >= d.m || col >= d.n) continue;
+                if (!vector) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < d.n) or_write_out<1>(O, k, at + j, x[u] + j);
+                } else if (O.x) {
+                    or_write_out<4>(O, k, at, x[u]);
+                } else {
+                    *reinterpret_cast<float4*>(O.master + at) =
+                        make_float4(w[u].x * k.shrink - k.lr * x[u][0], w[u].y * k.shrink - k.lr * x[u][1],
+                                    w[u].z * k.shrink - k.lr * x[u][2], w[u].w * k.shrink - k.lr * x[u][3]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// what an epilogue warp does with its 32 rows x 64 columns (rows row - lane ..., column block cb of 64)
+template <bool PRECISE>
+__device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step, int which, int i, int row, int cb,
+                                          uint32_t blk, int blocks, int lane, float* v) {
+    const OrthoPlace L = or_place(O, or_get(O, which), step);
+    const int r0 = row - lane;
+    if (kind == OR_UPDATE) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] *= 1.0f / ORTHO_SB;
+        unsigned char* tile = L.x_next + i * L.x_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
+        or_store_rows(blk, blocks, tile, lane, v, 2);
+        return;
+    }
+    unsigned char* dst = kind == OR_GRAM ? L.a : L.b;
+    const float factor = kind == OR_GRAM ? ORTHO_SA / (ORTHO_SX * ORTHO_SX)
+                                         : (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA));
+    const float diagonal = kind == OR_GRAM ? 0.0f : O.a * ORTHO_SB;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == cb * 64 + j ? diagonal : 0.0f);
+    unsigned char* tile = dst + i * L.a_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
+    or_store_rows(blk, blocks, tile, lane, v, PRECISE ? 2 : 1);
+    if (cb * 64 >= (i + 1) * 128) {
+        // the mirrored place of (row, cb * 64 + j): row block cb / 2, column block row / 64, row (cb & 1) * 64 + j
+        // of that tile; lanes are neighbours
+        const int mc = row & 63;
+        unsigned char* mt = dst + (int64_t)(cb >> 1) * L.a_row + (int64_t)(row >> 6) * ORTHO_TILE + (cb & 1) * 8192 + (mc & 7) * 2;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            unsigned char* at = mt + j * 128 + (((mc >> 3) ^ j) << 4);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                __half hi, lo;
+                or_split(v[8 * q + j], hi, lo);
+                *reinterpret_cast<__half*>(at + q * 1024) = hi;
+                if (PRECISE) *reinterpret_cast<__half*>(at + q * 1024 + 16384) = lo;
+            }
+        }
+    }
+}
+
+struct OrthoShared {
+    uint64_t full[ORTHO_STAGES], empty[ORTHO_STAGES], acc_full[2], acc_empty[2], done;
+    uint32_t tmem;
+    int ok;
+    volatile int abort_flag;
+};
+
+// Between two phases: every role of every block arrives (the launch is cooperative, so all blocks run);
+// bounded.  False when the wait, or a role, gave up.
+__device__ __forceinline__ bool or_phase_end(const OrthoArgs& O, OrthoShared& S, uint32_t phases) {
     asm volatile("fence.proxy.async;" ::: "memory");
-    __syncthreads();
+    asm volatile("bar.sync 1, %0;" ::"n"(ORTHO_THREADS) : "memory");
     if (threadIdx.x == 0) {
+        const uint32_t target = phases * gridDim.x;
         __threadfence();
         uint32_t seen = atomicAdd(O.barrier, 1u) + 1u;
         for (uint32_t i = 0; (int32_t)(seen - target) < 0 && i < ORTHO_WAIT_TRIES; ++i)
@@ -690,43 +684,272 @@ __device__ bool or_grid_sync(const OrthoArgs& O, OrthoShared& S, uint32_t& targe
         __threadfence();
         S.ok = ok && !S.abort_flag;
     }
-    __syncthreads();
+    asm volatile("bar.sync 1, %0;" ::"n"(ORTHO_THREADS) : "memory");
     asm volatile("fence.proxy.async;" ::: "memory");
-    return S.ok != 0;
+    return *reinterpret_cast<volatile int*>(&S.ok) != 0;
 }
 
-// the transition where a direction is not finite: the matrices' gradients are cleared
-__device__ void or_phase_clear(const OrthoArgs& O) {
-    for (int64_t t = blockIdx.x; t < O.convs; t += gridDim.x) {
-        const OrthoDesc d = or_get(O, or_find(O, t, &OrthoDesc::conv0, O.one_conv));
-        const int64_t total = (int64_t)d.m * d.n;
-        const int64_t begin = (t - d.conv0) * 8192;  // a tile's worth of elements in storage order
-        const int64_t end = begin + 8192 < total ? begin + 8192 : total;
-        for (int64_t i = begin + threadIdx.x; i < end; i += ORTHO_THREADS) O.grad[d.src + i] = 0.0f;
+// The operand stages of a kind of product: the row operand's tile (hi, or hi and lo), then up to three
+// 64-wide pieces of the other operand, hi parts and lo parts.
+struct OrthoStage {
+    int pa, pb, stages;
+    uint32_t a_bytes, b_part, bytes;
+};
+template <bool PRECISE>
+__device__ __forceinline__ OrthoStage or_stage(int kind, int bn) {
+    OrthoStage G;
+    G.pa = PRECISE ? 2 : 1;
+    G.pb = PRECISE || kind == OR_UPDATE ? 2 : 1;
+    G.a_bytes = G.pa * 16384u;
+    G.b_part = (uint32_t)bn * 128u;
+    G.bytes = G.a_bytes + G.pb * G.b_part;
+    G.stages = min(ORTHO_STAGES, (int)(ORTHO_RING / G.bytes));
+    return G;
+}
+
+// A producer warp's elected lane, one phase.  A stage is copy 0, the row operand, and copies 1 .. 6, a 64-row
+// or 64-column piece of the other operand each, hi and lo; the producer warps take them in turn.  `pipe`:
+// parity of each stage's next use, a bit a stage, kept from phase to phase.
+template <bool PRECISE>
+__device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int producer,
+                                           uint32_t& pipe) {
+    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const OrthoStage G = or_stage<PRECISE>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
+    bool ok = true;
+    int s = 0;
+    uint32_t used = 0;
+    for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const OrthoTile T = or_tile(O, kind, t);
+        const int kblocks = or_kblocks(O, kind, T), pieces = T.width >> 6;
+        const OrthoPlace L = or_place(O, or_get(O, T.which), step);
+        const unsigned char* src[3];  // of k-blocks 0 and 1
+        uint32_t dst[3], bytes[3], expect = 0;
+        // what an odd k-block and a pair of them add to the pieces (to copy 0: one tile each)
+        const int64_t odd = kind == OR_UPDATE ? 8192 : ORTHO_TILE, pair = kind == OR_UPDATE ? L.x_row : 2 * ORTHO_TILE;
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const int copy = q * ORTHO_PRODUCERS + producer;
+            if (copy == 0) {
+                src[q] = kind == OR_GRAM ? L.x + T.i * L.x_row : kind == OR_SQUARE ? L.a + T.i * L.a_row : L.b + T.i * L.a_row;
+                if (kind == OR_SQUARE && O.c == 0.0f) src[q] += (int64_t)(T.c0 >> 6) * ORTHO_TILE;
+                dst[q] = 0, bytes[q] = G.a_bytes;
+            } else {
+                const int piece = (copy - 1) >> (G.pb - 1), part = (copy - 1) & (G.pb - 1);
+                const int cb = (T.c0 >> 6) + piece;
+                dst[q] = G.a_bytes + part * G.b_part + piece * 8192u;
+                bytes[q] = piece < pieces ? 8192u : 0u;
+                if (kind == OR_UPDATE) src[q] = L.x + (int64_t)cb * ORTHO_TILE + part * 16384;  // 64 k-rows of column block cb
+                else src[q] = (kind == OR_GRAM ? L.x + (cb >> 1) * L.x_row : L.a + (cb >> 1) * L.a_row) + (cb & 1) * 8192 + part * 16384;
+            }
+            expect += bytes[q];
+        }
+        for (int kb = 0; kb < kblocks; ++kb) {
+            if (!or_wait(empty0 + 8 * s, ((pipe >> s) & 1u) ^ 1u, &S.abort_flag)) {
+                ok = false;
+                break;
+            }
+            pipe ^= 1u << s;
+            used |= 1u << s;
+            const uint32_t bar = full0 + 8 * s, at = ring + s * G.bytes;
+            or_expect_tx(bar, expect);
+#pragma unroll
+            for (int q = 0; q < 3; ++q) {
+                const bool row = q == 0 && producer == 0;
+                if (bytes[q]) or_bulk_load(at + dst[q], src[q] + (kb & 1 ? (row ? ORTHO_TILE : odd) : 0), bytes[q], bar);
+                if (kb & 1) src[q] += row ? 2 * ORTHO_TILE : pair;
+            }
+            if (++s == G.stages) s = 0;
+        }
+    }
+    if (!ok) {
+        atomicCAS(O.error, 0u, 1u);
+        S.abort_flag = 1;
+    }
+    if (S.abort_flag) {  // every copy under way lands before the block can end
+        for (int q = 0; q < G.stages; ++q)
+            for (uint32_t i = 0; ((used >> q) & 1u) && i < ORTHO_WAIT_TRIES &&
+                                 !or_try_wait(full0 + 8 * q, ((pipe >> q) & 1u) ^ 1u); ++i) {
+            }
     }
 }
 
-// Phases: 0 squares, 1 conversion, then per step the Gram matrix, its polynomial, and the update.
+// The issuing warp's elected lane, one phase.  `acc` counts accumulators used.
+template <bool PRECISE>
+__device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, uint32_t& pipe,
+                                         uint32_t& acc) {
+    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const OrthoStage G = or_stage<PRECISE>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
+    const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
+    const bool linear = kind == OR_SQUARE && O.c == 0.0f;
+    const int chunk = PRECISE && !linear ? 1 : 1 << 20;
+    const int mn = kind == OR_UPDATE;
+    const uint32_t b_step = mn ? 2048u >> 4 : 32u >> 4, lbo = mn ? 8192u : 16u;
+    const uint32_t eye = or_desc(ring + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK, 16), eye_idesc = or_idesc(16, 0);
+    const uint32_t tmem = S.tmem;
+    bool ok = true;
+    int s = 0;
+    for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const OrthoTile T = or_tile(O, kind, t);
+        const int kblocks = or_kblocks(O, kind, T);
+        const uint32_t idesc = or_idesc(T.width, mn);
+        const int eye0 = kind == OR_SQUARE ? T.c0 >> 6 : 1 << 30, eye1 = eye0 + (T.width >> 6);
+        for (int k0 = 0; ok && k0 < kblocks; k0 += chunk, ++acc) {
+            const uint32_t b = acc & 1u;
+            if (!or_wait(acc_empty0 + 8 * b, ((acc >> 1) & 1u) ^ 1u, &S.abort_flag)) {
+                ok = false;
+                break;
+            }
+            or_fence_after();
+            const uint32_t d = tmem + b * 256u;
+            const int k1 = min(k0 + chunk, kblocks);
+            for (int kb = k0; kb < k1; ++kb) {
+                if (!or_wait(full0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                pipe ^= 1u << s;
+                or_fence_after();
+                const uint32_t a = or_desc(ring + s * G.bytes, 16), al = a + (16384u >> 4);
+                const uint32_t bh = or_desc(ring + s * G.bytes + G.a_bytes, lbo), bl = bh + (G.b_part >> 4);
+                if (linear) {
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) {
+                        const uint32_t dd = d + (uint32_t)kb * 64u + ks * 16;
+                        if (PRECISE) or_mma(dd, al + ks * 2, eye, eye_idesc, 0u);
+                        or_mma(dd, a + ks * 2, eye, eye_idesc, PRECISE);
+                    }
+                } else {
+                    // the small products first: they are added to a small sum
+                    uint32_t more = kb > k0;
+                    if (PRECISE) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma(d, al + ks * 2, bh + ks * b_step, idesc, more);
+                    }
+                    if (G.pb == 2) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma(d, a + ks * 2, bl + ks * b_step, idesc, more);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma(d, a + ks * 2, bh + ks * b_step, idesc, more);
+                    if (kb >= eye0 && kb < eye1) {
+                        // c A A + b A = c (A A + A (b / c) I): this k-block's columns once more, 16 at a time,
+                        // against a scaled identity
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) {
+                            const uint32_t dd = d + (uint32_t)(kb - eye0) * 64u + ks * 16;
+                            or_mma(dd, a + ks * 2, eye, eye_idesc, 1u);
+                            or_mma(dd, a + ks * 2, eye + 2, eye_idesc, 1u);
+                            if (PRECISE) or_mma(dd, al + ks * 2, eye, eye_idesc, 1u);
+                        }
+                    }
+                }
+                or_commit(empty0 + 8 * s);
+                if (++s == G.stages) s = 0;
+            }
+            if (ok) or_commit(acc_full0 + 8 * b);
+        }
+    }
+    if (!ok) {
+        atomicCAS(O.error, 0u, 2u);
+        S.abort_flag = 1;
+    }
+}
+
+// An epilogue warp, one phase: a quarter of the rows, a 64-column part of each tile.
+template <bool PRECISE>
+__device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int e,
+                                           uint32_t& acc) {
+    const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, part = e >> 2;
+    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const int bn = kind == OR_UPDATE ? O.bn_upd : O.bn_sym;
+    const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
+    const int chunk = PRECISE && !(kind == OR_SQUARE && O.c == 0.0f) ? 1 : 1 << 20;
+    // with tiles one part wide the other parts' staging blocks are free
+    const int blocks = bn == 64 ? ORTHO_EPI_WARPS / 4 : 1;
+    const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * ORTHO_BLOCK;
+    const uint32_t taddr0 = S.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * 64);
+    bool ok = true;
+    for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const OrthoTile T = or_tile(O, kind, t);
+        const bool mine = part < (T.width >> 6);
+        const int chunks = (or_kblocks(O, kind, T) - 1) / chunk + 1;
+        float v[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) v[j] = 0.0f;
+        for (int k = 0; k < chunks; ++k, ++acc) {
+            const uint32_t b = acc & 1u;
+            ok = __all_sync(0xffffffffu, or_wait(acc_full0 + 8 * b, (acc >> 1) & 1u, &S.abort_flag));
+            if (!ok) break;
+            or_fence_after();
+            if (mine) {
+                or_tmem_add32(taddr0 + b * 256u, v);
+                or_tmem_add32(taddr0 + b * 256u + 32, v + 32);
+            }
+            or_fence_before();
+            __syncwarp();
+            if (lane == 0) or_arrive(acc_empty0 + 8 * b);
+        }
+        if (ok && mine) {
+            const int row = T.i * 128 + quad * 32 + lane, cb = (T.c0 >> 6) + part;
+            if (kind == OR_UPDATE && step == O.steps - 1) or_finish_out(O, T.which, row, cb, blk, lane, v);
+            else or_finish<PRECISE>(O, kind, step, T.which, T.i, row, cb, blk, blocks, lane, v);
+        }
+    }
+    if (!ok) {
+        if (lane == 0) atomicCAS(O.error, 0u, 3u);
+        S.abort_flag = 1;
+    }
+    // the staging blocks' copies have been written before anyone reads them
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+}
+
+// The steps' products: per step the Gram matrix, its polynomial and the update, a phase each over all
+// matrices, each role running through the phases on its own.
+template <bool PRECISE>
 __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const __grid_constant__ OrthoArgs O) {
-    extern __shared__ __align__(16) unsigned char or_raw[];
-    __shared__ __align__(8) OrthoShared S;
-    const uint32_t ring = (or_smem(or_raw) + 1023u) & ~1023u;
+    // the first kilobyte holds the barriers; the ring after it starts on the 1024 bytes of a swizzle atom
+    extern __shared__ __align__(1024) unsigned char or_raw[];
+    OrthoShared& S = *reinterpret_cast<OrthoShared*>(or_raw);
+    static_assert(sizeof(OrthoShared) <= 1024, "shared state fits its kilobyte");
+    const uint32_t ring = or_smem(or_raw) + 1024u;
+    if (ring & 1023u) {  // never: dynamic shared memory alone starts on a kilobyte
+        atomicCAS(O.error, 0u, 5u);
+        return;
+    }
+    if (!O.x && *O.bad) return;  // the transition leaves everything as it was
     const int warp = threadIdx.x >> 5;
-    const bool products = O.phase1 > 2;
     if (threadIdx.x == 0) {
         S.abort_flag = 0;
         for (int s = 0; s < ORTHO_STAGES; ++s) {
-            or_mbar_init(or_smem(&S.full[s]), 1);
+            or_mbar_init(or_smem(&S.full[s]), ORTHO_PRODUCERS);
             or_mbar_init(or_smem(&S.empty[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
             or_mbar_init(or_smem(&S.acc_full[b]), 1);
-            or_mbar_init(or_smem(&S.acc_empty[b]), 32 * ORTHO_EPI_WARPS);
+            or_mbar_init(or_smem(&S.acc_empty[b]), ORTHO_EPI_WARPS);
         }
         or_mbar_init(or_smem(&S.done), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (products && warp == 1) {
+    if (threadIdx.x >= 128 && threadIdx.x < 256) {
+        // 16 rows x 8 chunks of 16 bytes, swizzled: chunks 0-1 hold hi (columns 0-15), chunks 2-3 lo
+        const int r = (threadIdx.x - 128) >> 3, chunk = (threadIdx.x - 128) & 7;
+        const float value = O.c != 0.0f ? O.b / O.c * ORTHO_SA : ORTHO_SA;
+        __align__(16) __half h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            __half hi, lo;
+            or_split((chunk & 1) * 8 + e == r ? value : 0.0f, hi, lo);
+            h[e] = chunk < 2 ? hi : chunk < 4 ? lo : __float2half_rn(0.0f);
+        }
+        unsigned char* at = or_raw + 1024 + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK + r * 128 + ((chunk ^ (r & 7)) << 4);
+        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(h);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(or_smem(&S.tmem)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -734,24 +957,29 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
     or_fence_before();
     __syncthreads();
     or_fence_after();
-    OrthoPipe P = {0u, 0u, 0u};
-    uint32_t target = 0;
-    for (int phase = O.phase0; phase < O.phase1; ++phase) {
-        if (phase > O.phase0 && !or_grid_sync(O, S, target)) break;
-        const bool bad = phase > 0 && !O.x && __ldcg(O.bad) != 0u;
-        if (phase == 0) or_phase_squares(O, S);
-        else if (bad) {
-            if (phase == 1) or_phase_clear(O);
-        } else if (phase == 1) {
-            or_phase_convert(O, S);
-        } else {
-            or_phase_product(O, S, P, ring, (phase - 2) % 3, (phase - 2) / 3);
-            if (S.abort_flag) break;
+    const int phases = 3 * O.steps;
+    uint32_t pipe = 0, acc = 0;
+    if (warp == 0) {
+        for (int p = 0; p < phases; ++p) {
+            if (or_elect()) or_issue<PRECISE>(O, S, ring, p % 3, p / 3, pipe, acc);
+            __syncwarp();
+            if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
+        }
+    } else if (warp <= ORTHO_PRODUCERS) {
+        for (int p = 0; p < phases; ++p) {
+            if (or_elect()) or_produce<PRECISE>(O, S, ring, p % 3, p / 3, warp - 1, pipe);
+            __syncwarp();
+            if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
+        }
+    } else {
+        for (int p = 0; p < phases; ++p) {
+            or_collect<PRECISE>(O, S, ring, p % 3, p / 3, warp - 1 - ORTHO_PRODUCERS, acc);
+            if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     }
     __syncthreads();
-    if (products && warp == 1) {
-        if ((threadIdx.x & 31) == 0) {
+    if (warp == 0) {
+        if (or_elect()) {
             // nothing that this thread issued is under way when the memory is freed
             or_commit(or_smem(&S.done));
             for (uint32_t i = 0; i < ORTHO_WAIT_TRIES && !or_try_wait(or_smem(&S.done), 0u); ++i) {
@@ -787,15 +1015,15 @@ static OrthoDesc or_make(int64_t rows, int64_t cols) {
 }
 
 // Output tile width, by an estimate of the busiest SM's cycles: a k-block of 64 costs 12 instructions of
-// 48, 64 or 128 cycles at widths 64, 128 and 256 (the narrow ones wait for shared memory), an output tile
-// some 1,500 cycles and 6 a column to finish.  Wide tiles carry long products (256: 0.9 of the cycles per
-// multiply-add that 128 takes, 0.67 of 64), narrow ones spread a few small matrices over more SMs.
+// 48, 64 or 96 cycles at widths 64, 128 and 192 (the narrowest wait for shared memory), an output tile some
+// 1,500 cycles and 6 a column to finish.  Wide tiles read less per multiply-add, narrow ones spread a few
+// small matrices over more SMs.
 struct OrthoWidths {
     double sum[2][3], top[2][3];
 };
-static const int OR_WIDTHS[3] = {64, 128, 256};
+static const int OR_WIDTHS[3] = {64, 128, 192};
 static void or_weigh(OrthoWidths& W, int m, int n, int64_t count) {
-    static const double block[3] = {576.0, 768.0, 1536.0};
+    static const double block[3] = {576.0, 768.0, 1152.0};
     for (int w = 0; w < 3; ++w)
         for (int kind = 0; kind < 2; ++kind) {
             const int bn = OR_WIDTHS[w];
@@ -817,46 +1045,70 @@ static int or_width(const OrthoWidths& W, int kind) {
 
 static int64_t or_up(int64_t v) { return (v + 1023) / 1024 * 1024; }
 
-static int or_launch(const OrthoArgs& O, cudaStream_t s) {
+static int or_squares(const OrthoArgs& O, cudaStream_t s) {
+    PBG_REQUIRE(O.spans < (1ll << 31), "orthogonalize: too many elements for one launch");
+    orthogonalize_squares_kernel<<<(unsigned)O.spans, ORTHO_FLAT, 0, s>>>(O);
+    return launch_status("orthogonalize: squares");
+}
+
+// conversion, then the products
+static int or_products(const OrthoArgs& O, cudaStream_t s) {
+    const void* kernel = O.precise ? (const void*)orthogonalize_kernel<true> : (const void*)orthogonalize_kernel<false>;
     static int configured[64] = {0};
     int dev = 0;
     cudaGetDevice(&dev);
+    int rc = 0;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        const int rc = cuda_status(cudaFuncSetAttribute(orthogonalize_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
-                                   "orthogonalize: shared memory size");
+        rc = cuda_status(cudaFuncSetAttribute(orthogonalize_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
+                         "orthogonalize: shared memory size");
+        if (!rc)
+            rc = cuda_status(cudaFuncSetAttribute(orthogonalize_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
+                             "orthogonalize: shared memory size");
         if (rc) return rc;
         if (dev >= 0 && dev < 64) configured[dev] = 1;
     }
-    int64_t want = O.phase0 == 0 ? O.spans : 1;
-    if (O.phase1 > 1 && O.convs > want) want = O.convs;
-    if (O.phase1 > 2 && O.syms > want) want = O.syms;
-    if (O.phase1 > 2 && O.upds > want) want = O.upds;
-    const int grid = (int)(want < sm_count() ? want : sm_count());
-    int rc = cuda_status(cudaMemsetAsync(O.barrier, 0, 4, s), "orthogonalize: barrier");
+    rc = cuda_status(cudaMemsetAsync(O.barrier, 0, 4, s), "orthogonalize: barrier");
     if (rc) return rc;
+    PBG_REQUIRE(O.convs < (1ll << 31), "orthogonalize: too many tiles for one launch");
+    orthogonalize_convert_kernel<<<(unsigned)O.convs, ORTHO_FLAT, 0, s>>>(O);
+    rc = launch_status("orthogonalize: conversion");
+    if (rc) return rc;
+    const int64_t want = O.syms > O.upds ? O.syms : O.upds;
+    const int grid = (int)(want < sm_count() ? want : sm_count());
     void* args[] = {const_cast<OrthoArgs*>(&O)};
-    return cuda_status(cudaLaunchCooperativeKernel((const void*)orthogonalize_kernel, dim3((unsigned)grid), dim3(ORTHO_THREADS),
-                                                   args, (size_t)ORTHO_SMEM, s),
+    return cuda_status(cudaLaunchCooperativeKernel(kernel, dim3((unsigned)grid), dim3(ORTHO_THREADS), args, (size_t)ORTHO_SMEM, s),
                        "orthogonalize: cooperative launch");
 }
 
-// The fp16 scales hold while no singular value passes 2 and |a + b s^2 + c s^4| stays below 15: followed
-// step by step from [0, 1] over a fine grid (the polynomials in use stay within 1.3 and 3.5).
+// The fp16 scales hold while no singular value passes 2 and |a + b s^2 + c s^4| stays below 15: the range
+// [0, 1] of the first iterate followed step by step, the extremes of s (a + b s^2 + c s^4) and of its factor
+// being at the ends of a range and where their derivatives vanish (the polynomials in use stay within 1.3
+// and 3.5).
 static int or_check_polynomial(int steps, float a, float b, float c) {
     PBG_REQUIRE(steps >= 1 && steps <= 100, "orthogonalize: steps must be in [1,100]");
+    PBG_REQUIRE(c == 0.0f || (b / c < 7.9f && b / c > -7.9f), "orthogonalize: |b| must be below 7.9 |c| where c is not 0");
+    const double A = a, B = b, C = c;
+    double at[4] = {0.0, -1.0, -1.0, -1.0};  // squares of the inner extremes' places; the range's end joins them
+    if (C != 0.0) {
+        const double disc = 9.0 * B * B - 20.0 * A * C;
+        if (disc >= 0.0) at[1] = (-3.0 * B + sqrt(disc)) / (10.0 * C), at[2] = (-3.0 * B - sqrt(disc)) / (10.0 * C);
+        at[3] = -B / (2.0 * C);
+    } else if (B != 0.0) {
+        at[1] = -A / (3.0 * B);
+    }
     double top = 1.0;
     for (int k = 0; k < steps; ++k) {
         double next = 0.0;
-        for (int i = 0; i <= 1000; ++i) {
-            const double s = top * i / 1000.0, g = s * s, q = a + g * (b + g * c);
-            PBG_REQUIRE(q > -15.0 && q < 15.0 && b * g + a < 15.0, "orthogonalize: the coefficients leave the range of the products");
-            const double v = s * (q < 0 ? -q : q);
-            if (v > next) next = v;
+        for (int i = 0; i < 5; ++i) {
+            const double g = i < 4 ? at[i] : top * top;
+            if (!(g >= 0.0 && g <= top * top) && i < 4) continue;
+            const double q = fabs(A + g * (B + g * C));
+            PBG_REQUIRE(q < 15.0, "orthogonalize: the coefficients leave the range of the products");
+            next = fmax(next, sqrt(g) * q);
         }
         PBG_REQUIRE(next < 1.9, "orthogonalize: the coefficients let singular values grow past 2");
-        const bool same = next <= top;
-        top = next > 1.0 ? next : 1.0;
-        if (same && k > 0) break;
+        if (next <= top && k > 0) break;
+        top = fmax(next, 1.0);
     }
     return 0;
 }
@@ -908,7 +1160,6 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.x_type = x_type, O.out_type = out_type, O.error = error;
     O.precise = !(out_type == 1 && m >= ORTHO_SINGLE);
-    O.phase0 = 0, O.phase1 = 2 + 3 * steps;
     const int64_t xs = x_type == 0 ? 4 : 2, os = out_type == 0 ? 4 : 2;
     for (int64_t at = 0; at < batch; at += k) {
         O.count = batch - at < k ? batch - at : k;
@@ -920,7 +1171,9 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
         O.syms = O.count * O.one_sym, O.upds = O.count * O.one_upd;
         O.x = static_cast<const unsigned char*>(x) + at * rows * cols * xs;
         O.out = static_cast<unsigned char*>(out) + at * rows * cols * os;
-        rc = or_launch(O, as_stream(stream));
+        O.aligned = (uintptr_t)O.x % 16 == 0 && (uintptr_t)O.out % 16 == 0;
+        rc = or_squares(O, as_stream(stream));
+        if (!rc) rc = or_products(O, as_stream(stream));
         if (rc) return rc;
     }
     return 0;
@@ -996,23 +1249,19 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
     O.precise = 1;
     O.grad = grad, O.momentum = momentum, O.master = master, O.controls = controls;
     O.nesterov = nesterov, O.bad = skipped, O.error = error;
+    O.aligned = (uintptr_t)grad % 16 == 0 && (uintptr_t)momentum % 16 == 0 && (uintptr_t)master % 16 == 0;
     rc = cuda_status(cudaMemsetAsync(skipped, 0, 4, s), "muon_step: status");
     if (rc) return rc;
     const OrthoDesc* list = static_cast<const OrthoDesc*>(descriptors);
     const int64_t waves = plan[2];
-    if (waves > 1) {  // every direction is checked before anything is written
-        O.list = list, O.count = count, O.spans = plan[1];
-        O.phase0 = 0, O.phase1 = 1;
-        rc = or_launch(O, s);
-        if (rc) return rc;
-    }
+    O.list = list, O.count = count, O.spans = plan[1];
+    rc = or_squares(O, s);  // of all matrices: every direction is checked before anything is written
+    if (rc) return rc;
     for (int64_t i = 0; i < waves; ++i) {
         const int64_t* wave = plan + 8 + 5 * i;
         O.list = list + wave[0], O.count = wave[1];
         O.convs = wave[2], O.syms = wave[3], O.upds = wave[4];
-        O.phase0 = waves > 1 ? 1 : 0, O.phase1 = 2 + 3 * steps;
-        O.spans = plan[1];
-        rc = or_launch(O, s);
+        rc = or_products(O, s);
         if (rc) return rc;
     }
     return 0;
