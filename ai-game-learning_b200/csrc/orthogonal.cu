@@ -40,14 +40,15 @@
 
 namespace pbg {
 
-constexpr int ORTHO_EPI_WARPS = 12;    // four row quarters x three 64-column parts; 16 warps in all leave 128 registers
+constexpr int ORTHO_EPI_WARPS = 8;     // four row quarters x two column parts; 12 warps in all leave 168 registers
 constexpr int ORTHO_PRODUCERS = 3;      // warps that issue bulk copies, a third of a stage's each
 constexpr int ORTHO_THREADS = 32 * (1 + ORTHO_PRODUCERS + ORTHO_EPI_WARPS);  // warp 0 issues the products
 constexpr int ORTHO_RING = 192 * 1024;  // operand stages
 constexpr int ORTHO_STAGES = 8;         // at most
-constexpr int ORTHO_BLOCK = 2048;       // an epilogue warp's staging block
+constexpr int ORTHO_BLOCK = 2048;       // a staging block; an epilogue warp has two
 constexpr int ORTHO_EYE = 2048;         // 16 rows of 128 bytes: (b / c) 2^13 I in fp16 (2^13 I where c is 0), hi, and lo 32 bytes on
-constexpr int ORTHO_SMEM = 1024 + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK + ORTHO_EYE;
+constexpr int ORTHO_STAGING = 2 * ORTHO_EPI_WARPS * ORTHO_BLOCK;
+constexpr int ORTHO_SMEM = 1024 + ORTHO_RING + ORTHO_STAGING + ORTHO_EYE;
 constexpr int ORTHO_FLAT = 256;         // threads of the kernels around the products
 constexpr int ORTHO_SPAN = ORTHO_FLAT * 16;  // elements whose squares one block sums
 constexpr int ORTHO_TILE = 32768;       // bytes of a 128 x 64 tile, hi and lo
@@ -70,6 +71,7 @@ struct OrthoArgs {
     int64_t one_src, one_ws, one_span, one_conv, one_sym, one_upd;
     int64_t count, spans, convs, syms, upds;  // totals
     int bn_sym, bn_upd;  // output tile widths
+    int pair;            // output tiles of 256 rows, by two blocks each
     int steps, precise;  // precise: A and B as pairs
     float a, b, c;
     double eps;
@@ -134,20 +136,33 @@ __device__ __forceinline__ void or_bulk_load(uint32_t dst, const void* src, uint
 // columns of 8 k-rows an atom, the next k-rows 1024 bytes on, the next 64 columns `lbo` bytes on).  The low
 // word of the descriptor, whose high word is the same for both.
 __device__ __forceinline__ uint32_t or_desc(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
-// kind::f16: fp16 x fp16 -> fp32, M 128, A K-major, B K-major or MN-major
+// kind::f16: fp16 x fp16 -> fp32, M 128 or (pair) 256, A K-major, B K-major or MN-major
+template <bool PAIR>
 __device__ __forceinline__ uint32_t or_idesc(int n, int mn_major) {
-    return (1u << 4) | ((uint32_t)mn_major << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+    return (1u << 4) | ((uint32_t)mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((PAIR ? 16u : 8u) << 24);
 }
+template <bool PAIR>
 __device__ __forceinline__ void or_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29);
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-        "mov.b64 da, {%1, %5};\n\t"
-        "mov.b64 db, {%2, %5};\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(high)
-        : "memory");
+    if constexpr (PAIR) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %5};\n\t"
+            "mov.b64 db, {%2, %5};\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(high)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %5};\n\t"
+            "mov.b64 db, {%2, %5};\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(high)
+            : "memory");
+    }
 }
 // one lane of a converged warp; the compiler knows that it runs alone and keeps descriptors in uniform registers
 __device__ __forceinline__ bool or_elect() {
@@ -155,25 +170,67 @@ __device__ __forceinline__ bool or_elect() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
     return one != 0;
 }
+// the products issued so far arrive at a barrier when done; a pair's at both blocks' barriers
+template <bool PAIR>
 __device__ __forceinline__ void or_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Arrival at the pair's first block's barrier.  Relaxed: the arriving thread has written nothing that the
+// other block reads (it has seen its own block's copies land, or taken its accumulators' columns), and a
+// release at cluster scope here costs as long as a k-block's products.
+__device__ __forceinline__ void or_arrive_first(uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\t"
+        "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
+        : "memory");
+}
+// a wait for arrivals of the other block too
+__device__ __forceinline__ bool or_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+template <bool PAIR>
+__device__ __forceinline__ bool or_wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (uint32_t i = 0; i < ORTHO_WAIT_TRIES; ++i) {
+        if (PAIR ? or_try_wait_cluster(bar, parity) : or_try_wait(bar, parity)) return true;
+        if ((i & 1023u) == 1023u && *abort_flag) return false;
+    }
+    return false;
+}
+__device__ __forceinline__ void or_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t or_cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
 __device__ __forceinline__ void or_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void or_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void or_tmem_add32(uint32_t taddr, float* acc) {
-    uint32_t r[32];
+__device__ __forceinline__ void or_tmem_add16(uint32_t taddr, float* acc) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int j = 0; j < 32; ++j) acc[j] += __uint_as_float(r[j]);
+    for (int j = 0; j < 16; ++j) acc[j] += __uint_as_float(r[j]);
 }
 
 // ------------------------------------------------------------ descriptors
@@ -205,13 +262,17 @@ __device__ __forceinline__ int64_t or_find(const OrthoArgs& O, int64_t t, int64_
 __host__ __device__ __forceinline__ int or_mb(int m) { return (m + 127) >> 7; }
 __host__ __device__ __forceinline__ int or_b64(int v) { return (v + 63) >> 6; }
 // tiles from one row block to the next, odd: the blocks that read one column of tiles at a time would
-// otherwise meet in a few memory slices where the pitch is a power of two
-__host__ __device__ __forceinline__ int or_pitch_x(int n) { return or_b64(n) | 1; }
+// otherwise meet in a few memory slices where the pitch is a power of two (a row block of X has a tile to
+// spare: a pair of blocks reads columns by 128)
+__host__ __device__ __forceinline__ int or_pitch_x(int n) { return (or_b64(n) + 1) | 1; }
 __host__ __device__ __forceinline__ int or_pitch_a(int m) { return 2 * or_mb(m) | 1; }
 __host__ __device__ __forceinline__ int64_t or_x_bytes(int m, int n) { return (int64_t)or_mb(m) * or_pitch_x(n) * ORTHO_TILE; }
 __host__ __device__ __forceinline__ int64_t or_a_bytes(int m) { return (int64_t)or_mb(m) * or_pitch_a(m) * ORTHO_TILE; }
-// symmetric tiles of row block i: from column 128 i on
-__host__ __device__ __forceinline__ int or_sym_row(int m, int i, int bn) { return (or_b64(m) * 64 - i * 128 + bn - 1) / bn; }
+// symmetric tiles of row block (pair of row blocks) i: from its first row's column on
+__host__ __device__ __forceinline__ int or_sym_row(int m, int i, int bn, int pair) {
+    return pair ? (or_mb(m) + 1) / 2 - i : (or_b64(m) * 64 - i * 128 + bn - 1) / bn;
+}
+__host__ __device__ __forceinline__ int or_row_blocks(int m, int pair) { return pair ? (or_mb(m) + 1) / 2 : or_mb(m); }
 
 // ------------------------------------------------------------ the direction that is orthogonalised
 
@@ -400,24 +461,33 @@ struct OrthoTile {
     int which, i, c0, width;
 };
 
-__device__ __forceinline__ OrthoTile or_tile(const OrthoArgs& O, int kind, int64_t t) {
+// Tile t as one block (or the block of rank `rank` of a pair) sees it.  A pair's second row block may not
+// exist (i = or_mb(m)); its columns come by 128.
+template <bool PAIR>
+__device__ __forceinline__ OrthoTile or_tile(const OrthoArgs& O, int kind, int64_t t, int rank) {
     OrthoTile T;
     const bool sym = kind != OR_UPDATE;
     const int64_t w = sym ? or_find(O, t, &OrthoDesc::sym0, O.one_sym) : or_find(O, t, &OrthoDesc::upd0, O.one_upd);
     T.which = (int)w;
     const int64_t first = O.list ? (sym ? O.list[w].sym0 : O.list[w].upd0) : w * (sym ? O.one_sym : O.one_upd);
     const int m = O.list ? O.list[w].m : O.one.m, n = O.list ? O.list[w].n : O.one.n;
-    int local = (int)(t - first);
+    int local = (int)(t - first), columns;
     if (sym) {
         T.i = 0;
-        for (int r; local >= (r = or_sym_row(m, T.i, O.bn_sym)); ++T.i) local -= r;
-        T.c0 = T.i * 128 + local * O.bn_sym;
-        T.width = min(O.bn_sym, or_b64(m) * 64 - T.c0);
+        for (int r; local >= (r = or_sym_row(m, T.i, O.bn_sym, PAIR)); ++T.i) local -= r;
+        T.c0 = T.i * (PAIR ? 256 : 128) + local * O.bn_sym;
+        columns = or_b64(m) * 64 - T.c0;
+        T.width = min(O.bn_sym, columns);
     } else {
         const int across = (or_b64(n) * 64 + O.bn_upd - 1) / O.bn_upd;
         T.i = local / across;
         T.c0 = (local % across) * O.bn_upd;
-        T.width = min(O.bn_upd, or_b64(n) * 64 - T.c0);
+        columns = or_b64(n) * 64 - T.c0;
+        T.width = min(O.bn_upd, columns);
+    }
+    if (PAIR) {
+        T.i = 2 * T.i + rank;
+        T.width = (T.width + 127) & ~127;
     }
     return T;
 }
@@ -447,8 +517,8 @@ __device__ __forceinline__ OrthoPlace or_place(const OrthoArgs& O, const OrthoDe
 }
 
 // A thread's 64 finished values of one row as a row of a 128 x 64 tile, hi then lo, by way of the warp's
-// staging blocks of 16 rows (rows of 128 bytes are contiguous in the tile, so each block is one bulk copy).
-// `blocks` of them 4 ORTHO_BLOCK apart belong to the warp: those of the warps without columns are used too.
+// staging blocks of 16 rows (rows of 128 bytes are contiguous in the tile, so each block is one bulk copy):
+// two, or four where the warp of the other column part has no columns.
 __device__ __forceinline__ void or_store_rows(uint32_t blk, int blocks, unsigned char* dst, int lane, float* v, int parts) {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
@@ -457,13 +527,10 @@ __device__ __forceinline__ void or_store_rows(uint32_t blk, int blocks, unsigned
         {
             const bool low = round >= 2;
             if (round >= blocks) {
-                if (lane == 0) {
-                    if (blocks == 1) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                }
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                 __syncwarp();
             }
-            const uint32_t at = blk + (uint32_t)(round % blocks) * (4u * ORTHO_BLOCK);
+            const uint32_t at = blk + (uint32_t)(round & 1) * ORTHO_BLOCK + (low && blocks == 4 ? 8u * ORTHO_BLOCK : 0u);
             if ((lane >> 4) == (round & 1)) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
@@ -634,6 +701,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
         or_store_rows(blk, blocks, tile, lane, v, 2);
         return;
     }
+    if ((cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
     unsigned char* dst = kind == OR_GRAM ? L.a : L.b;
     const float factor = kind == OR_GRAM ? ORTHO_SA / (ORTHO_SX * ORTHO_SX)
                                          : (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA));
@@ -662,7 +730,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
 }
 
 struct OrthoShared {
-    uint64_t full[ORTHO_STAGES], empty[ORTHO_STAGES], acc_full[2], acc_empty[2], done;
+    uint64_t full[ORTHO_STAGES], empty[ORTHO_STAGES], peer[ORTHO_STAGES], acc_full[2], acc_empty[2], done;
     uint32_t tmem;
     int ok;
     volatile int abort_flag;
@@ -682,26 +750,27 @@ __device__ __forceinline__ bool or_phase_end(const OrthoArgs& O, OrthoShared& S,
         const bool ok = (int32_t)(seen - target) >= 0;
         if (!ok) atomicCAS(O.error, 0u, 4u);
         __threadfence();
-        S.ok = ok && !S.abort_flag;
+        // no phase after one that any block gave up
+        S.ok = ok && !S.abort_flag && *reinterpret_cast<volatile uint32_t*>(O.error) == 0u;
     }
     asm volatile("bar.sync 1, %0;" ::"n"(ORTHO_THREADS) : "memory");
     asm volatile("fence.proxy.async;" ::: "memory");
     return *reinterpret_cast<volatile int*>(&S.ok) != 0;
 }
 
-// The operand stages of a kind of product: the row operand's tile (hi, or hi and lo), then up to three
-// 64-wide pieces of the other operand, hi parts and lo parts.
+// The operand stages of a kind of product: the row operand's tile (hi, or hi and lo), then up to three (of a
+// pair, two: half of the columns) 64-wide pieces of the other operand, hi parts and lo parts.
 struct OrthoStage {
     int pa, pb, stages;
     uint32_t a_bytes, b_part, bytes;
 };
-template <bool PRECISE>
+template <bool PRECISE, bool PAIR>
 __device__ __forceinline__ OrthoStage or_stage(int kind, int bn) {
     OrthoStage G;
     G.pa = PRECISE ? 2 : 1;
     G.pb = PRECISE || kind == OR_UPDATE ? 2 : 1;
     G.a_bytes = G.pa * 16384u;
-    G.b_part = (uint32_t)bn * 128u;
+    G.b_part = (uint32_t)(PAIR ? bn / 2 : bn) * 128u;
     G.bytes = G.a_bytes + G.pb * G.b_part;
     G.stages = min(ORTHO_STAGES, (int)(ORTHO_RING / G.bytes));
     return G;
@@ -710,19 +779,21 @@ __device__ __forceinline__ OrthoStage or_stage(int kind, int bn) {
 // A producer warp's elected lane, one phase.  A stage is copy 0, the row operand, and copies 1 .. 6, a 64-row
 // or 64-column piece of the other operand each, hi and lo; the producer warps take them in turn.  `pipe`:
 // parity of each stage's next use, a bit a stage, kept from phase to phase.
-template <bool PRECISE>
-__device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int producer,
-                                           uint32_t& pipe) {
+template <bool PRECISE, bool PAIR>
+__device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int rank,
+                                           int producer, uint32_t& pipe) {
     const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
-    const OrthoStage G = or_stage<PRECISE>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
     bool ok = true;
     int s = 0;
     uint32_t used = 0;
-    for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const OrthoTile T = or_tile(O, kind, t);
-        const int kblocks = or_kblocks(O, kind, T), pieces = T.width >> 6;
-        const OrthoPlace L = or_place(O, or_get(O, T.which), step);
+    for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
+        OrthoTile T = or_tile<PAIR>(O, kind, t, rank);
+        const int kblocks = or_kblocks(O, kind, T), pieces = T.width >> (PAIR ? 7 : 6);
+        const OrthoDesc desc = or_get(O, T.which);
+        const OrthoPlace L = or_place(O, desc, step);
+        if (PAIR) T.i = min(T.i, or_mb(desc.m) - 1);  // the row block that is not there: any other, never stored
         const unsigned char* src[3];  // of k-blocks 0 and 1
         uint32_t dst[3], bytes[3], expect = 0;
         // what an odd k-block and a pair of them add to the pieces (to copy 0: one tile each)
@@ -736,7 +807,7 @@ __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, u
                 dst[q] = 0, bytes[q] = G.a_bytes;
             } else {
                 const int piece = (copy - 1) >> (G.pb - 1), part = (copy - 1) & (G.pb - 1);
-                const int cb = (T.c0 >> 6) + piece;
+                const int cb = (T.c0 >> 6) + (PAIR ? rank * pieces : 0) + piece;
                 dst[q] = G.a_bytes + part * G.b_part + piece * 8192u;
                 bytes[q] = piece < pieces ? 8192u : 0u;
                 if (kind == OR_UPDATE) src[q] = L.x + (int64_t)cb * ORTHO_TILE + part * 16384;  // 64 k-rows of column block cb
@@ -774,30 +845,31 @@ __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, u
     }
 }
 
-// The issuing warp's elected lane, one phase.  `acc` counts accumulators used.
-template <bool PRECISE>
-__device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, uint32_t& pipe,
+// The issuing warp's elected lane (of a pair's first block), one phase.  `acc` counts accumulators used.
+template <bool PRECISE, bool PAIR>
+__device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, uint32_t& pipe,
                                          uint32_t& acc) {
     const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
-    const OrthoStage G = or_stage<PRECISE>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
+    const uint32_t peer0 = or_smem(&S.peer[0]);
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
     const bool linear = kind == OR_SQUARE && O.c == 0.0f;
     const int chunk = PRECISE && !linear ? 1 : 1 << 20;
     const int mn = kind == OR_UPDATE;
     const uint32_t b_step = mn ? 2048u >> 4 : 32u >> 4, lbo = mn ? 8192u : 16u;
-    const uint32_t eye = or_desc(ring + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK, 16), eye_idesc = or_idesc(16, 0);
+    const uint32_t eye = or_desc(ring + ORTHO_RING + ORTHO_STAGING, 16), eye_idesc = or_idesc<PAIR>(16, 0);
     const uint32_t tmem = S.tmem;
     bool ok = true;
     int s = 0;
-    for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const OrthoTile T = or_tile(O, kind, t);
+    for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
+        const OrthoTile T = or_tile<PAIR>(O, kind, t, 0);
         const int kblocks = or_kblocks(O, kind, T);
-        const uint32_t idesc = or_idesc(T.width, mn);
+        const uint32_t idesc = or_idesc<PAIR>(T.width, mn);
         const int eye0 = kind == OR_SQUARE ? T.c0 >> 6 : 1 << 30, eye1 = eye0 + (T.width >> 6);
         for (int k0 = 0; ok && k0 < kblocks; k0 += chunk, ++acc) {
             const uint32_t b = acc & 1u;
-            if (!or_wait(acc_empty0 + 8 * b, ((acc >> 1) & 1u) ^ 1u, &S.abort_flag)) {
+            if (!or_wait_pair<PAIR>(acc_empty0 + 8 * b, ((acc >> 1) & 1u) ^ 1u, &S.abort_flag)) {
                 ok = false;
                 break;
             }
@@ -805,7 +877,8 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
             const uint32_t d = tmem + b * 256u;
             const int k1 = min(k0 + chunk, kblocks);
             for (int kb = k0; kb < k1; ++kb) {
-                if (!or_wait(full0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag)) {
+                if (!or_wait(full0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag) ||
+                    (PAIR && !or_wait_pair<PAIR>(peer0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag))) {
                     ok = false;
                     break;
                 }
@@ -817,38 +890,38 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
                         const uint32_t dd = d + (uint32_t)kb * 64u + ks * 16;
-                        if (PRECISE) or_mma(dd, al + ks * 2, eye, eye_idesc, 0u);
-                        or_mma(dd, a + ks * 2, eye, eye_idesc, PRECISE);
+                        if (PRECISE) or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 0u);
+                        or_mma<PAIR>(dd, a + ks * 2, eye, eye_idesc, PRECISE);
                     }
                 } else {
                     // the small products first: they are added to a small sum
                     uint32_t more = kb > k0;
                     if (PRECISE) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma(d, al + ks * 2, bh + ks * b_step, idesc, more);
+                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma<PAIR>(d, al + ks * 2, bh + ks * b_step, idesc, more);
                     }
                     if (G.pb == 2) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma(d, a + ks * 2, bl + ks * b_step, idesc, more);
+                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma<PAIR>(d, a + ks * 2, bl + ks * b_step, idesc, more);
                     }
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma(d, a + ks * 2, bh + ks * b_step, idesc, more);
+                    for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma<PAIR>(d, a + ks * 2, bh + ks * b_step, idesc, more);
                     if (kb >= eye0 && kb < eye1) {
                         // c A A + b A = c (A A + A (b / c) I): this k-block's columns once more, 16 at a time,
                         // against a scaled identity
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks) {
                             const uint32_t dd = d + (uint32_t)(kb - eye0) * 64u + ks * 16;
-                            or_mma(dd, a + ks * 2, eye, eye_idesc, 1u);
-                            or_mma(dd, a + ks * 2, eye + 2, eye_idesc, 1u);
-                            if (PRECISE) or_mma(dd, al + ks * 2, eye, eye_idesc, 1u);
+                            or_mma<PAIR>(dd, a + ks * 2, eye, eye_idesc, 1u);
+                            or_mma<PAIR>(dd, a + ks * 2, eye + 2, eye_idesc, 1u);
+                            if (PRECISE) or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 1u);
                         }
                     }
                 }
-                or_commit(empty0 + 8 * s);
+                or_commit<PAIR>(empty0 + 8 * s);
                 if (++s == G.stages) s = 0;
             }
-            if (ok) or_commit(acc_full0 + 8 * b);
+            if (ok) or_commit<PAIR>(acc_full0 + 8 * b);
         }
     }
     if (!ok) {
@@ -857,44 +930,86 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
     }
 }
 
-// An epilogue warp, one phase: a quarter of the rows, a 64-column part of each tile.
+// The same warp of a pair's second block: tells the first when a stage's copies have landed here.
 template <bool PRECISE>
-__device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int e,
+__device__ __forceinline__ void or_relay(const OrthoArgs& O, OrthoShared& S, int kind, uint32_t& pipe) {
+    constexpr bool PAIR = true;
+    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const uint32_t full0 = or_smem(&S.full[0]), peer0 = or_smem(&S.peer[0]);
+    bool ok = true;
+    int s = 0;
+    for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
+        const int kblocks = or_kblocks(O, kind, or_tile<PAIR>(O, kind, t, 1));
+        for (int kb = 0; kb < kblocks; ++kb) {
+            if (!or_wait(full0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag)) {
+                ok = false;
+                break;
+            }
+            pipe ^= 1u << s;
+            or_arrive_first(peer0 + 8 * s);
+            if (++s == G.stages) s = 0;
+        }
+    }
+    if (!ok) {
+        atomicCAS(O.error, 0u, 6u);
+        S.abort_flag = 1;
+    }
+}
+
+// An epilogue warp, one phase: a quarter of the rows, one or (tiles wider than 128) two groups of 64
+// columns of each tile.
+template <bool PRECISE, bool PAIR>
+__device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int rank, int e,
                                            uint32_t& acc) {
     const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, part = e >> 2;
     const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
     const int bn = kind == OR_UPDATE ? O.bn_upd : O.bn_sym;
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
     const int chunk = PRECISE && !(kind == OR_SQUARE && O.c == 0.0f) ? 1 : 1 << 20;
-    // with tiles one part wide the other parts' staging blocks are free
-    const int blocks = bn == 64 ? ORTHO_EPI_WARPS / 4 : 1;
-    const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * ORTHO_BLOCK;
-    const uint32_t taddr0 = S.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * 64);
+    const int group0 = bn > 128 ? 2 * part : part;
+    const int blocks = bn == 64 ? 4 : 2;
+    const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * (2u * ORTHO_BLOCK);
+    const uint32_t taddr0 = S.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(group0 * 64);
     bool ok = true;
-    for (int64_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const OrthoTile T = or_tile(O, kind, t);
-        const bool mine = part < (T.width >> 6);
+    for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
+        const OrthoTile T = or_tile<PAIR>(O, kind, t, rank);
+        const int groups = min(bn > 128 ? 2 : 1, (T.width >> 6) - group0);
         const int chunks = (or_kblocks(O, kind, T) - 1) / chunk + 1;
-        float v[64];
+        float v[128];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] = 0.0f;
+        for (int j = 0; j < 128; ++j) v[j] = 0.0f;
         for (int k = 0; k < chunks; ++k, ++acc) {
             const uint32_t b = acc & 1u;
             ok = __all_sync(0xffffffffu, or_wait(acc_full0 + 8 * b, (acc >> 1) & 1u, &S.abort_flag));
             if (!ok) break;
             or_fence_after();
-            if (mine) {
-                or_tmem_add32(taddr0 + b * 256u, v);
-                or_tmem_add32(taddr0 + b * 256u + 32, v + 32);
+            if (groups > 0) {
+#pragma unroll
+                for (int j = 0; j < 64; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
+            }
+            if (groups > 1) {
+#pragma unroll
+                for (int j = 64; j < 128; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
             }
             or_fence_before();
             __syncwarp();
-            if (lane == 0) or_arrive(acc_empty0 + 8 * b);
+            if (lane == 0) {
+                if (PAIR) or_arrive_first(acc_empty0 + 8 * b);
+                else or_arrive(acc_empty0 + 8 * b);
+            }
         }
-        if (ok && mine) {
-            const int row = T.i * 128 + quad * 32 + lane, cb = (T.c0 >> 6) + part;
-            if (kind == OR_UPDATE && step == O.steps - 1) or_finish_out(O, T.which, row, cb, blk, lane, v);
-            else or_finish<PRECISE>(O, kind, step, T.which, T.i, row, cb, blk, blocks, lane, v);
+        int m, n;
+        if (O.list) m = O.list[T.which].m, n = O.list[T.which].n;
+        else m = O.one.m, n = O.one.n;
+        const int row = T.i * 128 + quad * 32 + lane;
+        const int last_cb = or_b64(kind == OR_UPDATE ? n : m);  // a pair's tile may reach past the matrix
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int cb = (T.c0 >> 6) + group0 + g;
+            if (!ok || g >= groups || (PAIR && (cb >= last_cb || T.i >= or_mb(m)))) continue;
+            if (kind == OR_UPDATE && step == O.steps - 1) or_finish_out(O, T.which, row, cb, blk, lane, v + 64 * g);
+            else or_finish<PRECISE>(O, kind, step, T.which, T.i, row, cb, blk, blocks, lane, v + 64 * g);
         }
     }
     if (!ok) {
@@ -907,8 +1022,10 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
 }
 
 // The steps' products: per step the Gram matrix, its polynomial and the update, a phase each over all
-// matrices, each role running through the phases on its own.
-template <bool PRECISE>
+// matrices, each role running through the phases on its own.  PAIR: launched in clusters of two blocks, which
+// work on tiles of 256 rows together (a block's own row block, half of the columns' operand each, the first
+// block issuing), a third fewer bytes to fetch per product.
+template <bool PRECISE, bool PAIR>
 __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const __grid_constant__ OrthoArgs O) {
     // the first kilobyte holds the barriers; the ring after it starts on the 1024 bytes of a swizzle atom
     extern __shared__ __align__(1024) unsigned char or_raw[];
@@ -921,73 +1038,90 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
     }
     if (!O.x && *O.bad) return;  // the transition leaves everything as it was
     const int warp = threadIdx.x >> 5;
+    const int rank = PAIR ? (int)or_cluster_rank() : 0;
     if (threadIdx.x == 0) {
         S.abort_flag = 0;
         for (int s = 0; s < ORTHO_STAGES; ++s) {
             or_mbar_init(or_smem(&S.full[s]), ORTHO_PRODUCERS);
             or_mbar_init(or_smem(&S.empty[s]), 1);
+            or_mbar_init(or_smem(&S.peer[s]), 1);
         }
         for (int b = 0; b < 2; ++b) {
             or_mbar_init(or_smem(&S.acc_full[b]), 1);
-            or_mbar_init(or_smem(&S.acc_empty[b]), ORTHO_EPI_WARPS);
+            or_mbar_init(or_smem(&S.acc_empty[b]), PAIR ? 2 * ORTHO_EPI_WARPS : ORTHO_EPI_WARPS);
         }
         or_mbar_init(or_smem(&S.done), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x >= 128 && threadIdx.x < 256) {
-        // 16 rows x 8 chunks of 16 bytes, swizzled: chunks 0-1 hold hi (columns 0-15), chunks 2-3 lo
+        // 16 rows x 8 chunks of 16 bytes, swizzled: chunks 0-1 hold hi (columns 0-15), chunks 2-3 lo; of a pair
+        // each block has eight of the identity's rows
         const int r = (threadIdx.x - 128) >> 3, chunk = (threadIdx.x - 128) & 7;
         const float value = O.c != 0.0f ? O.b / O.c * ORTHO_SA : ORTHO_SA;
         __align__(16) __half h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             __half hi, lo;
-            or_split((chunk & 1) * 8 + e == r ? value : 0.0f, hi, lo);
+            or_split((chunk & 1) * 8 + e == r + 8 * rank ? value : 0.0f, hi, lo);
             h[e] = chunk < 2 ? hi : chunk < 4 ? lo : __float2half_rn(0.0f);
         }
-        unsigned char* at = or_raw + 1024 + ORTHO_RING + ORTHO_EPI_WARPS * ORTHO_BLOCK + r * 128 + ((chunk ^ (r & 7)) << 4);
+        unsigned char* at = or_raw + 1024 + ORTHO_RING + ORTHO_STAGING + r * 128 + ((chunk ^ (r & 7)) << 4);
         *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(h);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(or_smem(&S.tmem)), "r"(512u)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(or_smem(&S.tmem)), "r"(512u)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(or_smem(&S.tmem)), "r"(512u)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     or_fence_before();
     __syncthreads();
+    if (PAIR) or_cluster_sync();  // both blocks' barriers are there
     or_fence_after();
     const int phases = 3 * O.steps;
     uint32_t pipe = 0, acc = 0;
     if (warp == 0) {
         for (int p = 0; p < phases; ++p) {
-            if (or_elect()) or_issue<PRECISE>(O, S, ring, p % 3, p / 3, pipe, acc);
+            if (or_elect()) {
+                if (PAIR && rank) or_relay<PRECISE>(O, S, p % 3, pipe);
+                else or_issue<PRECISE, PAIR>(O, S, ring, p % 3, pipe, acc);
+            }
             __syncwarp();
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     } else if (warp <= ORTHO_PRODUCERS) {
         for (int p = 0; p < phases; ++p) {
-            if (or_elect()) or_produce<PRECISE>(O, S, ring, p % 3, p / 3, warp - 1, pipe);
+            if (or_elect()) or_produce<PRECISE, PAIR>(O, S, ring, p % 3, p / 3, rank, warp - 1, pipe);
             __syncwarp();
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     } else {
         for (int p = 0; p < phases; ++p) {
-            or_collect<PRECISE>(O, S, ring, p % 3, p / 3, warp - 1 - ORTHO_PRODUCERS, acc);
+            or_collect<PRECISE, PAIR>(O, S, ring, p % 3, p / 3, rank, warp - 1 - ORTHO_PRODUCERS, acc);
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     }
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 0 && !(PAIR && rank)) {
         if (or_elect()) {
             // nothing that this thread issued is under way when the memory is freed
-            or_commit(or_smem(&S.done));
+            or_commit<PAIR>(or_smem(&S.done));
             for (uint32_t i = 0; i < ORTHO_WAIT_TRIES && !or_try_wait(or_smem(&S.done), 0u); ++i) {
             }
         }
         __syncwarp();
+    }
+    if (PAIR) or_cluster_sync();  // neither block's shared memory or accumulators are in use any more
+    if (warp == 0) {
         or_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(S.tmem), "r"(512u) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(S.tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(S.tmem), "r"(512u) : "memory");
     }
 }
 
@@ -998,12 +1132,14 @@ constexpr int ORTHO_SINGLE = 512;
 
 static int64_t or_tiles_bytes(int m, int n) { return 2 * or_x_bytes(m, n) + 2 * or_a_bytes(m); }
 static int64_t or_spans(int64_t total) { return (total + ORTHO_SPAN - 1) / ORTHO_SPAN; }
-static int64_t or_syms(int m, int bn) {
+static int64_t or_syms(int m, int bn, int pair) {
     int64_t n = 0;
-    for (int i = 0; i < or_mb(m); ++i) n += or_sym_row(m, i, bn);
+    for (int i = 0; i < or_row_blocks(m, pair); ++i) n += or_sym_row(m, i, bn, pair);
     return n;
 }
-static int64_t or_upds(int m, int n, int bn) { return (int64_t)or_mb(m) * ((or_b64(n) * 64 + bn - 1) / bn); }
+static int64_t or_upds(int m, int n, int bn, int pair) {
+    return (int64_t)or_row_blocks(m, pair) * ((or_b64(n) * 64 + bn - 1) / bn);
+}
 
 static OrthoDesc or_make(int64_t rows, int64_t cols) {
     OrthoDesc d = {};
@@ -1014,33 +1150,36 @@ static OrthoDesc or_make(int64_t rows, int64_t cols) {
     return d;
 }
 
-// Output tile width, by an estimate of the busiest SM's cycles: a k-block of 64 costs 12 instructions of
-// 48, 64 or 96 cycles at widths 64, 128 and 192 (the narrowest wait for shared memory), an output tile some
-// 1,500 cycles and 6 a column to finish.  Wide tiles read less per multiply-add, narrow ones spread a few
-// small matrices over more SMs.
+// Output tile shapes, by an estimate of the busiest block's cycles: a k-block of 64 and an output tile's end
+// cost what they were measured to on matrices of 4,096 (k-blocks) and of 256 x 1,024 (ends): 128 x 64, x 128
+// and x 192 by one block, 256 x 256 by a pair.  Wide tiles fetch less per multiply-add, narrow ones spread a
+// few small matrices over more SMs.
 struct OrthoWidths {
-    double sum[2][3], top[2][3];
+    double sum[2][4], top[2][4];
 };
-static const int OR_WIDTHS[3] = {64, 128, 192};
+static const int OR_WIDTHS[4] = {64, 128, 192, 256};
 static void or_weigh(OrthoWidths& W, int m, int n, int64_t count) {
-    static const double block[3] = {576.0, 768.0, 1152.0};
-    for (int w = 0; w < 3; ++w)
+    static const double block[4] = {850.0, 1400.0, 2200.0, 1900.0}, end[4] = {3500.0, 4000.0, 5500.0, 6500.0};
+    for (int w = 0; w < 4; ++w)
         for (int kind = 0; kind < 2; ++kind) {
-            const int bn = OR_WIDTHS[w];
-            // the Gram matrix (kind 0) is the longer of the two symmetric products
-            const double cost = (kind == 0 ? or_b64(n) : or_b64(m)) * block[w] + 1500.0 + 6.0 * bn;
-            W.sum[kind][w] += cost * (double)count * (double)(kind == 0 ? or_syms(m, bn) : or_upds(m, n, bn));
+            const int bn = OR_WIDTHS[w], pair = w == 3;
+            // kind 0: the Gram matrix and its square together
+            const double cost = kind == 0 ? (or_b64(n) + or_b64(m)) * block[w] + 2 * end[w] : or_b64(m) * block[w] + end[w];
+            W.sum[kind][w] += cost * (double)count * (double)(kind == 0 ? or_syms(m, bn, pair) : or_upds(m, n, bn, pair)) * (pair ? 2 : 1);
             if (cost > W.top[kind][w]) W.top[kind][w] = cost;
         }
 }
-static int or_width(const OrthoWidths& W, int kind) {
-    int best = 0;
-    double least = 0.0;
-    for (int w = 0; w < 3; ++w) {
-        const double cost = W.sum[kind][w] / sm_count() + W.top[kind][w];
-        if (w == 0 || cost < least) best = w, least = cost;
+static double or_cost(const OrthoWidths& W, int kind, int w) { return W.sum[kind][w] / sm_count() + 0.75 * W.top[kind][w]; }
+static void or_choose(const OrthoWidths& W, int& bn_sym, int& bn_upd, int& pair) {
+    int best[2];
+    for (int kind = 0; kind < 2; ++kind) {
+        best[kind] = 0;
+        for (int w = 1; w < 3; ++w)
+            if (or_cost(W, kind, w) < or_cost(W, kind, best[kind])) best[kind] = w;
     }
-    return OR_WIDTHS[best];
+    bn_sym = OR_WIDTHS[best[0]], bn_upd = OR_WIDTHS[best[1]];
+    pair = or_cost(W, 0, 3) + or_cost(W, 1, 3) < or_cost(W, 0, best[0]) + or_cost(W, 1, best[1]);
+    if (pair) bn_sym = bn_upd = 256;
 }
 
 static int64_t or_up(int64_t v) { return (v + 1023) / 1024 * 1024; }
@@ -1053,18 +1192,17 @@ static int or_squares(const OrthoArgs& O, cudaStream_t s) {
 
 // conversion, then the products
 static int or_products(const OrthoArgs& O, cudaStream_t s) {
-    const void* kernel = O.precise ? (const void*)orthogonalize_kernel<true> : (const void*)orthogonalize_kernel<false>;
+    const void* const kernels[4] = {(const void*)orthogonalize_kernel<false, false>, (const void*)orthogonalize_kernel<true, false>,
+                                    (const void*)orthogonalize_kernel<false, true>, (const void*)orthogonalize_kernel<true, true>};
     static int configured[64] = {0};
-    int dev = 0;
+    int dev = 0, rc = 0;
     cudaGetDevice(&dev);
-    int rc = 0;
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        rc = cuda_status(cudaFuncSetAttribute(orthogonalize_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
-                         "orthogonalize: shared memory size");
-        if (!rc)
-            rc = cuda_status(cudaFuncSetAttribute(orthogonalize_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
+        for (int i = 0; i < 4; ++i) {
+            rc = cuda_status(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
                              "orthogonalize: shared memory size");
-        if (rc) return rc;
+            if (rc) return rc;
+        }
         if (dev >= 0 && dev < 64) configured[dev] = 1;
     }
     rc = cuda_status(cudaMemsetAsync(O.barrier, 0, 4, s), "orthogonalize: barrier");
@@ -1073,10 +1211,25 @@ static int or_products(const OrthoArgs& O, cudaStream_t s) {
     orthogonalize_convert_kernel<<<(unsigned)O.convs, ORTHO_FLAT, 0, s>>>(O);
     rc = launch_status("orthogonalize: conversion");
     if (rc) return rc;
-    const int64_t want = O.syms > O.upds ? O.syms : O.upds;
-    const int grid = (int)(want < sm_count() ? want : sm_count());
+    // one block per SM, all of them running at once
+    const int64_t tiles = O.syms > O.upds ? O.syms : O.upds;
+    const int64_t most = O.pair ? sm_count() / 2 * 2 : sm_count();
+    const int64_t want = O.pair ? 2 * tiles : tiles;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(want < most ? want : most));
+    config.blockDim = dim3(ORTHO_THREADS);
+    config.dynamicSmemBytes = ORTHO_SMEM;
+    config.stream = s;
+    cudaLaunchAttribute attribute[2];
+    attribute[0].id = cudaLaunchAttributeCooperative;
+    attribute[0].val.cooperative = 1;
+    attribute[1].id = cudaLaunchAttributeClusterDimension;
+    attribute[1].val.clusterDim.x = 2;
+    attribute[1].val.clusterDim.y = attribute[1].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = O.pair ? 2 : 1;
     void* args[] = {const_cast<OrthoArgs*>(&O)};
-    return cuda_status(cudaLaunchCooperativeKernel(kernel, dim3((unsigned)grid), dim3(ORTHO_THREADS), args, (size_t)ORTHO_SMEM, s),
+    return cuda_status(cudaLaunchKernelExC(&config, kernels[(O.pair ? 2 : 0) + (O.precise ? 1 : 0)], args),
                        "orthogonalize: cooperative launch");
 }
 
@@ -1165,8 +1318,8 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
         O.count = batch - at < k ? batch - at : k;
         OrthoWidths W = {};
         or_weigh(W, m, n, O.count);
-        O.bn_sym = or_width(W, 0), O.bn_upd = or_width(W, 1);
-        O.one_sym = or_syms(m, O.bn_sym), O.one_upd = or_upds(m, n, O.bn_upd);
+        or_choose(W, O.bn_sym, O.bn_upd, O.pair);
+        O.one_sym = or_syms(m, O.bn_sym, O.pair), O.one_upd = or_upds(m, n, O.bn_upd, O.pair);
         O.spans = O.count * O.one_span, O.convs = O.count * O.one_conv;
         O.syms = O.count * O.one_sym, O.upds = O.count * O.one_upd;
         O.x = static_cast<const unsigned char*>(x) + at * rows * cols * xs;
@@ -1200,7 +1353,8 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
     });
     OrthoWidths W = {};
     for (int64_t i = 0; i < count; ++i) or_weigh(W, list[i].m, list[i].n, 1);
-    const int bn_sym = or_width(W, 0), bn_upd = or_width(W, 1);
+    int bn_sym, bn_upd, pair;
+    or_choose(W, bn_sym, bn_upd, pair);
     int64_t spans = 0, waves = 0, most = 0;
     int64_t* wave = plan + 8;
     OrthoDesc at = {};
@@ -1218,14 +1372,14 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
         spans += or_spans((int64_t)m * n);
         at.ws += bytes;
         at.conv0 += (int64_t)or_mb(m) * or_b64(n);
-        at.sym0 += or_syms(m, bn_sym);
-        at.upd0 += or_upds(m, n, bn_upd);
+        at.sym0 += or_syms(m, bn_sym, pair);
+        at.upd0 += or_upds(m, n, bn_upd, pair);
         if (at.ws > most) most = at.ws;
         wave[1] = i + 1 - wave[0], wave[2] = at.conv0, wave[3] = at.sym0, wave[4] = at.upd0;
     }
     plan[0] = 1024 + or_up(spans * 8) + most;
     plan[1] = spans, plan[2] = waves, plan[3] = bn_sym, plan[4] = bn_upd;
-    plan[5] = plan[6] = plan[7] = 0;
+    plan[5] = pair, plan[6] = plan[7] = 0;
     return 0;
 }
 
@@ -1244,7 +1398,7 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
     O.barrier = reinterpret_cast<uint32_t*>(w);
     O.sums = reinterpret_cast<double*>(w + 1024);
     O.tiles = w + 1024 + or_up(plan[1] * 8);
-    O.bn_sym = (int)plan[3], O.bn_upd = (int)plan[4];
+    O.bn_sym = (int)plan[3], O.bn_upd = (int)plan[4], O.pair = (int)plan[5];
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.precise = 1;
     O.grad = grad, O.momentum = momentum, O.master = master, O.controls = controls;
