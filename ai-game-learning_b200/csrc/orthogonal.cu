@@ -60,7 +60,9 @@ struct OrthoDesc {
     int64_t ws;      // bytes of workspace before this matrix's tiles: X, X', A, B
     int64_t span0;   // spans, conversion tiles, symmetric and update tiles of the matrices before it
     int64_t conv0, sym0, upd0;
+    int64_t slot0;   // blocks of the teams before it (short sides up to 128)
     int32_t m, n;    // short and long side
+    int32_t team;    // blocks that work on it, where its short side is at most 128; else 0
     int32_t tall;    // stored n x m
     float adjust;
 };
@@ -69,7 +71,7 @@ struct OrthoArgs {
     const OrthoDesc* list;  // device, or null: `count` matrices like `one`, `one`'s sizes apart
     OrthoDesc one;
     int64_t one_src, one_ws, one_span, one_conv, one_sym, one_upd;
-    int64_t count, spans, convs, syms, upds;  // totals
+    int64_t count, spans, convs, syms, upds, slots;  // totals
     int bn_sym, bn_upd;  // output tile widths
     int pair;            // output tiles of 256 rows, by two blocks each
     int steps, precise;  // precise: A and B as pairs
@@ -134,8 +136,9 @@ __device__ __forceinline__ void or_bulk_load(uint32_t dst, const void* src, uint
 }
 // 128-byte-swizzled operand: K-major (rows of 128 bytes, 8-row atoms 1024 bytes apart), or MN-major (64
 // columns of 8 k-rows an atom, the next k-rows 1024 bytes on, the next 64 columns `lbo` bytes on).  The low
-// word of the descriptor, whose high word is the same for both.
-__device__ __forceinline__ uint32_t or_desc(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+// word of the descriptor, whose high word is the same for both.  (The address masked: in a cluster a block's
+// shared addresses carry its rank above.)
+__device__ __forceinline__ uint32_t or_desc(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | ((lbo >> 4) << 16); }
 // kind::f16: fp16 x fp16 -> fp32, M 128 or (pair) 256, A K-major, B K-major or MN-major
 template <bool PAIR>
 __device__ __forceinline__ uint32_t or_idesc(int n, int mn_major) {
@@ -211,6 +214,7 @@ __device__ __forceinline__ bool or_wait_pair(uint32_t bar, uint32_t parity, vola
     return false;
 }
 __device__ __forceinline__ void or_cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t or_cluster_rank() {
@@ -244,6 +248,7 @@ __device__ __forceinline__ OrthoDesc or_get(const OrthoArgs& O, int64_t i) {
     d.conv0 = i * O.one_conv;
     d.sym0 = i * O.one_sym;
     d.upd0 = i * O.one_upd;
+    d.slot0 = i * d.team;
     return d;
 }
 
@@ -737,21 +742,19 @@ struct OrthoShared {
 };
 
 // Between two phases: every role of every block arrives (the launch is cooperative, so all blocks run);
-// bounded.  False when the wait, or a role, gave up.
+// bounded.  False when the wait, or a role of any block, gave up (the word's top bit).
 __device__ __forceinline__ bool or_phase_end(const OrthoArgs& O, OrthoShared& S, uint32_t phases) {
     asm volatile("fence.proxy.async;" ::: "memory");
     asm volatile("bar.sync 1, %0;" ::"n"(ORTHO_THREADS) : "memory");
     if (threadIdx.x == 0) {
         const uint32_t target = phases * gridDim.x;
-        __threadfence();
-        uint32_t seen = atomicAdd(O.barrier, 1u) + 1u;
-        for (uint32_t i = 0; (int32_t)(seen - target) < 0 && i < ORTHO_WAIT_TRIES; ++i)
+        if (S.abort_flag) atomicOr(O.barrier, 0x80000000u);
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(O.barrier) : "memory");
+        uint32_t seen = 0;
+        for (uint32_t i = 0; seen < target && i < ORTHO_WAIT_TRIES; ++i)
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(O.barrier) : "memory");
-        const bool ok = (int32_t)(seen - target) >= 0;
-        if (!ok) atomicCAS(O.error, 0u, 4u);
-        __threadfence();
-        // no phase after one that any block gave up
-        S.ok = ok && !S.abort_flag && *reinterpret_cast<volatile uint32_t*>(O.error) == 0u;
+        if (seen < target) atomicCAS(O.error, 0u, 4u);
+        S.ok = seen >= target && !(seen & 0x80000000u);
     }
     asm volatile("bar.sync 1, %0;" ::"n"(ORTHO_THREADS) : "memory");
     asm volatile("fence.proxy.async;" ::: "memory");
@@ -1125,12 +1128,416 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
     }
 }
 
+// ------------------------------------------------------------ short sides up to 128
+
+// A matrix whose short side is at most 128 stays in shared memory: a team of 1, 2, 4 or 8 blocks of a
+// cluster holds up to three 64-column tiles of X each (long sides up to 1,536), and A and B whole.  A step
+// is the team's Gram matrices of its columns, summed over the team (each block the rows that are its share,
+// in rank order, and handed to all), the polynomial, which every block takes for itself, and the update of
+// its own columns: no pass through L2 and no grid barrier, about a third of the time of the general path on
+// a few such matrices.  A cluster is as large as the largest team; smaller teams share clusters and take
+// part in all of the cluster's barriers.
+constexpr int ORTHO_TEAM_TILES = 3;
+constexpr int ORTHO_TEAM_MAX = 8;
+constexpr int ORTHO_TEAM_A = 2 * ORTHO_TILE;           // A, then B: 128 x 128
+constexpr int ORTHO_TEAM_SUM = 128 * 128 * 4;          // a block's own Gram matrix, fp32; then staging
+constexpr int ORTHO_TEAM_SMEM = 1024 + ORTHO_TEAM_TILES * ORTHO_TILE + ORTHO_TEAM_A + ORTHO_TEAM_SUM + ORTHO_EYE;
+
+struct OrthoTeam {
+    uint64_t acc_full[2], acc_empty[2], done;
+    double squares[ORTHO_TEAM_MAX];
+    double part[ORTHO_THREADS / 32];
+    uint32_t tmem;
+    volatile int abort_flag;
+};
+
+__device__ __forceinline__ uint32_t or_map(uint32_t addr, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
+}
+
+// 64 finished values of a row to a tile in shared memory, hi and lo
+__device__ __forceinline__ void or_keep_rows(uint32_t tile, int row, const float* v) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x0 = v[8 * q + 2 * j], x1 = v[8 * q + 2 * j + 1];
+            const __half2 h = __floats2half2_rn(x0, x1);
+            const float2 f = __half22float2(h);
+            const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
+            hi[j] = *reinterpret_cast<const uint32_t*>(&h);
+            lo[j] = *reinterpret_cast<const uint32_t*>(&l);
+        }
+        const uint32_t at = tile + (uint32_t)row * 128u + (uint32_t)((q ^ (row & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + 16384u), "r"(lo[0]), "r"(lo[1]), "r"(lo[2]), "r"(lo[3]) : "memory");
+    }
+}
+
+__global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(const __grid_constant__ OrthoArgs O, int cluster) {
+    extern __shared__ __align__(1024) unsigned char or_raw[];
+    OrthoTeam& S = *reinterpret_cast<OrthoTeam*>(or_raw);
+    static_assert(sizeof(OrthoTeam) <= 1024, "shared state fits its kilobyte");
+    const uint32_t xs = or_smem(or_raw) + 1024u;
+    const uint32_t as = xs + ORTHO_TEAM_TILES * ORTHO_TILE, sums = as + ORTHO_TEAM_A, eye_at = sums + ORTHO_TEAM_SUM;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (xs & 1023u) {  // never: dynamic shared memory alone starts on a kilobyte
+        atomicCAS(O.error, 0u, 5u);
+        return;
+    }
+    if (!O.x && *O.bad) {  // the transition leaves everything as it was but the gradients
+        if (blockIdx.x < O.slots) {
+            const OrthoDesc d = or_get(O, or_find(O, blockIdx.x, &OrthoDesc::slot0, O.one.team));
+            const int64_t total = (int64_t)d.m * d.n;
+            for (int64_t i = (int64_t)(blockIdx.x - d.slot0) * ORTHO_THREADS + threadIdx.x; i < total; i += (int64_t)d.team * ORTHO_THREADS)
+                O.grad[d.src + i] = 0.0f;
+        }
+        return;
+    }
+    const bool here = blockIdx.x < O.slots;  // the last cluster may have blocks to spare
+    OrthoDesc d = {};
+    int which = 0, rank = 0;
+    if (here) {
+        which = (int)or_find(O, blockIdx.x, &OrthoDesc::slot0, O.one.team);
+        d = or_get(O, which);
+        rank = (int)(blockIdx.x - d.slot0);
+    } else {
+        d.team = 1;
+    }
+    const int nb = or_b64(d.n), m64 = or_b64(d.m), team = d.team;
+    const int each = (nb + team - 1) / team;                        // tiles of a block
+    const int first = rank * each;                                  // its first column block
+    const int tiles = max(0, min(each, nb - first));
+    const int base = cluster > 1 ? (int)or_cluster_rank() - rank : 0;  // the team's first block in the cluster
+
+    if (threadIdx.x == 0) {
+        S.abort_flag = 0;
+        for (int b = 0; b < 2; ++b) {
+            or_mbar_init(or_smem(&S.acc_full[b]), 1);
+            or_mbar_init(or_smem(&S.acc_empty[b]), ORTHO_EPI_WARPS);
+        }
+        or_mbar_init(or_smem(&S.done), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x >= 128 && threadIdx.x < 256) {
+        const int r = (threadIdx.x - 128) >> 3, chunk = (threadIdx.x - 128) & 7;
+        const float value = O.c != 0.0f ? O.b / O.c * ORTHO_SA : ORTHO_SA;
+        __align__(16) __half h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            __half hi, lo;
+            or_split((chunk & 1) * 8 + e == r ? value : 0.0f, hi, lo);
+            h[e] = chunk < 2 ? hi : chunk < 4 ? lo : __float2half_rn(0.0f);
+        }
+        *reinterpret_cast<uint4*>(or_raw + (eye_at - or_smem(or_raw)) + r * 128 + ((chunk ^ (r & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(or_smem(&S.tmem)), "r"(512u)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // ---------------------------------------------------- the direction, its norm, and X
+    const OrthoDirection k = or_controls(O);
+    const bool vector = O.aligned && d.src % 4 == 0 && d.n % 4 == 0;
+    constexpr int ROUNDS = ORTHO_TEAM_TILES * 1024 / ORTHO_THREADS;  // chunks of 8 columns a thread
+    static_assert(ROUNDS * ORTHO_THREADS == ORTHO_TEAM_TILES * 1024, "the chunks divide evenly");
+    {
+        double square = 0.0;
+        float u[ROUNDS][8];
+#pragma unroll
+        for (int h = 0; h < ROUNDS; ++h) {
+            const int q = h * ORTHO_THREADS + threadIdx.x, t = q >> 10, c = q & 1023;
+            const int row = d.tall ? c & 127 : c >> 3, chunk = d.tall ? c >> 7 : c & 7;
+            const int col = (first + t) * 64 + chunk * 8;
+            const int live = t < tiles && row < d.m ? max(0, min(8, d.n - col)) : 0;
+            const int64_t i = d.src + (d.tall ? (int64_t)col * d.m + row : (int64_t)row * d.n + col);
+            const int64_t next = d.tall ? d.m : 1;
+            const void* src = O.x ? O.x : O.grad;
+            const int type = O.x ? O.x_type : 0;
+            float m[8];
+            if (d.tall) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    u[h][e] = e < live ? or_load(src, type, i + e * next) : 0.0f;
+                    if (!O.x) m[e] = e < live ? O.momentum[i + e * next] : 0.0f;
+                }
+            } else {
+                or_load8(src, type, i, vector, live, u[h]);
+                if (!O.x) or_load8(O.momentum, 0, i, vector, live, m);
+            }
+            if (!O.x) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    m[e] = or_momentum(k, u[h][e], m[e]);
+                    u[h][e] = or_direction(k, u[h][e], m[e]);
+                }
+                if (!d.tall && vector && live >= 8) {
+                    float4* p = reinterpret_cast<float4*>(O.momentum + i);
+                    p[0] = make_float4(m[0], m[1], m[2], m[3]);
+                    p[1] = make_float4(m[4], m[5], m[6], m[7]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < live) O.momentum[i + e * next] = m[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) square += (double)u[h][e] * (double)u[h][e];
+            }
+        }
+        double total = 0.0;
+        if (O.x) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+            if (lane == 0) S.part[warp] = square;
+            if (cluster > 1) or_cluster_sync();  // the others run: their shared memory may be written
+            else __syncthreads();
+            if (threadIdx.x < team) {
+                double own = 0.0;
+                for (int w = 0; w < ORTHO_THREADS / 32; ++w) own += S.part[w];
+                const uint32_t at = or_smem(&S.squares[rank]);
+                if (team == 1) S.squares[0] = own;
+                else asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(or_map(at, base + (int)threadIdx.x)), "d"(own) : "memory");
+            }
+            if (cluster > 1) or_cluster_sync();
+            else __syncthreads();
+            for (int r = 0; r < team; ++r) total += S.squares[r];
+        } else {
+            const int64_t spans = ((int64_t)d.m * d.n + ORTHO_SPAN - 1) / ORTHO_SPAN;
+            for (int64_t r = 0; r < spans; ++r) total += __ldg(O.sums + d.span0 + r);
+        }
+        const double wide = (double)ORTHO_SX / (sqrt(total) + O.eps);
+        const float scale = (float)wide;
+        const bool plain = scale < 1.0e30f;
+#pragma unroll
+        for (int h = 0; h < ROUNDS; ++h) {
+            const int q = h * ORTHO_THREADS + threadIdx.x, t = q >> 10, c = q & 1023;
+            const int row = d.tall ? c & 127 : c >> 3, chunk = d.tall ? c >> 7 : c & 7;
+            const int col = (first + t) * 64 + chunk * 8;
+            if (t < tiles) {
+                __align__(16) __half hi[8];
+                __align__(16) __half lo[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool in = row < d.m && col + e < d.n;
+                    or_split(in ? (plain ? u[h][e] * scale : (float)((double)u[h][e] * wide)) : 0.0f, hi[e], lo[e]);
+                }
+                unsigned char* at = or_raw + 1024 + t * ORTHO_TILE + row * 128 + ((chunk ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(hi);
+                *reinterpret_cast<uint4*>(at + 16384) = *reinterpret_cast<uint4*>(lo);
+            }
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    or_fence_before();
+    __syncthreads();
+    or_fence_after();
+
+    // ---------------------------------------------------- the steps
+    const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
+    const uint32_t tmem = S.tmem;
+    const int e = warp - 1 - ORTHO_PRODUCERS, quad = warp & 3, part = e >> 2;  // epilogue warps
+    const int row = quad * 32 + lane;
+    uint32_t acc = 0;
+    for (int step = 0; step < O.steps; ++step) {
+        for (int kind = 0; kind < 3; ++kind) {
+            const bool linear = kind == OR_SQUARE && O.c == 0.0f;
+            const int kblocks = tiles == 0 && kind != OR_SQUARE ? 0 : kind == OR_GRAM ? tiles : m64;
+            const int groups_all = kind == OR_UPDATE ? tiles : m64;  // 64-column groups of the product
+            float v[128];
+#pragma unroll
+            for (int j = 0; j < 128; ++j) v[j] = 0.0f;
+            const int per = kind == OR_UPDATE ? 2 : 1;  // groups an epilogue warp takes
+            const int group0 = part * per, groups = min(per, groups_all - group0);
+            bool ok = true;
+            if (warp == 0) {
+                if (or_elect()) {
+                    const uint32_t idesc = or_idesc<false>(groups_all * 64, kind == OR_UPDATE), eye_idesc = or_idesc<false>(16, 0);
+                    const uint32_t eye = or_desc(eye_at, 16);
+                    for (int kb = 0; kb < kblocks; ++kb) {
+                        // K-major operands: column block kb of X or A against the same rows; the update: column
+                        // block kb of B against rows 64 kb of X, its column blocks a tile apart
+                        const uint32_t b = acc & 1u;
+                        if (!linear || kb == 0) {
+                            if (!or_wait(acc_empty0 + 8 * b, ((acc >> 1) & 1u) ^ 1u, &S.abort_flag)) {
+                                ok = false;
+                                break;
+                            }
+                            or_fence_after();
+                        }
+                        const uint32_t dd = tmem + b * 256u;
+                        const uint32_t at = (kind == OR_GRAM ? xs : as) + (uint32_t)kb * ORTHO_TILE;
+                        const uint32_t a = or_desc(at, 16), al = a + (16384u >> 4);
+                        const uint32_t bh = kind == OR_UPDATE ? or_desc(xs + (uint32_t)kb * 8192u, ORTHO_TILE) : a;
+                        const uint32_t bl = bh + (16384u >> 4), b_step = kind == OR_UPDATE ? 2048u >> 4 : 2u;
+                        if (!linear) {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) or_mma<false>(dd, al + ks * 2, bh + ks * b_step, idesc, ks > 0);
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) or_mma<false>(dd, a + ks * 2, bl + ks * b_step, idesc, 1u);
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) or_mma<false>(dd, a + ks * 2, bh + ks * b_step, idesc, 1u);
+                        }
+                        if (kind == OR_SQUARE) {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) {
+                                const uint32_t dc = dd + (uint32_t)kb * 64u + ks * 16;
+                                or_mma<false>(dc, al + ks * 2, eye, eye_idesc, !linear);
+                                or_mma<false>(dc, a + ks * 2, eye, eye_idesc, 1u);
+                                if (!linear) or_mma<false>(dc, a + ks * 2, eye + 2, eye_idesc, 1u);
+                            }
+                        }
+                        if (!linear || kb == kblocks - 1) {
+                            or_commit<false>(acc_full0 + 8 * b);
+                            ++acc;
+                        }
+                    }
+                    if (!ok) {
+                        atomicCAS(O.error, 0u, 2u);
+                        S.abort_flag = 1;
+                    }
+                }
+                __syncwarp();
+            } else if (e >= 0) {
+                const int chunks = linear ? (kblocks > 0) : kblocks;
+                const uint32_t taddr0 = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(group0 * 64);
+                for (int c = 0; c < chunks; ++c, ++acc) {
+                    const uint32_t b = acc & 1u;
+                    ok = __all_sync(0xffffffffu, or_wait(acc_full0 + 8 * b, (acc >> 1) & 1u, &S.abort_flag));
+                    if (!ok) break;
+                    or_fence_after();
+                    if (groups > 0) {
+#pragma unroll
+                        for (int j = 0; j < 64; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
+                    }
+                    if (groups > 1) {
+#pragma unroll
+                        for (int j = 64; j < 128; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
+                    }
+                    or_fence_before();
+                    __syncwarp();
+                    if (lane == 0) or_arrive(acc_empty0 + 8 * b);
+                }
+                if (!ok) {
+                    if (lane == 0) atomicCAS(O.error, 0u, 3u);
+                    S.abort_flag = 1;
+                }
+                if (kind == OR_GRAM) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) v[j] *= ORTHO_SA / (ORTHO_SX * ORTHO_SX);
+                    if (team == 1) {
+                        if (groups > 0) or_keep_rows(as + part * ORTHO_TILE, row, v);
+                    } else if (part < m64) {
+                        // 32 chunks of four columns a row, swizzled by the row
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) {
+                            const uint32_t at = sums + (uint32_t)row * 512u + (uint32_t)(((part * 16 + q) ^ lane) << 4);
+                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[4 * q]), "f"(v[4 * q + 1]),
+                                         "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
+                                         : "memory");
+                        }
+                    }
+                } else if (kind == OR_SQUARE) {
+                    const float factor = (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA)), diagonal = O.a * ORTHO_SB;
+                    if (groups > 0) {
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == part * 64 + j ? diagonal : 0.0f);
+                        or_keep_rows(as + part * ORTHO_TILE, row, v);
+                    }
+                } else if (step + 1 < O.steps) {
+#pragma unroll
+                    for (int j = 0; j < 128; ++j) v[j] *= 1.0f / ORTHO_SB;
+                    if (groups > 0) or_keep_rows(xs + group0 * ORTHO_TILE, row, v);
+                    if (groups > 1) or_keep_rows(xs + (group0 + 1) * ORTHO_TILE, row, v + 64);
+                } else if (ok) {
+                    if (groups > 0) or_finish_out(O, which, row, first + group0, sums + (uint32_t)e * ORTHO_BLOCK, lane, v);
+                    if (groups > 1) or_finish_out(O, which, row, first + group0 + 1, sums + (uint32_t)e * ORTHO_BLOCK, lane, v + 64);
+                }
+            }
+            __syncwarp();
+            if (kind == OR_GRAM && cluster > 1) {
+                or_cluster_sync();
+                if (team > 1) {
+                    // this block's rows, summed over the team in rank order, as pairs to every block of the team
+                    const int rows = 128 / team;
+                    for (int q = threadIdx.x; q < rows * 32; q += ORTHO_THREADS) {
+                        const int r = rank * rows + (q >> 5), chunk = q & 31;  // four columns
+                        if (chunk >= m64 * 16) continue;
+                        const uint32_t at = sums + (uint32_t)r * 512u + (uint32_t)((chunk ^ (r & 31)) << 4);
+                        float4 t[ORTHO_TEAM_MAX];
+#pragma unroll
+                        for (int j = 0; j < ORTHO_TEAM_MAX; ++j)
+                            if (j < team)
+                                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                             : "=f"(t[j].x), "=f"(t[j].y), "=f"(t[j].z), "=f"(t[j].w)
+                                             : "r"(or_map(at, base + j))
+                                             : "memory");
+                        float4 f = t[0];
+#pragma unroll
+                        for (int j = 1; j < ORTHO_TEAM_MAX; ++j)
+                            if (j < team) f.x += t[j].x, f.y += t[j].y, f.z += t[j].z, f.w += t[j].w;
+                        const __half2 h0 = __floats2half2_rn(f.x, f.y), h1 = __floats2half2_rn(f.z, f.w);
+                        const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
+                        const __half2 l0 = __floats2half2_rn(f.x - g0.x, f.y - g0.y), l1 = __floats2half2_rn(f.z - g1.x, f.w - g1.y);
+                        // eight bytes of a 16-byte chunk of tile chunk / 16
+                        const uint32_t to = as + (uint32_t)(chunk >> 4) * ORTHO_TILE + (uint32_t)r * 128u +
+                                            (uint32_t)((((chunk & 15) >> 1) ^ (r & 7)) << 4) + (uint32_t)(chunk & 1) * 8u;
+#pragma unroll
+                        for (int j = 0; j < ORTHO_TEAM_MAX; ++j) {
+                            if (j < team) {
+                                const uint32_t there = or_map(to, base + j);
+                                asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(there),
+                                             "r"(*reinterpret_cast<const uint32_t*>(&h0)), "r"(*reinterpret_cast<const uint32_t*>(&h1))
+                                             : "memory");
+                                asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(there + 16384u),
+                                             "r"(*reinterpret_cast<const uint32_t*>(&l0)), "r"(*reinterpret_cast<const uint32_t*>(&l1))
+                                             : "memory");
+                            }
+                        }
+                    }
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    __syncwarp();
+                }
+                or_cluster_sync();
+                asm volatile("fence.proxy.async;" ::: "memory");
+                or_fence_after();
+            } else {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                or_fence_before();
+                __syncthreads();
+                or_fence_after();
+            }
+        }
+    }
+    if (warp == 0) {
+        if (or_elect()) {
+            or_commit<false>(or_smem(&S.done));
+            for (uint32_t i = 0; i < ORTHO_WAIT_TRIES && !or_try_wait(or_smem(&S.done), 0u); ++i) {
+            }
+        }
+        __syncwarp();
+        or_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
 // ------------------------------------------------------------ host
 
 constexpr int64_t ORTHO_BUDGET = 1ll << 30;  // bytes of tiles that one launch works in, where a matrix alone does not need more
 constexpr int ORTHO_SINGLE = 512;
 
-static int64_t or_tiles_bytes(int m, int n) { return 2 * or_x_bytes(m, n) + 2 * or_a_bytes(m); }
+// blocks of a matrix's team, 0 where it takes the general path
+static int or_team(int m, int n) {
+    if (m > 128 || or_b64(n) > ORTHO_TEAM_MAX * ORTHO_TEAM_TILES) return 0;
+    int team = 1;
+    while (team * ORTHO_TEAM_TILES < or_b64(n)) team *= 2;
+    return team;
+}
+static int64_t or_tiles_bytes(int m, int n) { return or_team(m, n) ? 0 : 2 * or_x_bytes(m, n) + 2 * or_a_bytes(m); }
 static int64_t or_spans(int64_t total) { return (total + ORTHO_SPAN - 1) / ORTHO_SPAN; }
 static int64_t or_syms(int m, int bn, int pair) {
     int64_t n = 0;
@@ -1147,6 +1554,7 @@ static OrthoDesc or_make(int64_t rows, int64_t cols) {
     d.m = (int)(d.tall ? cols : rows);
     d.n = (int)(d.tall ? rows : cols);
     d.adjust = 1.0f;
+    d.team = or_team(d.m, d.n);
     return d;
 }
 
@@ -1188,6 +1596,34 @@ static int or_squares(const OrthoArgs& O, cudaStream_t s) {
     PBG_REQUIRE(O.spans < (1ll << 31), "orthogonalize: too many elements for one launch");
     orthogonalize_squares_kernel<<<(unsigned)O.spans, ORTHO_FLAT, 0, s>>>(O);
     return launch_status("orthogonalize: squares");
+}
+
+// the matrices with teams: O.list (largest teams first) or O.one, O.slots blocks
+static int or_teams(const OrthoArgs& O, int cluster, cudaStream_t s) {
+    static int configured[64] = {0};
+    int dev = 0, rc = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        rc = cuda_status(cudaFuncSetAttribute(orthogonalize_team_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_TEAM_SMEM),
+                         "orthogonalize: shared memory size");
+        if (rc) return rc;
+        if (dev >= 0 && dev < 64) configured[dev] = 1;
+    }
+    const int64_t grid = (O.slots + cluster - 1) / cluster * cluster;
+    PBG_REQUIRE(grid < (1ll << 31), "orthogonalize: too many matrices for one launch");
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)grid);
+    config.blockDim = dim3(ORTHO_THREADS);
+    config.dynamicSmemBytes = ORTHO_TEAM_SMEM;
+    config.stream = s;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = cluster;
+    attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = cluster > 1 ? 1 : 0;
+    void* args[] = {const_cast<OrthoArgs*>(&O), &cluster};
+    return cuda_status(cudaLaunchKernelExC(&config, (const void*)orthogonalize_team_kernel, args), "orthogonalize: team launch");
 }
 
 // conversion, then the products
@@ -1267,6 +1703,7 @@ static int or_check_polynomial(int steps, float a, float b, float c) {
 }
 
 static int64_t or_at_once(int64_t batch, int m, int n) {
+    if (or_team(m, n)) return batch;
     int64_t k = ORTHO_BUDGET / or_tiles_bytes(m, n);
     k = k < 1 ? 1 : k;
     return k < batch ? k : batch;
@@ -1281,6 +1718,7 @@ extern "C" {
 int64_t pbg_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols) {
     if (batch <= 0 || rows <= 0 || cols <= 0 || rows > 65536 || cols > 65536) return 0;
     const OrthoDesc d = or_make(rows, cols);
+    if (d.team) return 1024;
     const int64_t k = or_at_once(batch, d.m, d.n);
     return 1024 + or_up(k * or_spans(rows * cols) * 8) + k * or_tiles_bytes(d.m, d.n);
 }
@@ -1313,6 +1751,12 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.x_type = x_type, O.out_type = out_type, O.error = error;
     O.precise = !(out_type == 1 && m >= ORTHO_SINGLE);
+    if (O.one.team) {
+        O.count = batch, O.slots = batch * O.one.team;
+        O.x = x, O.out = out;
+        O.aligned = (uintptr_t)x % 16 == 0 && (uintptr_t)out % 16 == 0;
+        return or_teams(O, O.one.team, as_stream(stream));
+    }
     const int64_t xs = x_type == 0 ? 4 : 2, os = out_type == 0 ? 4 : 2;
     for (int64_t at = 0; at < batch; at += k) {
         O.count = batch - at < k ? batch - at : k;
@@ -1334,7 +1778,7 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
 
 int64_t pbg_muon_descriptor_bytes(void) { return (int64_t)sizeof(OrthoDesc); }
 
-int64_t pbg_muon_plan_words(int64_t count) { return count < 0 ? 0 : 8 + 5 * count; }
+int64_t pbg_muon_plan_words(int64_t count) { return count < 0 ? 0 : 9 + 5 * count; }
 
 int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, const int64_t* cols, const float* adjust,
                   void* descriptors, int64_t* plan) {
@@ -1347,18 +1791,27 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
         list[i].src = offset[i];
         list[i].adjust = adjust[i];
     }
-    // long products first: the blocks take tiles in turn
+    // long products first: the blocks take tiles in turn; then the matrices with teams, the largest teams first
     std::stable_sort(list, list + count, [](const OrthoDesc& p, const OrthoDesc& q) {
+        if (!p.team != !q.team) return !p.team;
+        if (p.team) return p.team > q.team;
         return p.m != q.m ? p.m > q.m : p.n > q.n;
     });
     OrthoWidths W = {};
-    for (int64_t i = 0; i < count; ++i) or_weigh(W, list[i].m, list[i].n, 1);
+    int64_t general = 0, spans = 0, slots = 0;
+    for (; general < count && !list[general].team; ++general) or_weigh(W, list[general].m, list[general].n, 1);
+    for (int64_t i = 0; i < count; ++i) {
+        list[i].span0 = spans;
+        spans += or_spans((int64_t)list[i].m * list[i].n);
+        list[i].slot0 = slots;
+        slots += list[i].team;
+    }
     int bn_sym, bn_upd, pair;
-    or_choose(W, bn_sym, bn_upd, pair);
-    int64_t spans = 0, waves = 0, most = 0;
+    or_choose(W, bn_sym, bn_upd, pair);  // of the others
+    int64_t waves = 0, most = 0;
     int64_t* wave = plan + 8;
     OrthoDesc at = {};
-    for (int64_t i = 0; i < count; ++i) {
+    for (int64_t i = 0; i < general; ++i) {
         const int m = list[i].m, n = list[i].n;
         const int64_t bytes = or_tiles_bytes(m, n);
         if (i == 0 || at.ws + bytes > ORTHO_BUDGET) {  // the next launch
@@ -1368,8 +1821,6 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
             ++waves;
         }
         list[i].ws = at.ws, list[i].conv0 = at.conv0, list[i].sym0 = at.sym0, list[i].upd0 = at.upd0;
-        list[i].span0 = spans;
-        spans += or_spans((int64_t)m * n);
         at.ws += bytes;
         at.conv0 += (int64_t)or_mb(m) * or_b64(n);
         at.sym0 += or_syms(m, bn_sym, pair);
@@ -1379,7 +1830,8 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
     }
     plan[0] = 1024 + or_up(spans * 8) + most;
     plan[1] = spans, plan[2] = waves, plan[3] = bn_sym, plan[4] = bn_upd;
-    plan[5] = pair, plan[6] = plan[7] = 0;
+    plan[5] = pair, plan[6] = general, plan[7] = slots;
+    plan[8 + 5 * waves] = slots ? list[general].team : 0;  // the clusters' size
     return 0;
 }
 
@@ -1417,6 +1869,11 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
         O.convs = wave[2], O.syms = wave[3], O.upds = wave[4];
         rc = or_products(O, s);
         if (rc) return rc;
+    }
+    if (plan[7]) {
+        const int64_t general = plan[6];
+        O.list = list + general, O.count = count - general, O.slots = plan[7];
+        return or_teams(O, (int)plan[8 + 5 * waves], s);
     }
     return 0;
 }
