@@ -53,6 +53,11 @@ constexpr int ORTHO_FLAT = 256;         // threads of the kernels around the pro
 constexpr int ORTHO_SPAN = ORTHO_FLAT * 16;  // elements whose squares one block sums
 constexpr int ORTHO_TILE = 32768;       // bytes of a 128 x 64 tile, hi and lo
 constexpr uint32_t ORTHO_WAIT_TRIES = 1u << 24;
+// What truncation takes from the sums on average, given back where they are scaled: from the update's
+// 2^-22 of the result; the polynomial's, where the positive square loses against the negative multiple of A,
+// come out 2^-22 too large.  Measured: 2.0e-6 of the result instead of 3.3e-6 at 256 x 1,024, 1.8e-6 instead
+// of 3.1e-6 at 384 x 128 (fp32 operands: 2.1e-6 and 1.6e-6).
+constexpr float ORTHO_UPDATE_BACK = 1.0f + 0x1p-22f, ORTHO_SQUARE_BACK = 1.0f - 0x1p-22f;
 constexpr float ORTHO_SX = 16384.0f, ORTHO_SA = 8192.0f, ORTHO_SB = 4096.0f;
 
 struct OrthoDesc {
@@ -570,122 +575,110 @@ __device__ __forceinline__ void or_store_rows(uint32_t blk, int blocks, unsigned
     }
 }
 
+// one finished value at element i of the output, or into the master
 struct OrthoOut {
     float lr, shrink;  // of the transition
 };
-
-// N finished values (4: aligned) at element i of the output, or one into the master
-template <int N>
-__device__ __forceinline__ void or_write_out(const OrthoArgs& O, const OrthoOut& k, int64_t i, float* v) {
-    if (!O.x) {
-        float* p = O.master + i;
-        *p = *p * k.shrink - k.lr * v[0];
-    } else if (O.out_type == 0) {
-        float* p = static_cast<float*>(O.out) + i;
-        if constexpr (N == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        else *p = v[0];
-    } else if (O.out_type == 1) {
-        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(O.out) + i;
-        if constexpr (N == 4) {
-            __nv_bfloat162 w[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
-        } else {
-            *p = __float2bfloat16_rn(v[0]);
-        }
-    } else {
-        __half* p = static_cast<__half*>(O.out) + i;
-        if constexpr (N == 4) {
-            __half2 w[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
-            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(w);
-        } else {
-            *p = __float2half_rn(v[0]);
-        }
-    }
+__device__ __forceinline__ void or_write_one(const OrthoArgs& O, const OrthoOut& k, int64_t i, float v) {
+    if (!O.x) O.master[i] = O.master[i] * k.shrink - k.lr * v;
+    else if (O.out_type == 0) static_cast<float*>(O.out)[i] = v;
+    else if (O.out_type == 1) static_cast<__nv_bfloat16*>(O.out)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(O.out)[i] = __float2half_rn(v);
 }
 
-// the last update: rows of the result to the output or the master
-__device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int row, int cb, uint32_t blk, int lane,
-                                              float* v) {
+// The last update: 64 columns of a warp's 32 rows to the output or the master, 32 columns at a time by way
+// of the warp's staging blocks (32 rows of 128 bytes, chunks swizzled by the row), so that lanes are
+// neighbours in memory whichever side is stored along.  Loops are kept rolled: each launch runs this once, and
+// unrolled its instructions took longer to fetch (12 us) than to run.  v is used up.
+__device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int row, int cb, uint32_t blk, int lane, float* v) {
     const OrthoDesc d = or_get(O, which);
     const int r0 = row - lane;
     OrthoOut k = {0.0f, 1.0f};
-    float scale = 1.0f / (ORTHO_SB * ORTHO_SX);
     if (!O.x) {
         k.lr = O.controls[0];
         k.shrink = 1.0f - k.lr * O.controls[2];
         k.lr *= d.adjust;
     }
-#pragma unroll
-    for (int j = 0; j < 64; ++j) v[j] *= scale;
-    if (d.tall) {  // lanes are neighbours in memory
-        const int64_t base = d.src + (int64_t)cb * 64 * d.m + row;
-        const int cols = min(64, d.n - cb * 64);
-        if (row < d.m) {
-            if (!O.x) {
-#pragma unroll
-                for (int j0 = 0; j0 < 64; j0 += 8) {
-                    float w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) w[j] = j0 + j < cols ? O.master[base + (int64_t)(j0 + j) * d.m] : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j0 + j < cols) O.master[base + (int64_t)(j0 + j) * d.m] = w[j] * k.shrink - k.lr * v[j0 + j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 64; ++j)
-                    if (j < cols) or_write_out<1>(O, k, base + (int64_t)j * d.m, v + j);
-            }
-        }
-        return;
-    }
-    // 32 rows x 16 columns at a time by way of the staging block, so that lanes write along rows
+    const float scale = ORTHO_UPDATE_BACK / (ORTHO_SB * ORTHO_SX);
+    const bool vector = d.n % 4 == 0 && d.src % 4 == 0 && O.aligned;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
-    const bool vector = d.n % 4 == 0 && d.src % 4 == 0 && O.aligned;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const uint32_t addr = blk + (uint32_t)lane * 64u + (uint32_t)((q ^ ((lane >> 1) & 3)) << 4);
-            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[16 * p + 4 * q]),
-                         "f"(v[16 * p + 4 * q + 1]), "f"(v[16 * p + 4 * q + 2]), "f"(v[16 * p + 4 * q + 3])
+        for (int q = 0; q < 8; ++q)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(blk + (uint32_t)lane * 128u + (uint32_t)((q ^ (lane & 7)) << 4)),
+                         "f"(v[4 * q] * scale), "f"(v[4 * q + 1] * scale), "f"(v[4 * q + 2] * scale), "f"(v[4 * q + 3] * scale)
                          : "memory");
-        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = v[j + 32];
         __syncwarp();
-        // four columns a lane, four lanes a row
-        const int col = cb * 64 + p * 16 + (lane & 3) * 4;
-        const int64_t base = d.src + (int64_t)(r0 + (lane >> 2)) * d.n + col;
-#pragma unroll
-        for (int pair = 0; pair < 2; ++pair) {
-            float x[2][4];
-            float4 w[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int it = pair * 2 + u, rr = it * 8 + (lane >> 2), q = lane & 3;
-                const uint32_t addr = blk + (uint32_t)rr * 64u + (uint32_t)((q ^ ((rr >> 1) & 3)) << 4);
-                asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(x[u][0]), "=f"(x[u][1]), "=f"(x[u][2]), "=f"(x[u][3])
-                             : "r"(addr)
-                             : "memory");
-                if (vector && !O.x && r0 + rr < d.m && col < d.n)
-                    w[u] = *reinterpret_cast<const float4*>(O.master + base + (int64_t)it * 8 * d.n);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int it = pair * 2 + u, rr = it * 8 + (lane >> 2);
-                const int64_t at = base + (int64_t)it * 8 * d.n;
-                if (r0 + rr >= d.m || col >= d.n) continue;
-                if (!vector) {
+        const int col0 = cb * 64 + half * 32;
+        if (d.tall) {  // a column of the tile is a run in memory: a lane per row
+            const int cols = min(32, d.n - col0);
+            if (row < d.m) {
+#pragma unroll 1
+                for (int j0 = 0; j0 < cols; j0 += 4) {
+                    const int64_t at = d.src + (int64_t)(col0 + j0) * d.m + row;
+                    float x[4], w[4];
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                                 : "r"(blk + (uint32_t)lane * 128u + (uint32_t)(((j0 >> 2) ^ (lane & 7)) << 4))
+                                 : "memory");
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (col + j < d.n) or_write_out<1>(O, k, at + j, x[u] + j);
-                } else if (O.x) {
-                    or_write_out<4>(O, k, at, x[u]);
-                } else {
-                    *reinterpret_cast<float4*>(O.master + at) =
-                        make_float4(w[u].x * k.shrink - k.lr * x[u][0], w[u].y * k.shrink - k.lr * x[u][1],
-                                    w[u].z * k.shrink - k.lr * x[u][2], w[u].w * k.shrink - k.lr * x[u][3]);
+                        if (!O.x && j0 + j < cols) w[j] = O.master[at + (int64_t)j * d.m];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j0 + j >= cols) continue;
+                        if (!O.x) O.master[at + (int64_t)j * d.m] = w[j] * k.shrink - k.lr * x[j];
+                        else or_write_one(O, k, at + (int64_t)j * d.m, x[j]);
+                    }
+                }
+            }
+        } else {  // eight lanes a row, four columns each
+            const int col = col0 + (lane & 7) * 4;
+            const int rows = min(32, d.m - r0);
+#pragma unroll 1
+            for (int r1 = lane >> 3; r1 < rows; r1 += 8) {
+                float x[2][4];
+                float4 w[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r = r1 + 4 * u;
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(x[u][0]), "=f"(x[u][1]), "=f"(x[u][2]), "=f"(x[u][3])
+                                 : "r"(blk + (uint32_t)r * 128u + (uint32_t)(((lane & 7) ^ (r & 7)) << 4))
+                                 : "memory");
+                    if (!O.x && vector && r < rows && col < d.n)
+                        w[u] = *reinterpret_cast<const float4*>(O.master + d.src + (int64_t)(r0 + r) * d.n + col);
+                }
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int r = r1 + 4 * u;
+                    const int64_t at = d.src + (int64_t)(r0 + r) * d.n + col;
+                    if (r >= rows || col >= d.n) continue;
+                    if (!vector) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (col + j < d.n) or_write_one(O, k, at + j, x[u][j]);
+                    } else if (!O.x) {
+                        *reinterpret_cast<float4*>(O.master + at) =
+                            make_float4(w[u].x * k.shrink - k.lr * x[u][0], w[u].y * k.shrink - k.lr * x[u][1],
+                                        w[u].z * k.shrink - k.lr * x[u][2], w[u].w * k.shrink - k.lr * x[u][3]);
+                    } else if (O.out_type == 0) {
+                        *reinterpret_cast<float4*>(static_cast<float*>(O.out) + at) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+                    } else {
+                        uint2 b;
+                        if (O.out_type == 1) {
+                            const __nv_bfloat162 p = __floats2bfloat162_rn(x[u][0], x[u][1]), q = __floats2bfloat162_rn(x[u][2], x[u][3]);
+                            b.x = *reinterpret_cast<const uint32_t*>(&p), b.y = *reinterpret_cast<const uint32_t*>(&q);
+                        } else {
+                            const __half2 p = __floats2half2_rn(x[u][0], x[u][1]), q = __floats2half2_rn(x[u][2], x[u][3]);
+                            b.x = *reinterpret_cast<const uint32_t*>(&p), b.y = *reinterpret_cast<const uint32_t*>(&q);
+                        }
+                        *reinterpret_cast<uint2*>(static_cast<unsigned short*>(O.out) + at) = b;
+                    }
                 }
             }
         }
@@ -701,7 +694,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
     const int r0 = row - lane;
     if (kind == OR_UPDATE) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] *= 1.0f / ORTHO_SB;
+        for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
         unsigned char* tile = L.x_next + i * L.x_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
         or_store_rows(blk, blocks, tile, lane, v, 2);
         return;
@@ -709,7 +702,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
     if ((cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
     unsigned char* dst = kind == OR_GRAM ? L.a : L.b;
     const float factor = kind == OR_GRAM ? ORTHO_SA / (ORTHO_SX * ORTHO_SX)
-                                         : (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA));
+                                         : (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA) * ORTHO_SQUARE_BACK);
     const float diagonal = kind == OR_GRAM ? 0.0f : O.a * ORTHO_SB;
 #pragma unroll
     for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == cb * 64 + j ? diagonal : 0.0f);
@@ -1139,6 +1132,7 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
 // part in all of the cluster's barriers.
 constexpr int ORTHO_TEAM_TILES = 3;
 constexpr int ORTHO_TEAM_MAX = 8;
+constexpr int ORTHO_TEAM_THREADS = 512;                // warp 0 issues, warps 4 .. 15 take a row quarter of one column group each
 constexpr int ORTHO_TEAM_A = 2 * ORTHO_TILE;           // A, then B: 128 x 128
 constexpr int ORTHO_TEAM_SUM = 128 * 128 * 4;          // a block's own Gram matrix, fp32; then staging
 constexpr int ORTHO_TEAM_SMEM = 1024 + ORTHO_TEAM_TILES * ORTHO_TILE + ORTHO_TEAM_A + ORTHO_TEAM_SUM + ORTHO_EYE;
@@ -1146,7 +1140,7 @@ constexpr int ORTHO_TEAM_SMEM = 1024 + ORTHO_TEAM_TILES * ORTHO_TILE + ORTHO_TEA
 struct OrthoTeam {
     uint64_t acc_full[2], acc_empty[2], done;
     double squares[ORTHO_TEAM_MAX];
-    double part[ORTHO_THREADS / 32];
+    double part[ORTHO_TEAM_THREADS / 32];
     uint32_t tmem;
     volatile int abort_flag;
 };
@@ -1177,7 +1171,22 @@ __device__ __forceinline__ void or_keep_rows(uint32_t tile, int row, const float
     }
 }
 
-__global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(const __grid_constant__ OrthoArgs O, int cluster) {
+// chunk q of a block's columns from a matrix's elements: lanes run along the stored rows
+__device__ __forceinline__ void or_team_chunk(const OrthoArgs& O, const OrthoDesc& d, bool vector, int first, int q, const void* src,
+                                              int type, float* u) {
+    const int t = q >> 10, c = q & 1023;
+    const int row = d.tall ? c & 127 : c >> 3, col = (first + t) * 64 + (d.tall ? c >> 7 : c & 7) * 8;
+    const int live = row < d.m ? max(0, min(8, d.n - col)) : 0;
+    if (d.tall) {
+        const int64_t i = d.src + (int64_t)col * d.m + row;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[e] = e < live ? or_load(src, type, i + (int64_t)e * d.m) : 0.0f;
+    } else {
+        or_load8(src, type, d.src + (int64_t)row * d.n + col, vector, live, u);
+    }
+}
+
+__global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kernel(const __grid_constant__ OrthoArgs O, int cluster) {
     extern __shared__ __align__(1024) unsigned char or_raw[];
     OrthoTeam& S = *reinterpret_cast<OrthoTeam*>(or_raw);
     static_assert(sizeof(OrthoTeam) <= 1024, "shared state fits its kilobyte");
@@ -1192,7 +1201,7 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
         if (blockIdx.x < O.slots) {
             const OrthoDesc d = or_get(O, or_find(O, blockIdx.x, &OrthoDesc::slot0, O.one.team));
             const int64_t total = (int64_t)d.m * d.n;
-            for (int64_t i = (int64_t)(blockIdx.x - d.slot0) * ORTHO_THREADS + threadIdx.x; i < total; i += (int64_t)d.team * ORTHO_THREADS)
+            for (int64_t i = (int64_t)(blockIdx.x - d.slot0) * ORTHO_TEAM_THREADS + threadIdx.x; i < total; i += (int64_t)d.team * ORTHO_TEAM_THREADS)
                 O.grad[d.src + i] = 0.0f;
         }
         return;
@@ -1217,7 +1226,7 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
         S.abort_flag = 0;
         for (int b = 0; b < 2; ++b) {
             or_mbar_init(or_smem(&S.acc_full[b]), 1);
-            or_mbar_init(or_smem(&S.acc_empty[b]), ORTHO_EPI_WARPS);
+            or_mbar_init(or_smem(&S.acc_empty[b]), ORTHO_TEAM_THREADS / 32 - 4);
         }
         or_mbar_init(or_smem(&S.done), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1243,94 +1252,66 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
     // ---------------------------------------------------- the direction, its norm, and X
     const OrthoDirection k = or_controls(O);
     const bool vector = O.aligned && d.src % 4 == 0 && d.n % 4 == 0;
-    constexpr int ROUNDS = ORTHO_TEAM_TILES * 1024 / ORTHO_THREADS;  // chunks of 8 columns a thread
-    static_assert(ROUNDS * ORTHO_THREADS == ORTHO_TEAM_TILES * 1024, "the chunks divide evenly");
-    {
+    // Chunks of 8 columns, rolled loops; the squares' pass leaves the values in L1 and L2 for the second.
+    const int chunks_all = tiles * 1024;
+    double total = 0.0;
+    if (O.x) {
         double square = 0.0;
-        float u[ROUNDS][8];
+#pragma unroll 2
+        for (int q = threadIdx.x; q < chunks_all; q += ORTHO_TEAM_THREADS) {
+            float u[8];
+            or_team_chunk(O, d, vector, first, q, O.x, O.x_type, u);
 #pragma unroll
-        for (int h = 0; h < ROUNDS; ++h) {
-            const int q = h * ORTHO_THREADS + threadIdx.x, t = q >> 10, c = q & 1023;
-            const int row = d.tall ? c & 127 : c >> 3, chunk = d.tall ? c >> 7 : c & 7;
-            const int col = (first + t) * 64 + chunk * 8;
-            const int live = t < tiles && row < d.m ? max(0, min(8, d.n - col)) : 0;
+            for (int e = 0; e < 8; ++e) square += (double)u[e] * (double)u[e];
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
+        if (lane == 0) S.part[warp] = square;
+        if (cluster > 1) or_cluster_sync();  // the others run: their shared memory may be written
+        else __syncthreads();
+        if (threadIdx.x < team) {
+            double own = 0.0;
+            for (int w = 0; w < ORTHO_TEAM_THREADS / 32; ++w) own += S.part[w];
+            const uint32_t at = or_smem(&S.squares[rank]);
+            if (team == 1) S.squares[0] = own;
+            else asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(or_map(at, base + (int)threadIdx.x)), "d"(own) : "memory");
+        }
+        if (cluster > 1) or_cluster_sync();
+        else __syncthreads();
+        for (int r = 0; r < team; ++r) total += S.squares[r];
+    } else {
+        if (cluster > 1) or_cluster_sync();
+        const int64_t spans = ((int64_t)d.m * d.n + ORTHO_SPAN - 1) / ORTHO_SPAN;
+        for (int64_t r = 0; r < spans; ++r) total += __ldg(O.sums + d.span0 + r);
+    }
+    const double wide = (double)ORTHO_SX / (sqrt(total) + O.eps);
+    const float scale = (float)wide;
+    const bool plain = scale < 1.0e30f;
+#pragma unroll 2
+    for (int q = threadIdx.x; q < chunks_all; q += ORTHO_TEAM_THREADS) {
+        float u[8], m[8];
+        or_team_chunk(O, d, vector, first, q, O.x ? O.x : O.grad, O.x ? O.x_type : 0, u);
+        const int t = q >> 10, c = q & 1023;
+        const int row = d.tall ? c & 127 : c >> 3, chunk = d.tall ? c >> 7 : c & 7, col = (first + t) * 64 + chunk * 8;
+        const int live = row < d.m ? max(0, min(8, d.n - col)) : 0;
+        if (!O.x) {
+            or_team_chunk(O, d, vector, first, q, O.momentum, 0, m);
             const int64_t i = d.src + (d.tall ? (int64_t)col * d.m + row : (int64_t)row * d.n + col);
             const int64_t next = d.tall ? d.m : 1;
-            const void* src = O.x ? O.x : O.grad;
-            const int type = O.x ? O.x_type : 0;
-            float m[8];
-            if (d.tall) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    u[h][e] = e < live ? or_load(src, type, i + e * next) : 0.0f;
-                    if (!O.x) m[e] = e < live ? O.momentum[i + e * next] : 0.0f;
-                }
-            } else {
-                or_load8(src, type, i, vector, live, u[h]);
-                if (!O.x) or_load8(O.momentum, 0, i, vector, live, m);
-            }
-            if (!O.x) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    m[e] = or_momentum(k, u[h][e], m[e]);
-                    u[h][e] = or_direction(k, u[h][e], m[e]);
-                }
-                if (!d.tall && vector && live >= 8) {
-                    float4* p = reinterpret_cast<float4*>(O.momentum + i);
-                    p[0] = make_float4(m[0], m[1], m[2], m[3]);
-                    p[1] = make_float4(m[4], m[5], m[6], m[7]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e < live) O.momentum[i + e * next] = m[e];
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) square += (double)u[h][e] * (double)u[h][e];
+            for (int e = 0; e < 8; ++e) {
+                m[e] = or_momentum(k, u[e], m[e]);
+                u[e] = or_direction(k, u[e], m[e]);
+                if (e < live) O.momentum[i + e * next] = m[e];
             }
         }
-        double total = 0.0;
-        if (O.x) {
+        __align__(16) __half hi[8];
+        __align__(16) __half lo[8];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) square += __shfl_xor_sync(0xffffffffu, square, o);
-            if (lane == 0) S.part[warp] = square;
-            if (cluster > 1) or_cluster_sync();  // the others run: their shared memory may be written
-            else __syncthreads();
-            if (threadIdx.x < team) {
-                double own = 0.0;
-                for (int w = 0; w < ORTHO_THREADS / 32; ++w) own += S.part[w];
-                const uint32_t at = or_smem(&S.squares[rank]);
-                if (team == 1) S.squares[0] = own;
-                else asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(or_map(at, base + (int)threadIdx.x)), "d"(own) : "memory");
-            }
-            if (cluster > 1) or_cluster_sync();
-            else __syncthreads();
-            for (int r = 0; r < team; ++r) total += S.squares[r];
-        } else {
-            const int64_t spans = ((int64_t)d.m * d.n + ORTHO_SPAN - 1) / ORTHO_SPAN;
-            for (int64_t r = 0; r < spans; ++r) total += __ldg(O.sums + d.span0 + r);
-        }
-        const double wide = (double)ORTHO_SX / (sqrt(total) + O.eps);
-        const float scale = (float)wide;
-        const bool plain = scale < 1.0e30f;
-#pragma unroll
-        for (int h = 0; h < ROUNDS; ++h) {
-            const int q = h * ORTHO_THREADS + threadIdx.x, t = q >> 10, c = q & 1023;
-            const int row = d.tall ? c & 127 : c >> 3, chunk = d.tall ? c >> 7 : c & 7;
-            const int col = (first + t) * 64 + chunk * 8;
-            if (t < tiles) {
-                __align__(16) __half hi[8];
-                __align__(16) __half lo[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool in = row < d.m && col + e < d.n;
-                    or_split(in ? (plain ? u[h][e] * scale : (float)((double)u[h][e] * wide)) : 0.0f, hi[e], lo[e]);
-                }
-                unsigned char* at = or_raw + 1024 + t * ORTHO_TILE + row * 128 + ((chunk ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(hi);
-                *reinterpret_cast<uint4*>(at + 16384) = *reinterpret_cast<uint4*>(lo);
-            }
-        }
+        for (int e = 0; e < 8; ++e) or_split(e < live ? (plain ? u[e] * scale : (float)((double)u[e] * wide)) : 0.0f, hi[e], lo[e]);
+        unsigned char* at = or_raw + 1024 + t * ORTHO_TILE + row * 128 + ((chunk ^ (row & 7)) << 4);
+        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(hi);
+        *reinterpret_cast<uint4*>(at + 16384) = *reinterpret_cast<uint4*>(lo);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     or_fence_before();
@@ -1340,7 +1321,7 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
     // ---------------------------------------------------- the steps
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
     const uint32_t tmem = S.tmem;
-    const int e = warp - 1 - ORTHO_PRODUCERS, quad = warp & 3, part = e >> 2;  // epilogue warps
+    const int e = warp - 4, quad = warp & 3, part = e >> 2;  // epilogue warps: column group `part`
     const int row = quad * 32 + lane;
     uint32_t acc = 0;
     for (int step = 0; step < O.steps; ++step) {
@@ -1348,11 +1329,10 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
             const bool linear = kind == OR_SQUARE && O.c == 0.0f;
             const int kblocks = tiles == 0 && kind != OR_SQUARE ? 0 : kind == OR_GRAM ? tiles : m64;
             const int groups_all = kind == OR_UPDATE ? tiles : m64;  // 64-column groups of the product
-            float v[128];
+            float v[64];
 #pragma unroll
-            for (int j = 0; j < 128; ++j) v[j] = 0.0f;
-            const int per = kind == OR_UPDATE ? 2 : 1;  // groups an epilogue warp takes
-            const int group0 = part * per, groups = min(per, groups_all - group0);
+            for (int j = 0; j < 64; ++j) v[j] = 0.0f;
+            const bool mine = part < groups_all;
             bool ok = true;
             if (warp == 0) {
                 if (or_elect()) {
@@ -1404,19 +1384,15 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
                 __syncwarp();
             } else if (e >= 0) {
                 const int chunks = linear ? (kblocks > 0) : kblocks;
-                const uint32_t taddr0 = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(group0 * 64);
+                const uint32_t taddr0 = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(part * 64);
                 for (int c = 0; c < chunks; ++c, ++acc) {
                     const uint32_t b = acc & 1u;
                     ok = __all_sync(0xffffffffu, or_wait(acc_full0 + 8 * b, (acc >> 1) & 1u, &S.abort_flag));
                     if (!ok) break;
                     or_fence_after();
-                    if (groups > 0) {
+                    if (mine) {
 #pragma unroll
                         for (int j = 0; j < 64; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
-                    }
-                    if (groups > 1) {
-#pragma unroll
-                        for (int j = 64; j < 128; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
                     }
                     or_fence_before();
                     __syncwarp();
@@ -1430,32 +1406,33 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
 #pragma unroll
                     for (int j = 0; j < 64; ++j) v[j] *= ORTHO_SA / (ORTHO_SX * ORTHO_SX);
                     if (team == 1) {
-                        if (groups > 0) or_keep_rows(as + part * ORTHO_TILE, row, v);
+                        if (mine) or_keep_rows(as + part * ORTHO_TILE, row, v);
                     } else if (part < m64) {
-                        // 32 chunks of four columns a row, swizzled by the row
+                        // to the block whose share this row is: [rank][its rows][32 chunks of four columns],
+                        // chunks swizzled by the row
+                        const int rows = 128 / team;
+                        const uint32_t there = or_map(sums, base + row / rows) + (uint32_t)(rank * rows + row % rows) * 512u;
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) {
-                            const uint32_t at = sums + (uint32_t)row * 512u + (uint32_t)(((part * 16 + q) ^ lane) << 4);
-                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v[4 * q]), "f"(v[4 * q + 1]),
-                                         "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
+                        for (int q = 0; q < 16; ++q)
+                            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(there + (uint32_t)(((part * 16 + q) ^ lane) << 4)),
+                                         "f"(v[4 * q]), "f"(v[4 * q + 1]), "f"(v[4 * q + 2]), "f"(v[4 * q + 3])
                                          : "memory");
-                        }
                     }
                 } else if (kind == OR_SQUARE) {
-                    const float factor = (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA)), diagonal = O.a * ORTHO_SB;
-                    if (groups > 0) {
+                    const float factor = (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA) * ORTHO_SQUARE_BACK), diagonal = O.a * ORTHO_SB;
+                    if (mine) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == part * 64 + j ? diagonal : 0.0f);
                         or_keep_rows(as + part * ORTHO_TILE, row, v);
                     }
-                } else if (step + 1 < O.steps) {
+                } else if (mine && ok) {
+                    if (step + 1 < O.steps) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j) v[j] *= 1.0f / ORTHO_SB;
-                    if (groups > 0) or_keep_rows(xs + group0 * ORTHO_TILE, row, v);
-                    if (groups > 1) or_keep_rows(xs + (group0 + 1) * ORTHO_TILE, row, v + 64);
-                } else if (ok) {
-                    if (groups > 0) or_finish_out(O, which, row, first + group0, sums + (uint32_t)e * ORTHO_BLOCK, lane, v);
-                    if (groups > 1) or_finish_out(O, which, row, first + group0 + 1, sums + (uint32_t)e * ORTHO_BLOCK, lane, v + 64);
+                        for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
+                        or_keep_rows(xs + part * ORTHO_TILE, row, v);
+                    } else {
+                        or_finish_out(O, which, row, first + part, sums + (uint32_t)e * (2u * ORTHO_BLOCK), lane, v);
+                    }
                 }
             }
             __syncwarp();
@@ -1464,39 +1441,32 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_team_kernel(co
                 if (team > 1) {
                     // this block's rows, summed over the team in rank order, as pairs to every block of the team
                     const int rows = 128 / team;
-                    for (int q = threadIdx.x; q < rows * 32; q += ORTHO_THREADS) {
+                    for (int q = threadIdx.x; q < rows * 32; q += ORTHO_TEAM_THREADS) {
                         const int r = rank * rows + (q >> 5), chunk = q & 31;  // four columns
                         if (chunk >= m64 * 16) continue;
-                        const uint32_t at = sums + (uint32_t)r * 512u + (uint32_t)((chunk ^ (r & 31)) << 4);
-                        float4 t[ORTHO_TEAM_MAX];
-#pragma unroll
-                        for (int j = 0; j < ORTHO_TEAM_MAX; ++j)
-                            if (j < team)
-                                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                             : "=f"(t[j].x), "=f"(t[j].y), "=f"(t[j].z), "=f"(t[j].w)
-                                             : "r"(or_map(at, base + j))
-                                             : "memory");
-                        float4 f = t[0];
-#pragma unroll
-                        for (int j = 1; j < ORTHO_TEAM_MAX; ++j)
-                            if (j < team) f.x += t[j].x, f.y += t[j].y, f.z += t[j].z, f.w += t[j].w;
+                        float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int j = 0; j < team; ++j) {
+                            float4 t;
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                         : "=f"(t.x), "=f"(t.y), "=f"(t.z), "=f"(t.w)
+                                         : "r"(sums + (uint32_t)(j * rows + (q >> 5)) * 512u + (uint32_t)((chunk ^ (r & 31)) << 4))
+                                         : "memory");
+                            f.x += t.x, f.y += t.y, f.z += t.z, f.w += t.w;
+                        }
                         const __half2 h0 = __floats2half2_rn(f.x, f.y), h1 = __floats2half2_rn(f.z, f.w);
                         const float2 g0 = __half22float2(h0), g1 = __half22float2(h1);
                         const __half2 l0 = __floats2half2_rn(f.x - g0.x, f.y - g0.y), l1 = __floats2half2_rn(f.z - g1.x, f.w - g1.y);
                         // eight bytes of a 16-byte chunk of tile chunk / 16
                         const uint32_t to = as + (uint32_t)(chunk >> 4) * ORTHO_TILE + (uint32_t)r * 128u +
                                             (uint32_t)((((chunk & 15) >> 1) ^ (r & 7)) << 4) + (uint32_t)(chunk & 1) * 8u;
-#pragma unroll
-                        for (int j = 0; j < ORTHO_TEAM_MAX; ++j) {
-                            if (j < team) {
-                                const uint32_t there = or_map(to, base + j);
-                                asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(there),
-                                             "r"(*reinterpret_cast<const uint32_t*>(&h0)), "r"(*reinterpret_cast<const uint32_t*>(&h1))
-                                             : "memory");
-                                asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(there + 16384u),
-                                             "r"(*reinterpret_cast<const uint32_t*>(&l0)), "r"(*reinterpret_cast<const uint32_t*>(&l1))
-                                             : "memory");
-                            }
+                        for (int j = 0; j < team; ++j) {
+                            const uint32_t there = or_map(to, base + j);
+                            asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(there),
+                                         "r"(*reinterpret_cast<const uint32_t*>(&h0)), "r"(*reinterpret_cast<const uint32_t*>(&h1))
+                                         : "memory");
+                            asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(there + 16384u),
+                                         "r"(*reinterpret_cast<const uint32_t*>(&l0)), "r"(*reinterpret_cast<const uint32_t*>(&l1))
+                                         : "memory");
                         }
                     }
                     asm volatile("fence.proxy.async;" ::: "memory");
@@ -1613,7 +1583,7 @@ static int or_teams(const OrthoArgs& O, int cluster, cudaStream_t s) {
     PBG_REQUIRE(grid < (1ll << 31), "orthogonalize: too many matrices for one launch");
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)grid);
-    config.blockDim = dim3(ORTHO_THREADS);
+    config.blockDim = dim3(ORTHO_TEAM_THREADS);
     config.dynamicSmemBytes = ORTHO_TEAM_SMEM;
     config.stream = s;
     cudaLaunchAttribute attribute[1];
