@@ -33,6 +33,7 @@
 #include <cuda_fp16.h>
 
 #include <math.h>
+#include <string.h>
 
 #include <algorithm>
 
@@ -79,6 +80,7 @@ struct OrthoArgs {
     int64_t count, spans, convs, syms, upds, slots;  // totals
     int bn_sym, bn_upd;  // output tile widths
     int pair;            // output tiles of 256 rows, by two blocks each
+    int mirror;          // of A and B only what is on and above the diagonal is computed
     int steps, precise;  // precise: A and B as pairs
     float a, b, c;
     double eps;
@@ -278,9 +280,11 @@ __host__ __device__ __forceinline__ int or_pitch_x(int n) { return (or_b64(n) + 
 __host__ __device__ __forceinline__ int or_pitch_a(int m) { return 2 * or_mb(m) | 1; }
 __host__ __device__ __forceinline__ int64_t or_x_bytes(int m, int n) { return (int64_t)or_mb(m) * or_pitch_x(n) * ORTHO_TILE; }
 __host__ __device__ __forceinline__ int64_t or_a_bytes(int m) { return (int64_t)or_mb(m) * or_pitch_a(m) * ORTHO_TILE; }
-// symmetric tiles of row block (pair of row blocks) i: from its first row's column on
-__host__ __device__ __forceinline__ int or_sym_row(int m, int i, int bn, int pair) {
-    return pair ? (or_mb(m) + 1) / 2 - i : (or_b64(m) * 64 - i * 128 + bn - 1) / bn;
+// first column of the symmetric products' row block (pair of row blocks) i, and its tiles: from the diagonal on
+// where the rest is mirrored
+__host__ __device__ __forceinline__ int or_sym_first(int i, int pair, int mirror) { return mirror ? i * (pair ? 256 : 128) : 0; }
+__host__ __device__ __forceinline__ int or_sym_row(int m, int i, int bn, int pair, int mirror) {
+    return (or_b64(m) * 64 - or_sym_first(i, pair, mirror) + bn - 1) / bn;
 }
 __host__ __device__ __forceinline__ int or_row_blocks(int m, int pair) { return pair ? (or_mb(m) + 1) / 2 : or_mb(m); }
 
@@ -484,8 +488,8 @@ __device__ __forceinline__ OrthoTile or_tile(const OrthoArgs& O, int kind, int64
     int local = (int)(t - first), columns;
     if (sym) {
         T.i = 0;
-        for (int r; local >= (r = or_sym_row(m, T.i, O.bn_sym, PAIR)); ++T.i) local -= r;
-        T.c0 = T.i * (PAIR ? 256 : 128) + local * O.bn_sym;
+        for (int r; local >= (r = or_sym_row(m, T.i, O.bn_sym, PAIR, O.mirror)); ++T.i) local -= r;
+        T.c0 = or_sym_first(T.i, PAIR, O.mirror) + local * O.bn_sym;
         columns = or_b64(m) * 64 - T.c0;
         T.width = min(O.bn_sym, columns);
     } else {
@@ -699,7 +703,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
         or_store_rows(blk, blocks, tile, lane, v, 2);
         return;
     }
-    if ((cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
+    if (O.mirror && (cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
     unsigned char* dst = kind == OR_GRAM ? L.a : L.b;
     const float factor = kind == OR_GRAM ? ORTHO_SA / (ORTHO_SX * ORTHO_SX)
                                          : (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA) * ORTHO_SQUARE_BACK);
@@ -708,7 +712,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
     for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == cb * 64 + j ? diagonal : 0.0f);
     unsigned char* tile = dst + i * L.a_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
     or_store_rows(blk, blocks, tile, lane, v, PRECISE ? 2 : 1);
-    if (cb * 64 >= (i + 1) * 128) {
+    if (O.mirror && cb * 64 >= (i + 1) * 128) {
         // the mirrored place of (row, cb * 64 + j): row block cb / 2, column block row / 64, row (cb & 1) * 64 + j
         // of that tile; lanes are neighbours
         const int mc = row & 63;
@@ -728,7 +732,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
 }
 
 struct OrthoShared {
-    uint64_t full[ORTHO_STAGES], empty[ORTHO_STAGES], peer[ORTHO_STAGES], acc_full[2], acc_empty[2], done;
+    uint64_t full[ORTHO_STAGES], empty[ORTHO_STAGES], peer[ORTHO_STAGES], acc_full[4], acc_empty[4], done;
     uint32_t tmem;
     int ok;
     volatile int abort_flag;
@@ -771,6 +775,10 @@ __device__ __forceinline__ OrthoStage or_stage(int kind, int bn) {
     G.stages = min(ORTHO_STAGES, (int)(ORTHO_RING / G.bytes));
     return G;
 }
+
+// Accumulators in tensor memory, as a power of two: four where no tile is wider than 128 (a short k-block's
+// products take less time than an accumulator's way to the registers), else two.
+__device__ __forceinline__ uint32_t or_buffers(const OrthoArgs& O) { return max(O.bn_sym, O.bn_upd) <= 128 ? 2u : 1u; }
 
 // A producer warp's elected lane, one phase.  A stage is copy 0, the row operand, and copies 1 .. 6, a 64-row
 // or 64-column piece of the other operand each, hi and lo; the producer warps take them in turn.  `pipe`:
@@ -855,7 +863,7 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
     const int mn = kind == OR_UPDATE;
     const uint32_t b_step = mn ? 2048u >> 4 : 32u >> 4, lbo = mn ? 8192u : 16u;
     const uint32_t eye = or_desc(ring + ORTHO_RING + ORTHO_STAGING, 16), eye_idesc = or_idesc<PAIR>(16, 0);
-    const uint32_t tmem = S.tmem;
+    const uint32_t tmem = S.tmem, shift = or_buffers(O), buffers = 1u << shift;
     bool ok = true;
     int s = 0;
     for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
@@ -864,13 +872,13 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
         const uint32_t idesc = or_idesc<PAIR>(T.width, mn);
         const int eye0 = kind == OR_SQUARE ? T.c0 >> 6 : 1 << 30, eye1 = eye0 + (T.width >> 6);
         for (int k0 = 0; ok && k0 < kblocks; k0 += chunk, ++acc) {
-            const uint32_t b = acc & 1u;
-            if (!or_wait_pair<PAIR>(acc_empty0 + 8 * b, ((acc >> 1) & 1u) ^ 1u, &S.abort_flag)) {
+            const uint32_t b = acc & (buffers - 1u);
+            if (!or_wait_pair<PAIR>(acc_empty0 + 8 * b, ((acc >> shift) & 1u) ^ 1u, &S.abort_flag)) {
                 ok = false;
                 break;
             }
             or_fence_after();
-            const uint32_t d = tmem + b * 256u;
+            const uint32_t d = tmem + b * (512u >> shift);
             const int k1 = min(k0 + chunk, kblocks);
             for (int kb = k0; kb < k1; ++kb) {
                 if (!or_wait(full0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag) ||
@@ -963,6 +971,7 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
     const int bn = kind == OR_UPDATE ? O.bn_upd : O.bn_sym;
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
     const int chunk = PRECISE && !(kind == OR_SQUARE && O.c == 0.0f) ? 1 : 1 << 20;
+    const uint32_t shift = or_buffers(O), buffers = 1u << shift;
     const int group0 = bn > 128 ? 2 * part : part;
     const int blocks = bn == 64 ? 4 : 2;
     const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * (2u * ORTHO_BLOCK);
@@ -976,17 +985,17 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
 #pragma unroll
         for (int j = 0; j < 128; ++j) v[j] = 0.0f;
         for (int k = 0; k < chunks; ++k, ++acc) {
-            const uint32_t b = acc & 1u;
-            ok = __all_sync(0xffffffffu, or_wait(acc_full0 + 8 * b, (acc >> 1) & 1u, &S.abort_flag));
+            const uint32_t b = acc & (buffers - 1u);
+            ok = __all_sync(0xffffffffu, or_wait(acc_full0 + 8 * b, (acc >> shift) & 1u, &S.abort_flag));
             if (!ok) break;
             or_fence_after();
             if (groups > 0) {
 #pragma unroll
-                for (int j = 0; j < 64; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
+                for (int j = 0; j < 64; j += 16) or_tmem_add16(taddr0 + b * (512u >> shift) + j, v + j);
             }
             if (groups > 1) {
 #pragma unroll
-                for (int j = 64; j < 128; j += 16) or_tmem_add16(taddr0 + b * 256u + j, v + j);
+                for (int j = 64; j < 128; j += 16) or_tmem_add16(taddr0 + b * (512u >> shift) + j, v + j);
             }
             or_fence_before();
             __syncwarp();
@@ -1042,7 +1051,7 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
             or_mbar_init(or_smem(&S.empty[s]), 1);
             or_mbar_init(or_smem(&S.peer[s]), 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < 4; ++b) {
             or_mbar_init(or_smem(&S.acc_full[b]), 1);
             or_mbar_init(or_smem(&S.acc_empty[b]), PAIR ? 2 * ORTHO_EPI_WARPS : ORTHO_EPI_WARPS);
         }
@@ -1509,9 +1518,9 @@ static int or_team(int m, int n) {
 }
 static int64_t or_tiles_bytes(int m, int n) { return or_team(m, n) ? 0 : 2 * or_x_bytes(m, n) + 2 * or_a_bytes(m); }
 static int64_t or_spans(int64_t total) { return (total + ORTHO_SPAN - 1) / ORTHO_SPAN; }
-static int64_t or_syms(int m, int bn, int pair) {
+static int64_t or_syms(int m, int bn, int pair, int mirror) {
     int64_t n = 0;
-    for (int i = 0; i < or_row_blocks(m, pair); ++i) n += or_sym_row(m, i, bn, pair);
+    for (int i = 0; i < or_row_blocks(m, pair); ++i) n += or_sym_row(m, i, bn, pair, mirror);
     return n;
 }
 static int64_t or_upds(int m, int n, int bn, int pair) {
@@ -1528,36 +1537,60 @@ static OrthoDesc or_make(int64_t rows, int64_t cols) {
     return d;
 }
 
-// Output tile shapes, by an estimate of the busiest block's cycles: a k-block of 64 and an output tile's end
-// cost what they were measured to on matrices of 4,096 (k-blocks) and of 256 x 1,024 (ends): 128 x 64, x 128
-// and x 192 by one block, 256 x 256 by a pair.  Wide tiles fetch less per multiply-add, narrow ones spread a
-// few small matrices over more SMs.
-struct OrthoWidths {
-    double sum[2][4], top[2][4];
+// Output tile shapes: those whose busiest block has least to do, the tiles being dealt out in turn.  A k-block
+// of 64 and an output tile's end cost (microseconds) what they were measured to on matrices of 4,096 and of
+// 256 x 16,384, for tiles of 128 x 64, x 128, x 192 and x 256 by one block and of 256 x 256 by a pair, and
+// OR_MIRROR more where a tile's mirror image is written too.  Wide tiles fetch less per multiply-add, narrow
+// ones spread a few small matrices over more SMs; small matrices have SMs to spare for both triangles.
+static const int OR_SHAPES = 5;
+static const int OR_WIDTHS[OR_SHAPES] = {64, 128, 192, 256, 256};
+static const double OR_BLOCK[OR_SHAPES] = {0.64, 0.88, 1.1, 1.27, 1.18}, OR_END[OR_SHAPES] = {2.6, 3.2, 4.2, 4.5, 4.5};
+static const double OR_MIRROR = 2.5;
+
+struct OrthoShape {
+    int bn_sym, bn_upd, pair, mirror;
 };
-static const int OR_WIDTHS[4] = {64, 128, 192, 256};
-static void or_weigh(OrthoWidths& W, int m, int n, int64_t count) {
-    static const double block[4] = {850.0, 1400.0, 2200.0, 1900.0}, end[4] = {3500.0, 4000.0, 5500.0, 6500.0};
-    for (int w = 0; w < 4; ++w)
-        for (int kind = 0; kind < 2; ++kind) {
-            const int bn = OR_WIDTHS[w], pair = w == 3;
-            // kind 0: the Gram matrix and its square together
-            const double cost = kind == 0 ? (or_b64(n) + or_b64(m)) * block[w] + 2 * end[w] : or_b64(m) * block[w] + end[w];
-            W.sum[kind][w] += cost * (double)count * (double)(kind == 0 ? or_syms(m, bn, pair) : or_upds(m, n, bn, pair)) * (pair ? 2 : 1);
-            if (cost > W.top[kind][w]) W.top[kind][w] = cost;
+// `count` matrices of list, or of one size
+static OrthoShape or_choose(const OrthoDesc* list, int64_t count, bool same) {
+    const int sms = sm_count() < 1024 ? sm_count() : 1024;
+    OrthoShape best = {64, 64, 0, 1};
+    double least = -1.0, load[1024];
+    for (int pair = 0; pair < 2; ++pair) {
+        const int blocks = pair ? sms / 2 : sms, w0 = pair ? 4 : 0, w1 = pair ? 5 : 4;
+        // the busiest block's time of a kind of product: 0 the Gram matrix and its polynomial, 1 the update
+        auto busiest = [&](int kind, int w, int mirror) {
+            auto cost = [&](int m, int n) {
+                return kind ? or_b64(m) * OR_BLOCK[w] + OR_END[w]
+                            : (or_b64(n) + or_b64(m)) * OR_BLOCK[w] + 2 * (OR_END[w] + (mirror && m > (pair ? 256 : 128) ? OR_MIRROR : 0.0));
+            };
+            auto tiles = [&](int m, int n) { return kind ? or_upds(m, n, OR_WIDTHS[w], pair) : or_syms(m, OR_WIDTHS[w], pair, mirror); };
+            if (same) return (double)((count * tiles(list[0].m, list[0].n) + blocks - 1) / blocks) * cost(list[0].m, list[0].n);
+            double top = 0.0;
+            int at = 0;
+            for (int b = 0; b < blocks; ++b) load[b] = 0.0;
+            for (int64_t i = 0; i < count; ++i) {
+                const double c = cost(list[i].m, list[i].n);
+                for (int64_t t = tiles(list[i].m, list[i].n); t > 0; --t) {
+                    load[at] += c;
+                    if (load[at] > top) top = load[at];
+                    if (++at == blocks) at = 0;
+                }
+            }
+            return top;
+        };
+        double sym = -1.0, upd = -1.0;
+        OrthoShape shape = {0, 0, pair, 1};
+        for (int w = w0; w < w1; ++w) {
+            for (int mirror = 0; mirror < 2; ++mirror) {
+                const double t = busiest(0, w, mirror);
+                if (sym < 0.0 || t < sym) sym = t, shape.bn_sym = OR_WIDTHS[w], shape.mirror = mirror;
+            }
+            const double t = busiest(1, w, 0);
+            if (upd < 0.0 || t < upd) upd = t, shape.bn_upd = OR_WIDTHS[w];
         }
-}
-static double or_cost(const OrthoWidths& W, int kind, int w) { return W.sum[kind][w] / sm_count() + 0.75 * W.top[kind][w]; }
-static void or_choose(const OrthoWidths& W, int& bn_sym, int& bn_upd, int& pair) {
-    int best[2];
-    for (int kind = 0; kind < 2; ++kind) {
-        best[kind] = 0;
-        for (int w = 1; w < 3; ++w)
-            if (or_cost(W, kind, w) < or_cost(W, kind, best[kind])) best[kind] = w;
+        if (least < 0.0 || sym + upd < least) least = sym + upd, best = shape;
     }
-    bn_sym = OR_WIDTHS[best[0]], bn_upd = OR_WIDTHS[best[1]];
-    pair = or_cost(W, 0, 3) + or_cost(W, 1, 3) < or_cost(W, 0, best[0]) + or_cost(W, 1, best[1]);
-    if (pair) bn_sym = bn_upd = 256;
+    return best;
 }
 
 static int64_t or_up(int64_t v) { return (v + 1023) / 1024 * 1024; }
@@ -1730,10 +1763,9 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
     const int64_t xs = x_type == 0 ? 4 : 2, os = out_type == 0 ? 4 : 2;
     for (int64_t at = 0; at < batch; at += k) {
         O.count = batch - at < k ? batch - at : k;
-        OrthoWidths W = {};
-        or_weigh(W, m, n, O.count);
-        or_choose(W, O.bn_sym, O.bn_upd, O.pair);
-        O.one_sym = or_syms(m, O.bn_sym, O.pair), O.one_upd = or_upds(m, n, O.bn_upd, O.pair);
+        const OrthoShape shape = or_choose(&O.one, O.count, true);
+        O.bn_sym = shape.bn_sym, O.bn_upd = shape.bn_upd, O.pair = shape.pair, O.mirror = shape.mirror;
+        O.one_sym = or_syms(m, O.bn_sym, O.pair, O.mirror), O.one_upd = or_upds(m, n, O.bn_upd, O.pair);
         O.spans = O.count * O.one_span, O.convs = O.count * O.one_conv;
         O.syms = O.count * O.one_sym, O.upds = O.count * O.one_upd;
         O.x = static_cast<const unsigned char*>(x) + at * rows * cols * xs;
@@ -1767,17 +1799,16 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
         if (p.team) return p.team > q.team;
         return p.m != q.m ? p.m > q.m : p.n > q.n;
     });
-    OrthoWidths W = {};
     int64_t general = 0, spans = 0, slots = 0;
-    for (; general < count && !list[general].team; ++general) or_weigh(W, list[general].m, list[general].n, 1);
+    for (; general < count && !list[general].team;) ++general;
     for (int64_t i = 0; i < count; ++i) {
         list[i].span0 = spans;
         spans += or_spans((int64_t)list[i].m * list[i].n);
         list[i].slot0 = slots;
         slots += list[i].team;
     }
-    int bn_sym, bn_upd, pair;
-    or_choose(W, bn_sym, bn_upd, pair);  // of the others
+    const OrthoShape shape = or_choose(list, general, false);
+    const int bn_sym = shape.bn_sym, bn_upd = shape.bn_upd, pair = shape.pair;
     int64_t waves = 0, most = 0;
     int64_t* wave = plan + 8;
     OrthoDesc at = {};
@@ -1793,14 +1824,14 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
         list[i].ws = at.ws, list[i].conv0 = at.conv0, list[i].sym0 = at.sym0, list[i].upd0 = at.upd0;
         at.ws += bytes;
         at.conv0 += (int64_t)or_mb(m) * or_b64(n);
-        at.sym0 += or_syms(m, bn_sym, pair);
+        at.sym0 += or_syms(m, bn_sym, pair, shape.mirror);
         at.upd0 += or_upds(m, n, bn_upd, pair);
         if (at.ws > most) most = at.ws;
         wave[1] = i + 1 - wave[0], wave[2] = at.conv0, wave[3] = at.sym0, wave[4] = at.upd0;
     }
     plan[0] = 1024 + or_up(spans * 8) + most;
     plan[1] = spans, plan[2] = waves, plan[3] = bn_sym, plan[4] = bn_upd;
-    plan[5] = pair, plan[6] = general, plan[7] = slots;
+    plan[5] = pair + 2 * shape.mirror, plan[6] = general, plan[7] = slots;
     plan[8 + 5 * waves] = slots ? list[general].team : 0;  // the clusters' size
     return 0;
 }
@@ -1820,7 +1851,7 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
     O.barrier = reinterpret_cast<uint32_t*>(w);
     O.sums = reinterpret_cast<double*>(w + 1024);
     O.tiles = w + 1024 + or_up(plan[1] * 8);
-    O.bn_sym = (int)plan[3], O.bn_upd = (int)plan[4], O.pair = (int)plan[5];
+    O.bn_sym = (int)plan[3], O.bn_upd = (int)plan[4], O.pair = (int)plan[5] & 1, O.mirror = (int)plan[5] >> 1;
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.precise = 1;
     O.grad = grad, O.momentum = momentum, O.master = master, O.controls = controls;
