@@ -46,9 +46,9 @@ constexpr int ORTHO_PRODUCERS = 3;      // warps that issue bulk copies, a third
 constexpr int ORTHO_THREADS = 32 * (1 + ORTHO_PRODUCERS + ORTHO_EPI_WARPS);  // warp 0 issues the products
 constexpr int ORTHO_RING = 192 * 1024;  // operand stages
 constexpr int ORTHO_STAGES = 8;         // at most
-constexpr int ORTHO_BLOCK = 2048;       // a staging block; an epilogue warp has two
+constexpr int ORTHO_BLOCK = 4096;       // an epilogue warp's staging block
 constexpr int ORTHO_EYE = 2048;         // 16 rows of 128 bytes: (b / c) 2^13 I in fp16 (2^13 I where c is 0), hi, and lo 32 bytes on
-constexpr int ORTHO_STAGING = 2 * ORTHO_EPI_WARPS * ORTHO_BLOCK;
+constexpr int ORTHO_STAGING = ORTHO_EPI_WARPS * ORTHO_BLOCK;
 constexpr int ORTHO_SMEM = 1024 + ORTHO_RING + ORTHO_STAGING + ORTHO_EYE;
 constexpr int ORTHO_FLAT = 256;         // threads of the kernels around the products
 constexpr int ORTHO_SPAN = ORTHO_FLAT * 16;  // elements whose squares one block sums
@@ -531,50 +531,43 @@ __device__ __forceinline__ OrthoPlace or_place(const OrthoArgs& O, const OrthoDe
 }
 
 // A thread's 64 finished values of one row as a row of a 128 x 64 tile, hi then lo, by way of the warp's
-// staging blocks of 16 rows (rows of 128 bytes are contiguous in the tile, so each block is one bulk copy):
-// two, or four where the warp of the other column part has no columns.
-__device__ __forceinline__ void or_store_rows(uint32_t blk, int blocks, unsigned char* dst, int lane, float* v, int parts) {
+// staging block of 32 rows (rows of 128 bytes are contiguous in the tile, so each part is one bulk copy); lo
+// has a block of its own where the warp of the other column part has no columns (`spare`).
+__device__ __forceinline__ void or_store_rows(uint32_t blk, uint32_t spare, unsigned char* dst, int lane, float* v, int parts) {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
 #pragma unroll 1
-    for (int round = 0; round < 2 * parts; ++round) {
-        {
-            const bool low = round >= 2;
-            if (round >= blocks) {
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                __syncwarp();
-            }
-            const uint32_t at = blk + (uint32_t)(round & 1) * ORTHO_BLOCK + (low && blocks == 4 ? 8u * ORTHO_BLOCK : 0u);
-            if ((lane >> 4) == (round & 1)) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // opaque, or the conversions of every round would be made and kept before the first
-                        asm volatile("" : "+f"(v[8 * q + 2 * j]), "+f"(v[8 * q + 2 * j + 1]));
-                        const float x0 = v[8 * q + 2 * j], x1 = v[8 * q + 2 * j + 1];
-                        __half2 h = __floats2half2_rn(x0, x1);
-                        if (low) {
-                            const float2 f = __half22float2(h);
-                            h = __floats2half2_rn(x0 - f.x, x1 - f.y);
-                        }
-                        w[j] = *reinterpret_cast<uint32_t*>(&h);
-                    }
-                    const uint32_t addr = at + (uint32_t)(lane & 15) * 128u + (uint32_t)((q ^ (lane & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                                 "r"(w[3])
-                                 : "memory");
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    for (int low = 0; low < parts; ++low) {
+        const uint32_t at = low && spare ? spare : blk;
+        if (low && !spare) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
-            if (lane == 0) {
-                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::
-                                 "l"(dst + (low ? 16384 : 0) + (round & 1) * 2048), "r"(at), "r"(2048u)
-                             : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // opaque, or the conversions of both parts would be made and kept before the first
+                asm volatile("" : "+f"(v[8 * q + 2 * j]), "+f"(v[8 * q + 2 * j + 1]));
+                const float x0 = v[8 * q + 2 * j], x1 = v[8 * q + 2 * j + 1];
+                __half2 h = __floats2half2_rn(x0, x1);
+                if (low) {
+                    const float2 f = __half22float2(h);
+                    h = __floats2half2_rn(x0 - f.x, x1 - f.y);
+                }
+                w[j] = *reinterpret_cast<uint32_t*>(&h);
             }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (uint32_t)lane * 128u + (uint32_t)((q ^ (lane & 7)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (low ? 16384 : 0)), "r"(at), "r"(4096u)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
     }
 }
@@ -591,7 +584,7 @@ __device__ __forceinline__ void or_write_one(const OrthoArgs& O, const OrthoOut&
 }
 
 // The last update: 64 columns of a warp's 32 rows to the output or the master, 32 columns at a time by way
-// of the warp's staging blocks (32 rows of 128 bytes, chunks swizzled by the row), so that lanes are
+// of the warp's staging block (32 rows of 128 bytes, chunks swizzled by the row), so that lanes are
 // neighbours in memory whichever side is stored along.  Loops are kept rolled: each launch runs this once, and
 // unrolled its instructions took longer to fetch (12 us) than to run.  v is used up.
 __device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int row, int cb, uint32_t blk, int lane, float* v) {
@@ -693,14 +686,14 @@ __device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int
 // what an epilogue warp does with its 32 rows x 64 columns (rows row - lane ..., column block cb of 64)
 template <bool PRECISE>
 __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step, int which, int i, int row, int cb,
-                                          uint32_t blk, int blocks, int lane, float* v) {
+                                          uint32_t blk, uint32_t spare, int lane, float* v) {
     const OrthoPlace L = or_place(O, or_get(O, which), step);
     const int r0 = row - lane;
     if (kind == OR_UPDATE) {
 #pragma unroll
         for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
         unsigned char* tile = L.x_next + i * L.x_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
-        or_store_rows(blk, blocks, tile, lane, v, 2);
+        or_store_rows(blk, spare, tile, lane, v, 2);
         return;
     }
     if (O.mirror && (cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
@@ -711,7 +704,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
 #pragma unroll
     for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == cb * 64 + j ? diagonal : 0.0f);
     unsigned char* tile = dst + i * L.a_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
-    or_store_rows(blk, blocks, tile, lane, v, PRECISE ? 2 : 1);
+    or_store_rows(blk, spare, tile, lane, v, PRECISE ? 2 : 1);
     if (O.mirror && cb * 64 >= (i + 1) * 128) {
         // the mirrored place of (row, cb * 64 + j): row block cb / 2, column block row / 64, row (cb & 1) * 64 + j
         // of that tile; lanes are neighbours
@@ -973,8 +966,8 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
     const int chunk = PRECISE && !(kind == OR_SQUARE && O.c == 0.0f) ? 1 : 1 << 20;
     const uint32_t shift = or_buffers(O), buffers = 1u << shift;
     const int group0 = bn > 128 ? 2 * part : part;
-    const int blocks = bn == 64 ? 4 : 2;
-    const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * (2u * ORTHO_BLOCK);
+    const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * ORTHO_BLOCK;
+    const uint32_t spare = bn == 64 ? blk + 4u * ORTHO_BLOCK : 0u;  // the other column part's
     const uint32_t taddr0 = S.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(group0 * 64);
     bool ok = true;
     for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
@@ -1014,7 +1007,7 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
             const int cb = (T.c0 >> 6) + group0 + g;
             if (!ok || g >= groups || (PAIR && (cb >= last_cb || T.i >= or_mb(m)))) continue;
             if (kind == OR_UPDATE && step == O.steps - 1) or_finish_out(O, T.which, row, cb, blk, lane, v + 64 * g);
-            else or_finish<PRECISE>(O, kind, step, T.which, T.i, row, cb, blk, blocks, lane, v + 64 * g);
+            else or_finish<PRECISE>(O, kind, step, T.which, T.i, row, cb, blk, spare, lane, v + 64 * g);
         }
     }
     if (!ok) {
@@ -1440,7 +1433,7 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
                         for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
                         or_keep_rows(xs + part * ORTHO_TILE, row, v);
                     } else {
-                        or_finish_out(O, which, row, first + part, sums + (uint32_t)e * (2u * ORTHO_BLOCK), lane, v);
+                        or_finish_out(O, which, row, first + part, sums + (uint32_t)e * ORTHO_BLOCK, lane, v);
                     }
                 }
             }
