@@ -6,19 +6,26 @@
 // Both are bound by HBM: the forward reads each looked-up row and writes each output row once, the
 // backward reads each incoming row once and writes each table row once.
 //
-// The backward is one cooperative kernel without floating-point atomics, so the result is the same in
-// every run:
-//   1. a stable radix sort of (index, position) pairs: least significant digit first, at most 9 bits
-//      a pass (the least number of passes, bits shared evenly).  Each sorting block owns a contiguous
-//      range of tokens; a pass is its digit histogram, a scan of every digit's counts over the blocks,
-//      and the scatter, where a warp ranks 32 keys at a time by matching equal digits.  One block
-//      sorts alone, without grid barriers, when it holds all tokens.
-//   2. segment sums over equal shares of the sorted list (not of the table: a row looked up by half
-//      of the tokens is shared by as many workers as its tokens deserve).  A worker is a group of 8,
-//      16 or 32 lanes with 16-byte vectors side by side on a row; it keeps one fp32 sum per column in
-//      registers, four or eight rows in flight.  Runs inside a share are written at once; a run that crosses a
-//      border leaves its part in the workspace.
-//   3. the parts of each crossing run, added in order.
+// The backward has no floating-point atomics, so the result is the same in every run.  By size (measured
+// times are at 1965 MHz):
+//   - few tokens (EMB_SCAN): no sort.  A warp (up to 256 tokens) or a block per table row looks through all
+//     indices, 32 at a time, and adds the rows that match.  16 tokens into 50 x 64: 3.0 us, where the sort's
+//     phases alone take 12.
+//   - few table rows (EMB_TABLE): every warp keeps the whole table's sums for its columns in shared memory
+//     and adds its share of the tokens' rows in order; then the warps' and the blocks' tables are added in
+//     order.  1,000,003 x 128 bf16 into 4 rows: the sort and its gathered reads take 126 us.
+//   - else sorted tokens, one cooperative kernel:
+//     1. a stable radix sort of (index, position) pairs: least significant digit first, at most 9 bits a
+//        pass (the least number of passes, bits shared evenly).  Each sorting block owns a contiguous range
+//        of tokens; a pass is its digit histogram, a scan of every digit's counts over the blocks, and the
+//        scatter, where a warp ranks 32 keys at a time by matching equal digits.  The blocks that do not
+//        sort zero the table meanwhile.
+//     2. segment sums over equal shares of the sorted list (not of the table: a row looked up by half of the
+//        tokens is shared by as many workers as its tokens deserve).  A worker is a group of 8, 16 or 32
+//        lanes with 16-byte vectors side by side on a row; it keeps one fp32 sum per column in registers,
+//        four or eight rows in flight.  Runs inside a share are written at once; a run that crosses a border
+//        leaves its part in the workspace.
+//     3. the parts of each crossing run, added in order.
 // An index outside [0, rows) yields a row of zeros, takes no gradient and sets the sticky error word;
 // tokens with the padding index take no gradient.
 #include <cuda_bf16.h>
@@ -121,6 +128,16 @@ struct EmbArgs {
     uint32_t* error;
 };
 
+// a looked-up vector, scaled (zeros where the index is outside the table)
+template <typename T, int VEC>
+__device__ __forceinline__ void emb_scaled(const EmbArgs& E, int64_t at, bool live, const EmbVec<T, VEC>& x) {
+    float f[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[k] = live ? emb_float(x.v[k]) * E.scale : 0.0f;
+    emb_store<VEC>(E.out, at, E.out_type, f);
+}
+
+// Rows of more than a vector per lane: a group of lanes per row, four vectors a lane in flight.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embedding_kernel(EmbArgs E) {
     const int lanes = 1 << E.log_lanes;
@@ -134,28 +151,51 @@ __global__ void __launch_bounds__(256) embedding_kernel(EmbArgs E) {
         if (!live && lane == 0) *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
         const T* src = table + (live ? i : 0) * E.ldt;
         for (int64_t c0 = (int64_t)lane * VEC; c0 < E.width; c0 += (int64_t)lanes * VEC * 4) {
-            float f[4][VEC];
+            EmbVec<T, VEC> x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int64_t c = c0 + (int64_t)u * lanes * VEC;
-                if (live && c < E.width) {
-                    emb_load<T, VEC>(src + c, f[u]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k) f[u][k] = 0.0f;
-                }
+                if (live && c < E.width) x[u] = *reinterpret_cast<const EmbVec<T, VEC>*>(src + c);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int64_t c = c0 + (int64_t)u * lanes * VEC;
-                if (c < E.width) {
-                    if (live) {
-#pragma unroll
-                        for (int k = 0; k < VEC; ++k) f[u][k] *= E.scale;
-                    }
-                    emb_store<VEC>(E.out, t * E.width + c, E.out_type, f[u]);
-                }
+                if (c < E.width) emb_scaled<T, VEC>(E, t * E.width + c, live, x[u]);
             }
+        }
+    }
+}
+
+// Rows of at most a vector per lane: eight rows a group in flight, indices first.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) embedding_rows_kernel(EmbArgs E) {
+    const int lanes = 1 << E.log_lanes, groups = 256 >> E.log_lanes;
+    const int lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> E.log_lanes;
+    const int64_t c = (int64_t)lane * VEC;
+    const bool in = c < E.width;
+    const T* table = static_cast<const T*>(E.table);
+    for (int64_t t0 = (int64_t)blockIdx.x * groups * 8; t0 < E.tokens; t0 += (int64_t)gridDim.x * groups * 8) {
+        int64_t i[8];
+        EmbVec<T, VEC> x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int64_t t = t0 + u * groups + group;
+            i[u] = t < E.tokens ? emb_index(E.index, E.index64, t) : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int64_t t = t0 + u * groups + group;
+            if (i[u] < 0 || i[u] >= E.rows) {
+                if (t < E.tokens) *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
+                i[u] = -1;
+            } else if (in && t < E.tokens) {
+                x[u] = *reinterpret_cast<const EmbVec<T, VEC>*>(table + i[u] * E.ldt + c);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int64_t t = t0 + u * groups + group;
+            if (in && t < E.tokens) emb_scaled<T, VEC>(E, t * E.width + c, i[u] >= 0, x[u]);
         }
     }
 }
@@ -632,6 +672,185 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbG
     }
 }
 
+// ---------------------------------------------------------------- few tokens
+
+constexpr int EMB_SCAN_TOKENS = 4096;  // at most
+constexpr int EMB_SCAN_WARP = 256;     // up to here a warp per table row
+
+// the rows of the tokens in `match` (bits of tokens t0 ..), added in order, eight in flight
+template <typename T, int VEC>
+__device__ __forceinline__ void emb_add_matches(const EmbGradArgs& E, uint32_t match, int64_t t0, int64_t c, bool in, float* sum) {
+    const T* grad = static_cast<const T*>(E.grad);
+    while (match) {
+        EmbVec<T, VEC> x[8];
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (match) {
+                const int64_t t = t0 + __ffs(match) - 1;
+                match &= match - 1;
+                if (in) x[u] = *reinterpret_cast<const EmbVec<T, VEC>*>(grad + t * E.ldg + c);
+                n = u + 1;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (u < n && in) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sum[i] += emb_float(x[u].v[i]);
+            }
+        }
+    }
+}
+
+// a warp per table row (in turn), all indices in its lanes
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) embedding_backward_warp_kernel(EmbGradArgs E) {
+    const int lane = threadIdx.x & 31;
+    constexpr int K = EMB_SCAN_WARP / 32;
+    uint32_t key[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) key[k] = k * 32 + lane < E.tokens ? emb_key(E, k * 32 + lane) : 0xffffffffu;
+    for (int64_t r = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5; r < E.rows; r += (int64_t)gridDim.x * 8) {
+        uint32_t match[K], any = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            match[k] = k * 32 < E.tokens ? __ballot_sync(0xffffffffu, key[k] == (uint32_t)r) : 0u;
+            any |= match[k];
+        }
+        if (!any && E.accumulate) continue;
+        for (int64_t c = (int64_t)lane * VEC; c - lane * VEC < E.width; c += 32 * VEC) {
+            const bool in = c < E.width;
+            float sum[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+            if (any) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) emb_add_matches<T, VEC>(E, match[k], k * 32, c, in, sum);
+            }
+            if (in) emb_finish<VEC>(E, (uint32_t)r, c, sum);
+        }
+    }
+}
+
+// a block per table row and column tile: each warp a stretch of the indices, the warps' sums added in order
+template <typename T, int VEC>
+__global__ void __launch_bounds__(EMB_THREADS) embedding_backward_block_kernel(EmbGradArgs E) {
+    __shared__ float part[EMB_WARPS][32 * VEC];
+    __shared__ int any_s;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r = blockIdx.x, c = (int64_t)blockIdx.y * 32 * VEC + (int64_t)lane * VEC;
+    const bool in = c < E.width;
+    const int64_t each = ((E.tokens + EMB_WARPS - 1) / EMB_WARPS + 31) & ~31ll;
+    const int64_t lo = warp * each, hi = lo + each < E.tokens ? lo + each : E.tokens;
+    if (threadIdx.x == 0) any_s = 0;
+    __syncthreads();
+    float sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+    bool any = false;
+    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
+        const uint32_t key = t0 + lane < hi ? emb_key(E, t0 + lane) : 0xffffffffu;
+        const uint32_t match = __ballot_sync(0xffffffffu, key == (uint32_t)r);
+        any |= match != 0;
+        emb_add_matches<T, VEC>(E, match, t0, c, in, sum);
+    }
+    if (any) any_s = 1;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) part[warp][i * 32 + lane] = sum[i];
+    __syncthreads();
+    if (warp == 0 && in && (any_s || !E.accumulate)) {
+        for (int w = 1; w < EMB_WARPS; ++w) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum[i] += part[w][i * 32 + lane];
+        }
+        emb_finish<VEC>(E, (uint32_t)r, c, sum);
+    }
+}
+
+// ---------------------------------------------------------------- few table rows
+
+constexpr int EMB_TABLE_BYTES = 104 * 1024;  // a block's tables: two blocks fit an SM
+constexpr int EMB_TABLE_ROWS = 52;           // at most: four warps' tables of 128 columns
+
+// grid (blocks, column tiles); E.parts warps a block; tables [warp][row][32 lanes x VEC]
+template <typename T, int VEC>
+__global__ void __launch_bounds__(EMB_THREADS) embedding_backward_table_kernel(EmbGradArgs E) {
+    extern __shared__ __align__(16) float emb_tables[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = E.parts;
+    const int rows = (int)E.rows;
+    const int64_t c = (int64_t)blockIdx.y * 32 * VEC + (int64_t)lane * VEC;
+    const bool in = c < E.width;
+    const T* grad = static_cast<const T*>(E.grad);
+    EmbVec<float, VEC>* table = reinterpret_cast<EmbVec<float, VEC>*>(emb_tables) + (size_t)warp * rows * 32 + lane;
+    EmbVec<float, VEC> zero;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) zero.v[i] = 0.0f;
+    for (int r = 0; r < rows; ++r) table[r * 32] = zero;
+    // each warp a contiguous stretch
+    const int64_t lo = ((int64_t)blockIdx.x * warps + warp) * E.share, hi = lo + E.share < E.tokens ? lo + E.share : E.tokens;
+    for (int64_t t0 = lo; t0 < hi; t0 += 32) {
+        const uint32_t my_key = t0 + lane < hi ? emb_key(E, t0 + lane) : (uint32_t)rows;
+        const int n = hi - t0 < 32 ? (int)(hi - t0) : 32;
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            if (j0 >= n) break;
+            EmbVec<T, VEC> x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t k = __shfl_sync(0xffffffffu, my_key, j0 + j);
+                if (in && k < (uint32_t)rows) x[j] = *reinterpret_cast<const EmbVec<T, VEC>*>(grad + (t0 + j0 + j) * E.ldg + c);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t k = __shfl_sync(0xffffffffu, my_key, j0 + j);
+                if (k < (uint32_t)rows) {
+                    EmbVec<float, VEC> f = table[k * 32];
+                    if (in) {
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) f.v[i] += emb_float(x[j].v[i]);
+                    }
+                    table[k * 32] = f;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    // the warps' tables in order -> this block's, [block][row][width]
+    for (int r = warp; r < rows; r += warps) {
+        EmbVec<float, VEC> f = zero;
+        for (int w = 0; w < warps; ++w) {
+            const EmbVec<float, VEC> g = reinterpret_cast<EmbVec<float, VEC>*>(emb_tables)[((size_t)w * rows + r) * 32 + lane];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f.v[i] += g.v[i];
+        }
+        if (in) emb_store<VEC>(E.part_sums, ((int64_t)blockIdx.x * rows + r) * E.width + c, EMB_F32, f.v);
+    }
+}
+
+// the blocks' tables in order: 32 columns and 16 stretches of the blocks a block
+__global__ void __launch_bounds__(EMB_THREADS) embedding_backward_fold_kernel(EmbGradArgs E, int blocks) {
+    __shared__ float part[EMB_WARPS][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t total = E.rows * E.width, at = (int64_t)blockIdx.x * 32 + lane;
+    const int each = (blocks + EMB_WARPS - 1) / EMB_WARPS, lo = warp * each, hi = lo + each < blocks ? lo + each : blocks;
+    float sum = 0.0f;
+    if (at < total) {
+        for (int b = lo; b < hi; b += 4) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = b + u < hi ? __ldg(E.part_sums + (int64_t)(b + u) * total + at) : 0.0f;
+            sum += (x[0] + x[1]) + (x[2] + x[3]);
+        }
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && at < total) {
+        for (int w = 1; w < EMB_WARPS; ++w) sum += part[w][lane];
+        emb_finish<1>(E, (uint32_t)(at / E.width), at % E.width, &sum);
+    }
+}
+
 // ---------------------------------------------------------------- host
 
 // elements of a vector access: the widest of 16 bytes that width, strides and addresses allow
@@ -646,20 +865,32 @@ static int emb_vec(int size, int64_t width, int64_t ld, const void* p, int out_s
 
 static int emb_size(int type) { return type == EMB_F32 ? 4 : 2; }
 
+template <typename T, int VEC>
+static void (*emb_forward_of(bool one))(EmbArgs) { return one ? embedding_rows_kernel<T, VEC> : embedding_kernel<T, VEC>; }
 template <typename T>
-static void (*emb_forward_kernel(int vec))(EmbArgs) {
+static void (*emb_forward_kernel(int vec, bool one))(EmbArgs) {
     if constexpr (sizeof(T) == 2) {
-        if (vec == 8) return embedding_kernel<T, 8>;
+        if (vec == 8) return emb_forward_of<T, 8>(one);
     }
-    return vec == 4 ? embedding_kernel<T, 4> : vec == 2 ? embedding_kernel<T, 2> : embedding_kernel<T, 1>;
+    return vec == 4 ? emb_forward_of<T, 4>(one) : vec == 2 ? emb_forward_of<T, 2>(one) : emb_forward_of<T, 1>(one);
 }
 
-template <typename T>
-static void (*emb_backward_kernel(int vec))(EmbGradArgs) {
-    if constexpr (sizeof(T) == 2) {
-        if (vec == 8) return embedding_backward_kernel<T, 8>;
+enum { EMB_SORT = 0, EMB_WARP = 1, EMB_BLOCK = 2, EMB_TABLE = 3 };
+template <typename T, int VEC>
+static void (*emb_backward_of(int path))(EmbGradArgs) {
+    if (path == EMB_WARP) return embedding_backward_warp_kernel<T, VEC>;
+    if (path == EMB_BLOCK) return embedding_backward_block_kernel<T, VEC>;
+    if constexpr (VEC <= 4) {
+        if (path == EMB_TABLE) return embedding_backward_table_kernel<T, VEC>;
     }
-    return vec == 4 ? embedding_backward_kernel<T, 4> : vec == 2 ? embedding_backward_kernel<T, 2> : embedding_backward_kernel<T, 1>;
+    return embedding_backward_kernel<T, VEC>;
+}
+template <typename T>
+static void (*emb_backward_kernel(int vec, int path))(EmbGradArgs) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 8) return emb_backward_of<T, 8>(path);
+    }
+    return vec == 4 ? emb_backward_of<T, 4>(path) : vec == 2 ? emb_backward_of<T, 2>(path) : emb_backward_of<T, 1>(path);
 }
 
 struct EmbLayout {
@@ -700,7 +931,9 @@ static void emb_plan(int64_t tokens, int64_t rows, int64_t width, int vec, int g
         E.part_tokens = per * whole;
         E.parts = (int)((tokens + E.part_tokens - 1) / E.part_tokens);
     }
-    E.zero_first = !E.accumulate && tokens <= rows / 4;
+    // zeroing beside the sort is free up to what the device writes in its time; every row twice costs more
+    // than looking for the absent ones only in a large table that most tokens' rows fill
+    E.zero_first = !E.accumulate && (tokens <= rows || rows * width * 4 <= (192ll << 20));
     int64_t want = (E.shares * E.tiles + per_block - 1) / per_block;
     if (want < E.parts) want = E.parts;
     if (!E.accumulate) {  // blocks for the zeroed rows: 64 KB each
@@ -725,7 +958,10 @@ static EmbLayout emb_layout(int64_t tokens, int64_t width, int grid_max) {
     // their columns are at most 8 per resident thread
     const int64_t by_tokens = (tokens + EMB_MIN_SHARE - 1) / EMB_MIN_SHARE * width;
     const int64_t by_threads = (int64_t)grid_max * EMB_THREADS * 8 + 2 * width;
-    L.parts = at, at += up((by_tokens < by_threads ? by_tokens : by_threads) * 2 * 4);
+    const int64_t sums = (by_tokens < by_threads ? by_tokens : by_threads) * 2;
+    // a table of sums per block, grid_max / (column tiles of at least 32 columns) blocks or one
+    const int64_t tables = EMB_TABLE_ROWS * ((int64_t)grid_max * 128 + width);
+    L.parts = at, at += up((sums > tables ? sums : tables) * 4);
     L.bytes = at;
     return L;
 }
@@ -756,11 +992,12 @@ int pbg_embedding(int64_t tokens, int64_t rows, int64_t width, const void* index
     E.log_lanes = 0;
     while (E.log_lanes < 5 && (1LL << E.log_lanes) < vectors) ++E.log_lanes;
     while (E.log_lanes < 8 && (4LL << E.log_lanes) < vectors) ++E.log_lanes;
-    const int64_t need = ((tokens << E.log_lanes) + 255) / 256;
+    const bool one = vectors <= (1LL << E.log_lanes) && tokens > (8LL << (8 - E.log_lanes)) * sm_count();  // eight rows a group fill the device
+    const int64_t need = one ? ((tokens << E.log_lanes) + 2047) / 2048 : ((tokens << E.log_lanes) + 255) / 256;
     const int64_t most = (int64_t)sm_count() * 32;
-    void (*kernel)(EmbArgs) = table_type == EMB_F32 ? emb_forward_kernel<float>(vec)
-                              : table_type == EMB_BF16 ? emb_forward_kernel<__nv_bfloat16>(vec)
-                                                       : emb_forward_kernel<__half>(vec);
+    void (*kernel)(EmbArgs) = table_type == EMB_F32 ? emb_forward_kernel<float>(vec, one)
+                              : table_type == EMB_BF16 ? emb_forward_kernel<__nv_bfloat16>(vec, one)
+                                                       : emb_forward_kernel<__half>(vec, one);
     kernel<<<(unsigned)(need < most ? need : most), 256, 0, as_stream(stream)>>>(E);
     return launch_status("embedding");
 }
@@ -810,9 +1047,53 @@ int pbg_embedding_backward(int64_t tokens, int64_t rows, int64_t width, const vo
     E.pos[0] = reinterpret_cast<int32_t*>(w + L.pos0);
     E.pos[1] = reinterpret_cast<int32_t*>(w + L.pos1);
     E.part_sums = reinterpret_cast<float*>(w + L.parts);
-    void (*kernel)(EmbGradArgs) = grad_type == EMB_F32 ? emb_backward_kernel<float>(vec)
-                                  : grad_type == EMB_BF16 ? emb_backward_kernel<__nv_bfloat16>(vec)
-                                                          : emb_backward_kernel<__half>(vec);
+    auto of = [&](int v, int path) {
+        return grad_type == EMB_F32 ? emb_backward_kernel<float>(v, path)
+               : grad_type == EMB_BF16 ? emb_backward_kernel<__nv_bfloat16>(v, path) : emb_backward_kernel<__half>(v, path);
+    };
+    const int64_t column_tiles = (width + 32 * vec - 1) / (32 * vec);
+    if (tokens <= EMB_SCAN_WARP) {
+        const int64_t need = (rows + 7) / 8, most = (int64_t)sm_count() * 8;
+        of(vec, EMB_WARP)<<<(unsigned)(need < most ? need : most), 256, 0, s>>>(E);
+        return launch_status("embedding_backward");
+    }
+    // a block per row and column tile: up to a few of them per SM at once
+    if (tokens <= EMB_SCAN_TOKENS && rows * column_tiles <= 8 * (int64_t)sm_count() && column_tiles < 65536) {
+        of(vec, EMB_BLOCK)<<<dim3((unsigned)rows, (unsigned)column_tiles), EMB_THREADS, 0, s>>>(E);
+        return launch_status("embedding_backward");
+    }
+    if (rows <= EMB_TABLE_ROWS && width >= 32) {
+        // 32 lanes' vectors of at most 16 bytes of sums, no wider than the row
+        int v = vec > 4 ? 4 : vec;
+        while (v > 1 && 16 * v >= width) v /= 2;
+        const int64_t table = rows * 32 * v * 4, tiles = (width + 32 * v - 1) / (32 * v);
+        const int warps = (int)(EMB_TABLE_BYTES / table < EMB_WARPS ? EMB_TABLE_BYTES / table : EMB_WARPS);
+        int64_t blocks = grid_max / tiles > 1 ? grid_max / tiles : 1;
+        const int64_t least = (tokens + 32 * warps - 1) / (32 * warps);  // 32 tokens a warp at least
+        if (blocks > least) blocks = least;
+        E.parts = warps;
+        E.share = ((tokens + blocks * warps - 1) / (blocks * warps) + 31) / 32 * 32;
+        blocks = (tokens + E.share * warps - 1) / (E.share * warps);
+        if (tiles < 65536) {
+            auto table_kernel = of(v, EMB_TABLE);
+            static int configured[64][3][3] = {};
+            int dev = 0;
+            cudaGetDevice(&dev);
+            const int vi = v == 4 ? 2 : v - 1;
+            if (dev < 0 || dev >= 64 || !configured[dev][grad_type][vi]) {
+                const int rc = cuda_status(cudaFuncSetAttribute(table_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EMB_TABLE_BYTES),
+                                           "embedding_backward: shared memory size");
+                if (rc) return rc;
+                if (dev >= 0 && dev < 64) configured[dev][grad_type][vi] = 1;
+            }
+            table_kernel<<<dim3((unsigned)blocks, (unsigned)tiles), 32 * warps, (size_t)(warps * table), s>>>(E);
+            const int rc = launch_status("embedding_backward");
+            if (rc) return rc;
+            embedding_backward_fold_kernel<<<(unsigned)((rows * width + 31) / 32), EMB_THREADS, 0, s>>>(E, (int)blocks);
+            return launch_status("embedding_backward: fold");
+        }
+    }
+    auto kernel = of(vec, EMB_SORT);
     if (grid == 1) {
         kernel<<<1, EMB_THREADS, 0, s>>>(E);
         return launch_status("embedding_backward");

@@ -76,6 +76,18 @@ CASES = [
     (700, 40, 8192, F32, F32, "half"),        # 64 column tiles
     (300007, 3, 8, BF16, BF16, "one"),
     (90000, 50021, 264, F32, BF16, "zipf"),
+    (256, 40, 33, F32, F32, "zipf"),          # the last size of a warp per row, the first of a block per row
+    (257, 40, 33, F32, F32, "zipf"),
+    (200, 100003, 12, F16, F32, "half"),
+    (4096, 1000, 64, BF16, F32, "half"),      # the last size that is not sorted
+    (4096, 3, 2000, F32, F16, "one"),
+    (1000, 5000, 64, F32, F32, "zipf"),       # few tokens, but rows for the sort
+    (5000, 52, 32, F32, F32, "uniform"),      # the largest table that is kept whole, the smallest width
+    (5000, 53, 32, F32, F32, "uniform"),
+    (5000, 52, 31, F32, F32, "uniform"),
+    (9000, 40, 4102, BF16, F32, "zipf"),      # 65 column tiles of a kept table, odd pairs
+    (5000, 1, 130, F16, BF16, "one"),
+    (20011, 21, 100, BF16, F32, "half"),
 ]
 
 
@@ -100,7 +112,7 @@ def test_gradient_matches_float64(tokens, rows, width, gtype, otype, law):
 @pytest.mark.parametrize("tokens,rows,width,ttype,otype", [
     (1, 1, 1, F32, F32), (16, 4096, 1024, BF16, BF16), (5, 9, 8192, F32, BF16), (1000, 13, 128, F32, F32),
     (33, 7, 65, BF16, F32), (129, 50, 2046, F16, F16), (3, 5, 36, F32, F16), (70001, 169, 32, F32, F32),
-    (4097, 3000, 200, F16, BF16), (40000, 77, 6, BF16, BF16)])
+    (4097, 3000, 200, F16, BF16), (40000, 77, 6, BF16, BF16), (19000, 5, 128, F32, F32), (100003, 40, 250, BF16, F32)])
 @pytest.mark.parametrize("scale", [1.0, 11.3137085])
 def test_forward_is_one_product_and_one_rounding(tokens, rows, width, ttype, otype, scale):
     from pbg_b200.embedding import embedding
@@ -155,46 +167,47 @@ def test_empty_sizes():
     assert embedding_backward(torch.zeros(3, 0, device=DEV), some, 5).shape == (5, 0)
 
 
-@pytest.mark.parametrize("tokens", [100, 9000])
-def test_padding_and_indices_outside_the_table(tokens):
+@pytest.mark.parametrize("tokens,rows", [(100, 50), (3000, 50), (9000, 50), (9000, 500)])
+def test_padding_and_indices_outside_the_table(tokens, rows):
     from pbg_b200 import embedding as E
 
     gen = torch.Generator(device=DEV).manual_seed(tokens)
-    index = torch.randint(0, 50, (tokens,), generator=gen, device=DEV)
+    index = torch.randint(0, rows, (tokens,), generator=gen, device=DEV)
     grad = torch.randn(tokens, 40, generator=gen, device=DEV)
     assert E.index_error(DEV) == 0
-    _check_gradient(E.embedding_backward(grad, index, 50, padding_index=7), grad, index, 50, 1.0, padding=7)
+    _check_gradient(E.embedding_backward(grad, index, rows, padding_index=7), grad, index, rows, 1.0, padding=7)
     assert E.index_error(DEV) == 0
-    index[::3] = 50
+    index[::3] = rows
     index[1::17] = -1
     index[2::17] = 2 ** 40
     try:
-        _check_gradient(E.embedding_backward(grad, index, 50), grad, index, 50, 1.0)
+        _check_gradient(E.embedding_backward(grad, index, rows), grad, index, rows, 1.0)
         assert E.index_error(DEV) == 1
         E._error_word(DEV).zero_()
-        table = torch.randn(50, 40, generator=gen, device=DEV)
+        table = torch.randn(rows, 40, generator=gen, device=DEV)
         out = E.embedding(table, index, 3.0)
-        inside = (index >= 0) & (index < 50)
+        inside = (index >= 0) & (index < rows)
         assert bool((out[~inside] == 0).all()) and torch.equal(out[inside], 3.0 * table[index[inside]])
         assert E.index_error(DEV) == 1
-        all_out = torch.full((tokens,), 77, device=DEV)
-        assert bool((E.embedding_backward(grad, all_out, 50) == 0).all())
+        all_out = torch.full((tokens,), rows + 27, device=DEV)
+        assert bool((E.embedding_backward(grad, all_out, rows) == 0).all())
     finally:
         E._error_word(DEV).zero_()
 
 
-def test_non_finite_rows_stay_in_their_rows():
+@pytest.mark.parametrize("tokens,width", [(200, 24), (4000, 24), (6000, 24), (6000, 40)])
+def test_non_finite_rows_stay_in_their_rows(tokens, width):
     from pbg_b200.embedding import embedding_backward
 
-    index = torch.arange(6000, device=DEV) % 20
-    grad = torch.ones(6000, 24, device=DEV)
+    index = torch.arange(tokens, device=DEV) % 20
+    grad = torch.ones(tokens, width, device=DEV)
     grad[100] = float("nan")   # row 0
     grad[103] = float("inf")   # row 3
     got = embedding_backward(grad, index, 20)
     assert bool(got[0].isnan().all()) and bool(got[3].isinf().all())
     rest = torch.ones(20, dtype=torch.bool, device=DEV)
     rest[[0, 3]] = False
-    assert bool((got[rest] == 300).all())
+    assert bool((got[rest] == tokens // 20).all())
 
 
 def test_graph_replay_other_stream_and_two_graphs():
