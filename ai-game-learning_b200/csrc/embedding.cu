@@ -230,23 +230,23 @@ struct EmbGradArgs {
     float* part_sums;    // [shares][2][width]
 };
 
-// Arrivals counted in one word; the kernel is launched cooperatively, so every block runs.  A wait
-// that runs out records 2 in the error word and lets its block go on to the end of the kernel
-// without touching the output.
-__device__ __forceinline__ bool emb_grid_sync(const EmbGradArgs& E, uint32_t& target) {
-    if (gridDim.x == 1) {
+// Arrivals of `blocks` blocks counted in one word (E.barrier[0]: the whole grid, [1]: the sorting
+// blocks); the kernel is launched cooperatively, so every block runs.  A wait that runs out records 2 in
+// the error word and lets its block go on to the end of the kernel without touching the output.
+__device__ __forceinline__ bool emb_sync(const EmbGradArgs& E, int word, uint32_t blocks, uint32_t& target) {
+    if (blocks == 1) {
         __syncthreads();
         return true;
     }
     __shared__ int ok_s;
-    target += gridDim.x;
+    target += blocks;
     __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
-        uint32_t seen = atomicAdd(E.barrier, 1u) + 1u;
+        uint32_t seen = atomicAdd(E.barrier + word, 1u) + 1u;
         uint32_t i = 0;
         while ((int32_t)(seen - target) < 0 && i < EMB_WAIT_TRIES) {
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(E.barrier) : "memory");
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(E.barrier + word) : "memory");
             ++i;
         }
         const int ok = (int32_t)(seen - target) >= 0;
@@ -292,17 +292,16 @@ __device__ __forceinline__ uint32_t emb_block_scan(uint32_t v, uint32_t* warp_su
     return before + x - v;
 }
 
-// one radix pass of the calling block's range; false when a grid barrier gave up
+// one radix pass of the calling (sorting) block's range; false when a barrier gave up
 __device__ bool emb_radix_pass(const EmbGradArgs& E, int pass, uint32_t& target, EmbSortShared& S) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int shift = pass * E.bits, bins = 1 << E.bits;
     const uint32_t mask = (uint32_t)bins - 1u;
-    const bool sorting = (int)blockIdx.x < E.parts;
     const int64_t lo = (int64_t)blockIdx.x * E.part_tokens;
-    const int64_t hi = sorting ? (lo + E.part_tokens < E.tokens ? lo + E.part_tokens : E.tokens) : lo;
+    const int64_t hi = lo + E.part_tokens < E.tokens ? lo + E.part_tokens : E.tokens;
     const uint32_t* src_key = E.key[(pass & 1) ^ 1];
     const int32_t* src_pos = E.pos[(pass & 1) ^ 1];
-    if (sorting) {
+    {
         for (int b = threadIdx.x; b < bins; b += EMB_THREADS) S.base[b] = 0;
         __syncthreads();
         for (int64_t t0 = lo; t0 < hi; t0 += EMB_THREADS) {
@@ -315,17 +314,14 @@ __device__ bool emb_radix_pass(const EmbGradArgs& E, int pass, uint32_t& target,
         __syncthreads();
     }
     if (E.parts == 1) {  // the block's own counts are the totals
-        if (sorting) {
-            const uint32_t v = threadIdx.x < bins ? S.base[threadIdx.x] : 0;
-            const uint32_t x = emb_block_scan(v, S.scan);
-            if (threadIdx.x < bins) S.base[threadIdx.x] = x;
-            __syncthreads();
-        }
+        const uint32_t v = threadIdx.x < bins ? S.base[threadIdx.x] : 0;
+        const uint32_t x = emb_block_scan(v, S.scan);
+        if (threadIdx.x < bins) S.base[threadIdx.x] = x;
+        __syncthreads();
     } else {
-        if (sorting)
-            for (int b = threadIdx.x; b < bins; b += EMB_THREADS) E.counts[(int64_t)b * E.parts + blockIdx.x] = S.base[b];
-        if (!emb_grid_sync(E, target)) return false;
-        for (int b = blockIdx.x * EMB_WARPS + warp; b < bins; b += gridDim.x * EMB_WARPS) {
+        for (int b = threadIdx.x; b < bins; b += EMB_THREADS) E.counts[(int64_t)b * E.parts + blockIdx.x] = S.base[b];
+        if (!emb_sync(E, 1, E.parts, target)) return false;
+        for (int b = blockIdx.x * EMB_WARPS + warp; b < bins; b += E.parts * EMB_WARPS) {
             uint32_t run = 0;
             for (int p0 = 0; p0 < E.parts; p0 += 32) {
                 const int p = p0 + lane;
@@ -341,15 +337,13 @@ __device__ bool emb_radix_pass(const EmbGradArgs& E, int pass, uint32_t& target,
             }
             if (lane == 0) E.totals[b] = run;
         }
-        if (!emb_grid_sync(E, target)) return false;
-        if (sorting) {
-            const uint32_t v = threadIdx.x < bins ? __ldcg(E.totals + threadIdx.x) : 0;
-            const uint32_t x = emb_block_scan(v, S.scan);
-            if (threadIdx.x < bins) S.base[threadIdx.x] = x + __ldcg(E.counts + (int64_t)threadIdx.x * E.parts + blockIdx.x);
-            __syncthreads();
-        }
+        if (!emb_sync(E, 1, E.parts, target)) return false;
+        const uint32_t v = threadIdx.x < bins ? __ldcg(E.totals + threadIdx.x) : 0;
+        const uint32_t x = emb_block_scan(v, S.scan);
+        if (threadIdx.x < bins) S.base[threadIdx.x] = x + __ldcg(E.counts + (int64_t)threadIdx.x * E.parts + blockIdx.x);
+        __syncthreads();
     }
-    if (sorting) {
+    {
         uint32_t* dst_key = E.key[pass & 1];
         int32_t* dst_pos = E.pos[pass & 1];
         const int64_t tile = (int64_t)EMB_THREADS * E.kpt;
@@ -406,7 +400,7 @@ __device__ bool emb_radix_pass(const EmbGradArgs& E, int pass, uint32_t& target,
             __syncthreads();
         }
     }
-    return emb_grid_sync(E, target);
+    return pass + 1 == E.passes || emb_sync(E, 1, E.parts, target);
 }
 
 __device__ __forceinline__ int64_t emb_lower_bound(const uint32_t* key, int64_t n, uint32_t v) {
@@ -458,18 +452,23 @@ __device__ __forceinline__ uint32_t emb_last_key(const EmbGradArgs& E, const uin
     return __ldcg(key + (end < E.tokens ? end : E.tokens) - 1);
 }
 
-// parts of the run that starts in `share` and goes on past its end; 0 where there is none
-__device__ __forceinline__ int64_t emb_run_parts(const EmbGradArgs& E, const uint32_t* key, int64_t share) {
+// parts of the run that starts in `share` and goes on past its end; 0 where there is none.  The lanes of a
+// worker (in step) look at the first keys of as many shares after it at once.
+__device__ __forceinline__ int64_t emb_run_parts(const EmbGradArgs& E, const uint32_t* key, int64_t share, int lane, int lanes,
+                                                 uint32_t group_mask) {
     const int64_t begin = share * E.share, end = begin + E.share;
     if (end >= E.tokens) return 0;
     const uint32_t run = __ldcg(key + end - 1), next = __ldcg(key + end);
     const uint32_t before = begin > 0 ? __ldcg(key + begin - 1) : 0xffffffffu;
     if (run >= (uint32_t)E.rows || next != run || before == run) return 0;
-    // its last share: few steps when it ends in the next one, as most do
-    int64_t last = share + 1;
-    if (end + E.share < E.tokens && __ldcg(key + end + E.share) == run)
-        last = (emb_lower_bound(key, E.tokens, run + 1u) - 1) / E.share;
-    return last - share + 1;
+    int64_t parts = 1;
+    while (true) {
+        const int64_t at = (share + parts + lane) * E.share;
+        const uint32_t on = __ballot_sync(group_mask, at < E.tokens && __ldcg(key + at) == run) & group_mask;
+        const int more = __popc(on);  // sorted keys: the shares that the run reaches come first
+        parts += more;
+        if (more < lanes) return parts;
+    }
 }
 
 // parts [i0, i1) of the run that starts in `share`: part 0 is that share's tail, part i the head of the
@@ -511,15 +510,25 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbG
     const int lane32 = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * EMB_WARPS;
     const int64_t gwarp = (int64_t)blockIdx.x * EMB_WARPS + (threadIdx.x >> 5);
-    uint32_t target = 0;
+    uint32_t target = 0, sort_target = 0;
 
     if (E.zero_first && !(E.parts < (int)gridDim.x && (int)blockIdx.x < E.parts)) {
         // the blocks that do not sort zero the table meanwhile (all of them where every block sorts)
-        const int64_t skip = E.parts < (int)gridDim.x ? (int64_t)E.parts * EMB_WARPS : 0;
-        for (int64_t r = gwarp - skip; r < E.rows; r += warps - skip) emb_zero_row<VEC>(E, r, lane32, 32);
+        const int64_t skip = E.parts < (int)gridDim.x ? E.parts : 0, blocks = gridDim.x - skip, block = blockIdx.x - skip;
+        const int64_t bytes = E.rows * E.width * (E.out_type == EMB_F32 ? 4 : 2);
+        if ((E.ldo == E.width || E.rows == 1) && ((uintptr_t)E.out & 15) == 0) {
+            uint4* out = static_cast<uint4*>(E.out);
+#pragma unroll 8
+            for (int64_t i = block * EMB_THREADS + threadIdx.x; i < bytes / 16; i += blocks * EMB_THREADS) out[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (block == 0 && threadIdx.x < bytes % 16) static_cast<unsigned char*>(E.out)[bytes / 16 * 16 + threadIdx.x] = 0;
+        } else {
+            for (int64_t r = block * EMB_WARPS + (threadIdx.x >> 5); r < E.rows; r += blocks * EMB_WARPS) emb_zero_row<VEC>(E, r, lane32, 32);
+        }
     }
-    for (int pass = 0; pass < E.passes; ++pass)
-        if (!emb_radix_pass(E, pass, target, S)) return;
+    if ((int)blockIdx.x < E.parts)
+        for (int pass = 0; pass < E.passes; ++pass)
+            if (!emb_radix_pass(E, pass, sort_target, S)) return;
+    if (!emb_sync(E, 0, gridDim.x, target)) return;
     const uint32_t* key = E.key[(E.passes & 1) ^ 1];
     const int32_t* pos = E.pos[(E.passes & 1) ^ 1];
     const uint32_t rows = (uint32_t)E.rows;
@@ -619,7 +628,7 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbG
         }
     }
     if (E.shares <= 1) return;
-    if (!emb_grid_sync(E, target)) return;
+    if (!emb_sync(E, 0, gridDim.x, target)) return;
 
     // ------------------------------------------------ runs that cross shares
     // The worker of the share where such a run starts adds its parts in order; a run of more than
@@ -633,7 +642,7 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbG
         __syncthreads();
         int64_t count = 0;
         if (task0 + group < tasks) {
-            count = emb_run_parts(E, key, (task0 + group) % E.shares);
+            count = emb_run_parts(E, key, (task0 + group) % E.shares, lane, lanes, group_mask);
             if (count > EMB_SERIAL_PARTS && lane == 0) long_task[atomicAdd(&long_count, 1)] = task0 + group;
         }
         if (count > 0 && count <= EMB_SERIAL_PARTS) {
@@ -649,7 +658,7 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbG
         for (int i = 0; i < long_count; ++i) {
             const int64_t share = long_task[i] % E.shares;
             const int64_t c = (long_task[i] / E.shares) * ((int64_t)lanes * VEC) + (int64_t)lane * VEC;
-            const int64_t parts = emb_run_parts(E, key, share);
+            const int64_t parts = emb_run_parts(E, key, share, lane, lanes, group_mask);
             const int64_t each = (parts + groups - 1) / groups;
             const int64_t i0 = (int64_t)group * each;
             float sum[VEC];
@@ -775,7 +784,7 @@ constexpr int EMB_TABLE_ROWS = 52;           // at most: four warps' tables of 1
 
 // grid (blocks, column tiles); E.parts warps a block; tables [warp][row][32 lanes x VEC]
 template <typename T, int VEC>
-__global__ void __launch_bounds__(EMB_THREADS) embedding_backward_table_kernel(EmbGradArgs E) {
+__global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_table_kernel(EmbGradArgs E) {
     extern __shared__ __align__(16) float emb_tables[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = E.parts;
     const int rows = (int)E.rows;
@@ -933,7 +942,7 @@ static void emb_plan(int64_t tokens, int64_t rows, int64_t width, int vec, int g
     }
     // zeroing beside the sort is free up to what the device writes in its time; every row twice costs more
     // than looking for the absent ones only in a large table that most tokens' rows fill
-    E.zero_first = !E.accumulate && (tokens <= rows || rows * width * 4 <= (192ll << 20));
+    E.zero_first = !E.accumulate && (tokens <= rows || rows * width * 4 <= (256ll << 20));
     int64_t want = (E.shares * E.tiles + per_block - 1) / per_block;
     if (want < E.parts) want = E.parts;
     if (!E.accumulate) {  // blocks for the zeroed rows: 64 KB each
@@ -959,7 +968,7 @@ static EmbLayout emb_layout(int64_t tokens, int64_t width, int grid_max) {
     const int64_t by_tokens = (tokens + EMB_MIN_SHARE - 1) / EMB_MIN_SHARE * width;
     const int64_t by_threads = (int64_t)grid_max * EMB_THREADS * 8 + 2 * width;
     const int64_t sums = (by_tokens < by_threads ? by_tokens : by_threads) * 2;
-    // a table of sums per block, grid_max / (column tiles of at least 32 columns) blocks or one
+    // a table of sums per block, grid_max / (column tiles of at most 128 columns) blocks or one
     const int64_t tables = EMB_TABLE_ROWS * ((int64_t)grid_max * 128 + width);
     L.parts = at, at += up((sums > tables ? sums : tables) * 4);
     L.bytes = at;
@@ -1098,7 +1107,7 @@ int pbg_embedding_backward(int64_t tokens, int64_t rows, int64_t width, const vo
         kernel<<<1, EMB_THREADS, 0, s>>>(E);
         return launch_status("embedding_backward");
     }
-    int rc = cuda_status(cudaMemsetAsync(E.barrier, 0, 4, s), "embedding_backward: barrier");
+    int rc = cuda_status(cudaMemsetAsync(E.barrier, 0, 8, s), "embedding_backward: barrier");
     if (rc) return rc;
     void* args[] = {&E};
     return cuda_status(cudaLaunchCooperativeKernel((const void*)kernel, dim3((unsigned)grid), dim3(EMB_THREADS), args, 0, s),
