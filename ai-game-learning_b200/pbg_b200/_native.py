@@ -8,6 +8,7 @@ CUDA tensor, the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -197,6 +198,27 @@ def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().pbg_last_error().decode(errors="replace")
         raise NativeError(f"{what} failed ({rc}): {msg}")
+
+
+@functools.cache
+def entry(name: str):
+    """An entry point as a function that raises on failure, for callers whose calls are short: arguments are
+    plain integers and floats, and the tensors behind the addresses stay referenced by the caller."""
+
+    fn = getattr(lib(), name)
+
+    def run(*args) -> None:
+        rc = fn(*args)
+        if rc:
+            check(rc, name)
+
+    return run
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of a device, as an address."""
+
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 _keep = threading.local()

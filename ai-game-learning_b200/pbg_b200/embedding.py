@@ -19,8 +19,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
-from . import _native as N
-from ._native import NativeError, call, stream
+from ._native import NativeError, entry, lib, raw_stream
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ERROR: dict[int, Tensor] = {}
@@ -48,7 +47,7 @@ def index_error(device=None) -> int:
 def _rows_matrix(t: Tensor, width: int) -> Tensor:
     """t [..., width] as a matrix of rows with contiguous columns, without a copy where its strides allow."""
 
-    m = t[None] if t.ndim == 1 else t.flatten(0, -2)
+    m = t if t.ndim == 2 else t[None] if t.ndim == 1 else t.flatten(0, -2)
     if m.numel() and ((width > 1 and m.stride(1) != 1) or (m.shape[0] > 1 and m.stride(0) < width)):
         m = m.contiguous()
     return m
@@ -88,7 +87,7 @@ def embedding(table: Tensor, index: Tensor, scale: float = 1.0, *, out_dtype: to
         raise NativeError("embedding: out must be contiguous [*index.shape, width] of the output type, on the table's device")
     if out.dtype not in TYPES:
         raise NativeError("embedding: the output must be float32, bfloat16 or float16")
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _forward(table, index, scale, out, rows, width)
     return _forward(table, index, scale, out, rows, width)
@@ -96,9 +95,9 @@ def embedding(table: Tensor, index: Tensor, scale: float = 1.0, *, out_dtype: to
 
 def _forward(table, index, scale, out, rows, width):
     device = table.device
-    call("pbg_embedding", index.numel(), rows, width, index.data_ptr(), int(index.dtype == torch.int64), table.data_ptr(),
-         TYPES[table.dtype], _stride(table), float(scale), out.data_ptr(), TYPES[out.dtype],
-         _error_word(device).data_ptr(), stream(device))
+    entry("pbg_embedding")(index.numel(), rows, width, index.data_ptr(), int(index.dtype == torch.int64), table.data_ptr(),
+                           TYPES[table.dtype], _stride(table), float(scale), out.data_ptr(), TYPES[out.dtype],
+                           _error_word(device).data_ptr(), raw_stream(device.index))
     return out
 
 
@@ -139,7 +138,7 @@ def embedding_backward(grad: Tensor, index: Tensor, rows: int, scale: float = 1.
     if out.dtype not in TYPES:
         raise NativeError("embedding_backward: the output must be float32, bfloat16 or float16")
     grad = _rows_matrix(grad, width)
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _backward(grad, index, rows, width, scale, padding_index, out, accumulate)
     return _backward(grad, index, rows, width, scale, padding_index, out, accumulate)
@@ -148,11 +147,12 @@ def embedding_backward(grad: Tensor, index: Tensor, rows: int, scale: float = 1.
 def _backward(grad, index, rows, width, scale, padding_index, out, accumulate):
     device = grad.device
     tokens = index.numel()
-    size = int(N.lib().pbg_embedding_backward_workspace(tokens, width))
+    size = lib().pbg_embedding_backward_workspace(tokens, width)
     workspace = torch.empty(size, dtype=torch.uint8, device=device)
-    call("pbg_embedding_backward", tokens, rows, width, grad.data_ptr(), TYPES[grad.dtype], _stride(grad),
-         index.data_ptr(), int(index.dtype == torch.int64), padding_index, float(scale), out.data_ptr(), TYPES[out.dtype],
-         _stride(out), int(bool(accumulate)), workspace.data_ptr(), size, _error_word(device).data_ptr(), stream(device))
+    entry("pbg_embedding_backward")(tokens, rows, width, grad.data_ptr(), TYPES[grad.dtype], _stride(grad),
+                                    index.data_ptr(), int(index.dtype == torch.int64), padding_index, float(scale),
+                                    out.data_ptr(), TYPES[out.dtype], _stride(out), int(bool(accumulate)),
+                                    workspace.data_ptr(), size, _error_word(device).data_ptr(), raw_stream(device.index))
     return out
 
 

@@ -19,7 +19,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
-from ._native import NativeError, call, lib, ptr, stream
+from ._native import NativeError, call, entry, lib, ptr, raw_stream, stream
 
 CONTROL_NAMES = ("lr", "beta1", "beta2", "epsilon", "decay", "clip", "scale", "growth", "backoff", "interval")
 
@@ -98,7 +98,7 @@ def orthogonalize(x: Tensor, *, steps: int = 5, coefficients: tuple[float, float
     if out.dtype not in _TYPES:
         raise NativeError("orthogonalize: the output must be float32, bfloat16 or float16")
     x = x.contiguous()
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return _orthogonalize(x, steps, coefficients, epsilon, out)
     return _orthogonalize(x, steps, coefficients, epsilon, out)
@@ -111,9 +111,9 @@ def _orthogonalize(x, steps, coefficients, epsilon, out):
     size = int(lib().pbg_orthogonalize_workspace(batch, rows, cols))
     workspace = torch.empty(max(size, 1), dtype=torch.uint8, device=device)
     a, b, c = coefficients
-    call("pbg_orthogonalize", batch, rows, cols, x.data_ptr(), _TYPES[x.dtype], out.data_ptr(), _TYPES[out.dtype],
-         int(steps), float(a), float(b), float(c), float(epsilon), workspace.data_ptr(), size,
-         _error_word(device).data_ptr(), stream(device))
+    entry("pbg_orthogonalize")(batch, rows, cols, x.data_ptr(), _TYPES[x.dtype], out.data_ptr(), _TYPES[out.dtype],
+                               int(steps), float(a), float(b), float(c), float(epsilon), workspace.data_ptr(), size,
+                               _error_word(device).data_ptr(), raw_stream(device.index))
     return out
 
 
@@ -188,17 +188,18 @@ class FlatMuon:
         """Apply one transition from ``self.grad``; returns the device's ``skipped`` word (int32 [1])."""
 
         dev = self.master.device
-        if dev.index != torch.cuda.current_device():
+        if dev.index != torch._C._cuda_getDevice():
             with torch.cuda.device(dev):
                 return self._step(dev)
         return self._step(dev)
 
     def _step(self, dev) -> Tensor:
         a, b, c = self.coefficients
-        call("pbg_muon_step", len(self.matrices), self._descriptors.data_ptr(), self._plan.ctypes.data, self.grad.data_ptr(),
-             self.momentum.data_ptr(), self.master.data_ptr(), self.controls.data_ptr(), int(self.nesterov), self.steps,
-             float(a), float(b), float(c), self.epsilon, self._workspace.data_ptr(), self._workspace.numel(),
-             self.skipped.data_ptr(), _error_word(dev).data_ptr(), stream(dev))
+        entry("pbg_muon_step")(len(self.matrices), self._descriptors.data_ptr(), self._plan.ctypes.data,
+                               self.grad.data_ptr(), self.momentum.data_ptr(), self.master.data_ptr(),
+                               self.controls.data_ptr(), int(self.nesterov), self.steps, float(a), float(b), float(c),
+                               self.epsilon, self._workspace.data_ptr(), self._workspace.numel(),
+                               self.skipped.data_ptr(), _error_word(dev).data_ptr(), raw_stream(dev.index))
         return self.skipped
 
 
