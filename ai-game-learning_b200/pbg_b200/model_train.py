@@ -256,19 +256,28 @@ class FlatParameters:
     """Named parameters as leaf views of one flat fp32 master (in the given order); ``attach`` makes each
     leaf's ``.grad`` a view of one flat gradient buffer, so autograd accumulates the gradient in place
     there (shared parameters used by several forwards add up) and the optimizer and the gradient SUM
-    see one flat vector."""
+    see one flat vector.  With ``first(name, shape)`` the parameters that it holds for come first and
+    the others from ``split`` on, the next multiple of four elements (what lies between stays 0)."""
 
-    def __init__(self, params: dict, device) -> None:
+    def __init__(self, params: dict, device, first=None) -> None:
         dev = torch.device(device)
         self.names = list(params)
         self.shapes = {n: tuple(params[n].shape) for n in self.names}
+        self.split = leading = 0
+        if first is not None:
+            chosen = [n for n in self.names if first(n, self.shapes[n])]
+            self.names = chosen + [n for n in self.names if n not in set(chosen)]
+            leading = len(chosen)
+            self.split = -(-sum(math.prod(self.shapes[n]) for n in chosen) // 4) * 4
         self.offsets: dict[str, int] = {}
         total = 0
-        for n in self.names:
+        for i, n in enumerate(self.names):
+            if i == leading:
+                total = self.split
             self.offsets[n] = total
             total += math.prod(self.shapes[n])
         self.numel = total
-        self.master = torch.empty(total, dtype=torch.float32, device=dev)
+        self.master = torch.zeros(total, dtype=torch.float32, device=dev)
         self.leaves: dict[str, Tensor] = {}
         for n in self.names:
             view = self.view(self.master, n)
@@ -292,33 +301,56 @@ class FlatParameters:
 _FIELDS = ("type_logits", "omega", "mu", "s", "iota")
 
 
+def is_hidden_matrix(name: str, shape: tuple) -> bool:
+    """Whether a parameter is one that an orthogonalised update suits: a weight matrix of a map with more
+    than one row and column; not a table (embeddings, tokens), a vector or a scalar's affine map."""
+
+    return len(shape) == 2 and min(shape) > 1 and name.endswith(".weight") and "embedding" not in name
+
+
 class ModelLearnerStep:
     """The learner step over one batch per input family (pbg/core/training.py:336-424 with the queued
     model operation, pbg/games/poker/queued/model.py:403-415): for each batch the model's learner rows
     (the owner's sampled private row), the fused poker objective, and the backward of the objective's
-    gradient through the network into the flat gradient; then one AdamW transition of the flat master.
+    gradient through the network into the flat gradient; then one AdamW transition of the flat master
+    (or Muon's of its matrices and AdamW's of the rest).
 
     A batch is a dict with ``input_type``, ``model_input`` [S, F], ``sampled_private_state`` [S, P],
     ``owner`` [S], and the objective's ``mask``, ``action``, ``old_log_policy``, ``advantage_target``,
-    ``old_value``, ``value_target``, ``controls`` and ``lane_weight``."""
+    ``old_value``, ``value_target``, ``controls`` and ``lane_weight``.
+
+    ``muon``: options of ``FlatMuon`` (a dict, may be empty): the hidden matrices (``is_hidden_matrix``)
+    then take its transition and AdamW keeps the tables, vectors and head rows; ``grad`` is the whole
+    flat gradient either way.  Each transition guards its own part against gradients that are not finite.
+    ``sorted_embeddings``: the tables' gradients by sorted tokens instead of one-hot products."""
 
     def __init__(self, model, *, lr: float = 3e-4, beta1: float = 0.9, beta2: float = 0.999, epsilon: float = 1e-8,
-                 weight_decay: float = 0.0, grad_clip: float = 1.0) -> None:
+                 weight_decay: float = 0.0, grad_clip: float = 1.0, muon: dict | None = None,
+                 sorted_embeddings: bool = False) -> None:
         from .learner import PokerLearnerObjective
-        from .optim import FlatAdam
+        from .optim import FlatAdam, FlatMuon
 
         self.model = model
-        self.flat = model.enable_training()
-        self.adam = FlatAdam(self.flat.master, lr=lr, beta1=beta1, beta2=beta2, epsilon=epsilon, decay=weight_decay,
-                             clip=grad_clip)
-        self.flat.attach(self.adam.grad)
+        self.muon = None
+        options = dict(lr=lr, beta1=beta1, beta2=beta2, epsilon=epsilon, decay=weight_decay, clip=grad_clip)
+        if muon is None:
+            self.flat = flat = model.enable_training(sorted_embeddings=sorted_embeddings)
+            self.adam = FlatAdam(flat.master, **options)
+            self.grad = self.adam.grad
+        else:
+            self.flat = flat = model.enable_training(sorted_embeddings=sorted_embeddings, first=is_hidden_matrix)
+            self.grad = torch.zeros_like(flat.master)
+            matrices = [(flat.offsets[n], *flat.shapes[n]) for n in flat.names if is_hidden_matrix(n, flat.shapes[n])]
+            self.muon = FlatMuon(flat.master, matrices, grad=self.grad, **muon)
+            self.adam = FlatAdam(flat.master[flat.split:], grad=self.grad[flat.split:], **options)
+        self.flat.attach(self.grad)
         self.objective = PokerLearnerObjective(self.flat.master.device)
 
     def gradient(self, batches: list) -> list:
-        """Forward, objective and backward of every batch; the flat gradient lands in ``self.adam.grad``,
+        """Forward, objective and backward of every batch; the flat gradient lands in ``self.grad``,
         cleared first (the AdamW transition leaves the clipped gradient there, and autograd adds into it)."""
 
-        self.adam.grad.zero_()
+        self.grad.zero_()
         results = []
         for b in batches:
             evaluation = self.model.learner_operation(b["input_type"], b["model_input"], b["sampled_private_state"],
@@ -333,5 +365,7 @@ class ModelLearnerStep:
 
     def __call__(self, batches: list) -> list:
         results = self.gradient(batches)
+        if self.muon is not None:
+            self.muon.step()
         self.adam.step()
         return results

@@ -26,13 +26,16 @@ CONTROL_NAMES = ("lr", "beta1", "beta2", "epsilon", "decay", "clip", "scale", "g
 
 class FlatAdam:
     def __init__(self, master: Tensor, *, lr=1e-3, beta1=0.9, beta2=0.999, epsilon=1e-8, decay=0.0, clip=1.0,
-                 scale=1.0, decoupled=True) -> None:
+                 scale=1.0, decoupled=True, grad: Tensor | None = None) -> None:
         if master.dtype != torch.float32 or master.ndim != 1 or not master.is_cuda:
             raise ValueError("flat masters must be CUDA fp32 [N]")
         self.master = master
         n = master.numel()
         dev = master.device
-        self.grad = torch.zeros(n, dtype=torch.float32, device=dev)
+        if grad is not None and (grad.shape != master.shape or grad.dtype != torch.float32 or grad.device != dev
+                                 or not grad.is_contiguous()):
+            raise ValueError("the flat gradient must be like the master")
+        self.grad = torch.zeros(n, dtype=torch.float32, device=dev) if grad is None else grad
         self.first = torch.zeros(n, dtype=torch.float32, device=dev)
         self.second = torch.zeros(n, dtype=torch.float32, device=dev)
         self.controls = torch.tensor([lr, beta1, beta2, epsilon, decay, clip, scale, 2.0, 0.5, 2000.0],

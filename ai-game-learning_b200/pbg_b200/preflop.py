@@ -16,7 +16,9 @@ them) and the small elementwise steps are torch operations on the device.
 In training mode (``FamilyModel.train()``, after ``bind_parameters`` with leaf
 tensors) the same forward runs with every native step as an autograd function
 of ``pbg_b200.model_train`` (the learner step's backward); embedding rows are
-then one-hot products (``lookup``) so that their gradients are GEMMs.
+then one-hot products (``lookup``) so that their gradients are GEMMs, or with
+sorted embeddings looked up by ``embedding_train``, whose gradient sums the
+tokens' rows after sorting them by index.
 """
 
 from __future__ import annotations
@@ -30,7 +32,8 @@ from torch.nn import functional as F
 
 from ._native import NativeError, call, ptr, rows_ptr, stream
 from .model import attention, linear, linear_ex
-from .model_train import attention_train, incidence_combine_train, layernorm_train, linear_train, q_scale_of
+from .model_train import (attention_train, embedding_train, incidence_combine_train, layernorm_train, linear_train,
+                          q_scale_of)
 
 
 @dataclass(frozen=True)
@@ -96,10 +99,12 @@ class PolicyOutput:
 
 
 class _Binding:
-    """Mode shared by a model's maps: ``training`` routes every map through its autograd function."""
+    """Mode shared by a model's maps: ``training`` routes every map through its autograd function,
+    ``sorted_embeddings`` every table's lookup through the one whose gradient sums sorted tokens."""
 
     def __init__(self) -> None:
         self.training = False
+        self.sorted_embeddings = False
 
 
 class _Map:
@@ -325,6 +330,13 @@ class FamilyModel:
         if not mode:
             self.sync_weights()
         return self
+
+    def _lookup(self, table: Tensor, index: Tensor) -> Tensor:
+        """Rows of a table: ``lookup``, or while training with sorted embeddings ``embedding_train``."""
+
+        if self.binding.sorted_embeddings and table.requires_grad and torch.is_grad_enabled():
+            return embedding_train(table, index)
+        return lookup(table, index)
 
     # ------------------------------------------------------------ kernels
     def _ln(self, x: Tensor, gain_bias, out: Tensor | None = None) -> Tensor:
@@ -593,8 +605,8 @@ class PreflopModel(FamilyModel):
         scalars = torch.cat(groups, 1)
         type_ids = torch.cat([torch.full((n,), k, dtype=torch.long, device=dev) for n, k in kinds])
         w = p["public_scalar_affine.weight"][:, 0]
-        token = scalars[..., None] * w + p["public_scalar_affine.bias"] + lookup(p["public_type_embedding.weight"], type_ids)
-        seat_pos = lookup(p["seat_embedding.weight"], relative_seats)
+        token = scalars[..., None] * w + p["public_scalar_affine.bias"] + self._lookup(p["public_type_embedding.weight"], type_ids)
+        seat_pos = self._lookup(p["seat_embedding.weight"], relative_seats)
         rest = scalars.shape[1] - 1 - 2 * players
         zeros = lambda n: torch.zeros((batch, n, self.cfg.d_model), device=dev)  # noqa: E731
         token = token + torch.cat((zeros(1), seat_pos, seat_pos, zeros(rest)), 1)
@@ -605,11 +617,11 @@ class PreflopModel(FamilyModel):
             numeric = torch.stack([h[k].float() for k in ("amount", "pot_before", "call_amount", "current_bet",
                                                           "min_raise_to", "max_raise_to")], -1)
             ht = numeric @ p["history_numeric_affine.weight"].T + p["history_numeric_affine.bias"]
-            ht = ht + lookup(p["history_action_embedding.weight"], h["action"].clamp(0, 3).long())
-            ht = ht + lookup(p["history_street_embedding.weight"], h["street"].clamp(0, 3).long())
+            ht = ht + self._lookup(p["history_action_embedding.weight"], h["action"].clamp(0, 3).long())
+            ht = ht + self._lookup(p["history_street_embedding.weight"], h["street"].clamp(0, 3).long())
             ht = ht + p["history_position_embedding.weight"][: h["mask"].shape[1]][None]
             actor = h["actor"].clamp(0, players - 1).long()
-            ht = ht + lookup(p["seat_embedding.weight"], relative_seats.gather(1, actor)) * (h["actor"] >= 0)[..., None]
+            ht = ht + self._lookup(p["seat_embedding.weight"], relative_seats.gather(1, actor)) * (h["actor"] >= 0)[..., None]
             token = torch.cat((token, ht), 1)
             valid = torch.cat((valid, h["mask"].bool()), 1)
         mean = (token * valid[..., None]).sum(1) / valid.sum(1, keepdim=True)
@@ -653,13 +665,13 @@ class PreflopModel(FamilyModel):
                                  expanded_geometry, torch.ones_like(ranges)[..., None]), -1)
         actor_flag = (torch.arange(players, device=dev)[None] == actor[:, None]).long()
         # each seat's seat, status and actor embeddings, added to its K class rows in the map's epilogue
-        seat_terms = (lookup(p["seat_embedding.weight"], relative) + lookup(p["status_embedding.weight"], status)
-                      + lookup(p["actor_embedding.weight"], actor_flag))
+        seat_terms = (self._lookup(p["seat_embedding.weight"], relative) + self._lookup(p["status_embedding.weight"], status)
+                      + self._lookup(p["actor_embedding.weight"], actor_flag))
         row = _affine_rows(self.class_row_affine, row_feature, seat_terms, K)
         row_flat = row.reshape(batch, players * K, d)
         public_token, public_mask = self._public_tokens(pub, seat_mask, relative)
         actor_relative = relative.gather(1, actor[:, None]).squeeze(1)
-        anchors = p["anchor_tokens"][None] + lookup(p["anchor_seat_embedding.weight"], actor_relative)[:, None]
+        anchors = p["anchor_tokens"][None] + self._lookup(p["anchor_seat_embedding.weight"], actor_relative)[:, None]
         x = torch.cat((row_flat, public_token, anchors), 1)
         length = x.shape[1]
         key_mask = torch.cat((cmask.reshape(batch, players * K), public_mask,

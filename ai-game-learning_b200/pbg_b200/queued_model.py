@@ -96,10 +96,14 @@ class QueuedPokerModel:
             torch.arange(geometry.private_hands, dtype=torch.int32, device=self.device)).to(torch.int64)
 
     # ------------------------------------------------------------ training
-    def enable_training(self):
+    def enable_training(self, *, sorted_embeddings: bool = False, first=None):
         """Put both partition networks in training mode over ONE set of parameters: every parameter
         (``shared.*``, ``pre_encoder.*``, ``post_encoder.*``) a leaf view of one flat fp32 master, the
-        shared ones the same leaves in both networks.  Returns the ``FlatParameters``."""
+        shared ones the same leaves in both networks.  Returns the ``FlatParameters``.
+
+        ``sorted_embeddings``: the tables' gradients by sorted tokens instead of one-hot products.
+        ``first(name, shape)``: the parameters that it holds for come first in the flat master, the
+        others from the next multiple of four elements on."""
 
         from .model_train import FlatParameters
 
@@ -108,9 +112,10 @@ class QueuedPokerModel:
 
         params = {full("pre_encoder.", n): v for n, v in self.pre.p.items()}
         params.update({full("post_encoder.", n): v for n, v in self.post.p.items()})
-        flat = FlatParameters(params, self.device)
+        flat = FlatParameters(params, self.device, first=first)
         self.pre.bind_parameters({n: flat.leaves[full("pre_encoder.", n)] for n in self.pre.p})
         self.post.bind_parameters({n: flat.leaves[full("post_encoder.", n)] for n in self.post.p})
+        self.pre.binding.sorted_embeddings = self.post.binding.sorted_embeddings = bool(sorted_embeddings)
         self.pre.train()
         self.post.train()
         return flat
