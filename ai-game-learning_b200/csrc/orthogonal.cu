@@ -66,9 +66,12 @@ struct OrthoDesc {
     int64_t ws;      // bytes of workspace before this matrix's tiles: X, X', A, B
     int64_t span0;   // spans, conversion tiles, symmetric and update tiles of the matrices before it
     int64_t conv0, sym0, upd0;
+    int64_t gram0;   // its Gram matrix's items: tiles, each in `split` parts of its sum
+    int64_t part0;   // items of the matrices before it whose sums are split
     int64_t slot0;   // blocks of the teams before it (short sides up to 128)
     int32_t m, n;    // short and long side
     int32_t team;    // blocks that work on it, where its short side is at most 128; else 0
+    int32_t split;   // parts of the Gram matrix's sums
     int32_t tall;    // stored n x m
     float adjust;
 };
@@ -76,8 +79,8 @@ struct OrthoDesc {
 struct OrthoArgs {
     const OrthoDesc* list;  // device, or null: `count` matrices like `one`, `one`'s sizes apart
     OrthoDesc one;
-    int64_t one_src, one_ws, one_span, one_conv, one_sym, one_upd;
-    int64_t count, spans, convs, syms, upds, slots;  // totals
+    int64_t one_src, one_ws, one_span, one_conv, one_sym, one_upd, one_gram;
+    int64_t count, spans, convs, grams, syms, upds, slots;  // totals
     int bn_sym, bn_upd;  // output tile widths
     int pair;            // output tiles of 256 rows, by two blocks each
     int mirror;          // of A and B only what is on and above the diagonal is computed
@@ -99,6 +102,8 @@ struct OrthoArgs {
     // workspace
     double* sums;
     unsigned char* tiles;
+    float* parts;           // of split sums: [item][row quarter][64 columns][column][lane]
+    uint32_t* arrived;      // per item and epilogue warp, zero between uses
     uint32_t* barrier;
     uint32_t* error;
     int aligned;  // vector access to the flat buffers, x and out: 16 bytes at multiples of four elements
@@ -255,6 +260,7 @@ __device__ __forceinline__ OrthoDesc or_get(const OrthoArgs& O, int64_t i) {
     d.conv0 = i * O.one_conv;
     d.sym0 = i * O.one_sym;
     d.upd0 = i * O.one_upd;
+    d.gram0 = d.part0 = i * O.one_gram;
     d.slot0 = i * d.team;
     return d;
 }
@@ -470,46 +476,60 @@ __global__ void __launch_bounds__(ORTHO_FLAT) orthogonalize_convert_kernel(const
 
 enum { OR_GRAM = 0, OR_SQUARE = 1, OR_UPDATE = 2 };
 
-// one output tile: its matrix, row block, first column and width
+// one output tile: its matrix, row block, first column and width; the k-blocks of its sum that this item
+// takes (`part` of `split`), and the first of its items among the split ones
 struct OrthoTile {
-    int which, i, c0, width;
+    int which, i, c0, width, k0, kblocks, part, split;
+    int64_t item;
 };
 
-// Tile t as one block (or the block of rank `rank` of a pair) sees it.  A pair's second row block may not
-// exist (i = or_mb(m)); its columns come by 128.
-template <bool PAIR>
+// Tile (of the Gram matrix: item) t as one block (or the block of rank `rank` of a pair) sees it.  A pair's
+// second row block may not exist (i = or_mb(m)); its columns come by 128.
+template <bool PAIR, bool SPLIT>
 __device__ __forceinline__ OrthoTile or_tile(const OrthoArgs& O, int kind, int64_t t, int rank) {
     OrthoTile T;
-    const bool sym = kind != OR_UPDATE;
-    const int64_t w = sym ? or_find(O, t, &OrthoDesc::sym0, O.one_sym) : or_find(O, t, &OrthoDesc::upd0, O.one_upd);
+    const bool gram = SPLIT && kind == OR_GRAM;
+    const int64_t w = gram                  ? or_find(O, t, &OrthoDesc::gram0, O.one_gram)
+                      : kind != OR_UPDATE ? or_find(O, t, &OrthoDesc::sym0, O.one_sym)
+                                          : or_find(O, t, &OrthoDesc::upd0, O.one_upd);
     T.which = (int)w;
-    const int64_t first = O.list ? (sym ? O.list[w].sym0 : O.list[w].upd0) : w * (sym ? O.one_sym : O.one_upd);
-    const int m = O.list ? O.list[w].m : O.one.m, n = O.list ? O.list[w].n : O.one.n;
-    int local = (int)(t - first), columns;
-    if (sym) {
+    const OrthoDesc* d = O.list ? O.list + w : &O.one;
+    const int64_t first = O.list ? (gram ? d->gram0 : kind != OR_UPDATE ? d->sym0 : d->upd0)
+                                 : w * (gram ? O.one_gram : kind != OR_UPDATE ? O.one_sym : O.one_upd);
+    const int m = d->m, n = d->n;
+    int local = (int)(t - first);
+    T.part = 0, T.split = 1, T.k0 = 0, T.item = 0;
+    if (gram && d->split > 1) {
+        T.split = d->split;
+        T.part = local % T.split;
+        local /= T.split;
+        T.item = (O.list ? d->part0 : first) + (int64_t)local * T.split;
+    }
+    if (kind != OR_UPDATE) {
         T.i = 0;
         for (int r; local >= (r = or_sym_row(m, T.i, O.bn_sym, PAIR, O.mirror)); ++T.i) local -= r;
         T.c0 = or_sym_first(T.i, PAIR, O.mirror) + local * O.bn_sym;
-        columns = or_b64(m) * 64 - T.c0;
-        T.width = min(O.bn_sym, columns);
+        T.width = min(O.bn_sym, or_b64(m) * 64 - T.c0);
     } else {
         const int across = (or_b64(n) * 64 + O.bn_upd - 1) / O.bn_upd;
         T.i = local / across;
         T.c0 = (local % across) * O.bn_upd;
-        columns = or_b64(n) * 64 - T.c0;
-        T.width = min(O.bn_upd, columns);
+        T.width = min(O.bn_upd, or_b64(n) * 64 - T.c0);
     }
     if (PAIR) {
         T.i = 2 * T.i + rank;
         T.width = (T.width + 127) & ~127;
     }
+    if (kind == OR_SQUARE && O.c == 0.0f) {
+        T.kblocks = T.width >> 6;  // no square: only the tile's own columns of A
+    } else {
+        T.kblocks = or_b64(kind == OR_GRAM ? n : m);
+        if (T.split > 1) {
+            T.k0 = (int)((int64_t)T.kblocks * T.part / T.split);
+            T.kblocks = (int)((int64_t)T.kblocks * (T.part + 1) / T.split) - T.k0;
+        }
+    }
     return T;
-}
-
-__device__ __forceinline__ int or_kblocks(const OrthoArgs& O, int kind, const OrthoTile& T) {
-    if (kind == OR_SQUARE && O.c == 0.0f) return T.width >> 6;  // no square: only the tile's own columns of A
-    if (O.list) return kind == OR_GRAM ? or_b64(O.list[T.which].n) : or_b64(O.list[T.which].m);
-    return kind == OR_GRAM ? or_b64(O.one.n) : or_b64(O.one.m);
 }
 
 // where a matrix's tiles lie at a step
@@ -776,18 +796,18 @@ __device__ __forceinline__ uint32_t or_buffers(const OrthoArgs& O) { return max(
 // A producer warp's elected lane, one phase.  A stage is copy 0, the row operand, and copies 1 .. 6, a 64-row
 // or 64-column piece of the other operand each, hi and lo; the producer warps take them in turn.  `pipe`:
 // parity of each stage's next use, a bit a stage, kept from phase to phase.
-template <bool PRECISE, bool PAIR>
+template <bool PRECISE, bool PAIR, bool SPLIT>
 __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int rank,
                                            int producer, uint32_t& pipe) {
-    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
     const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
     bool ok = true;
     int s = 0;
     uint32_t used = 0;
     for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
-        OrthoTile T = or_tile<PAIR>(O, kind, t, rank);
-        const int kblocks = or_kblocks(O, kind, T), pieces = T.width >> (PAIR ? 7 : 6);
+        OrthoTile T = or_tile<PAIR, SPLIT>(O, kind, t, rank);
+        const int kblocks = T.kblocks, pieces = T.width >> (PAIR ? 7 : 6);
         const OrthoDesc desc = or_get(O, T.which);
         const OrthoPlace L = or_place(O, desc, step);
         if (PAIR) T.i = min(T.i, or_mb(desc.m) - 1);  // the row block that is not there: any other, never stored
@@ -810,6 +830,7 @@ __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, u
                 if (kind == OR_UPDATE) src[q] = L.x + (int64_t)cb * ORTHO_TILE + part * 16384;  // 64 k-rows of column block cb
                 else src[q] = (kind == OR_GRAM ? L.x + (cb >> 1) * L.x_row : L.a + (cb >> 1) * L.a_row) + (cb & 1) * 8192 + part * 16384;
             }
+            if (SPLIT) src[q] += (int64_t)T.k0 * ORTHO_TILE;
             expect += bytes[q];
         }
         for (int kb = 0; kb < kblocks; ++kb) {
@@ -843,10 +864,10 @@ __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, u
 }
 
 // The issuing warp's elected lane (of a pair's first block), one phase.  `acc` counts accumulators used.
-template <bool PRECISE, bool PAIR>
+template <bool PRECISE, bool PAIR, bool SPLIT>
 __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, uint32_t& pipe,
                                          uint32_t& acc) {
-    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
     const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
     const uint32_t peer0 = or_smem(&S.peer[0]);
@@ -860,8 +881,8 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
     bool ok = true;
     int s = 0;
     for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
-        const OrthoTile T = or_tile<PAIR>(O, kind, t, 0);
-        const int kblocks = or_kblocks(O, kind, T);
+        const OrthoTile T = or_tile<PAIR, SPLIT>(O, kind, t, 0);
+        const int kblocks = T.kblocks;
         const uint32_t idesc = or_idesc<PAIR>(T.width, mn);
         const int eye0 = kind == OR_SQUARE ? T.c0 >> 6 : 1 << 30, eye1 = eye0 + (T.width >> 6);
         for (int k0 = 0; ok && k0 < kblocks; k0 += chunk, ++acc) {
@@ -930,14 +951,14 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
 // The same warp of a pair's second block: tells the first when a stage's copies have landed here.
 template <bool PRECISE>
 __device__ __forceinline__ void or_relay(const OrthoArgs& O, OrthoShared& S, int kind, uint32_t& pipe) {
-    constexpr bool PAIR = true;
-    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    constexpr bool PAIR = true, SPLIT = false;
+    const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
     const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), peer0 = or_smem(&S.peer[0]);
     bool ok = true;
     int s = 0;
     for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
-        const int kblocks = or_kblocks(O, kind, or_tile<PAIR>(O, kind, t, 1));
+        const int kblocks = or_tile<PAIR, SPLIT>(O, kind, t, 1).kblocks;
         for (int kb = 0; kb < kblocks; ++kb) {
             if (!or_wait(full0 + 8 * s, (pipe >> s) & 1u, &S.abort_flag)) {
                 ok = false;
@@ -954,13 +975,43 @@ __device__ __forceinline__ void or_relay(const OrthoArgs& O, OrthoShared& S, int
     }
 }
 
+// A part of a split sum (an epilogue warp's rows and columns): to the workspace, and, where it is the last of
+// its tile's parts to arrive, the sum of all parts in order, so that the result does not depend on who is last.
+__device__ __forceinline__ bool or_join(const OrthoArgs& O, const OrthoTile& T, int e, int quad, int group0, int groups, int lane,
+                                        float* v) {
+    const int64_t next = (int64_t)128 * O.bn_sym;  // between a tile's parts
+    float* first = O.parts + T.item * next + ((int64_t)quad * (O.bn_sym >> 6) + group0) * 2048 + lane;
+    float* mine = first + T.part * next;
+#pragma unroll
+    for (int j = 0; j < 128; ++j)
+        if (j < 64 * groups) __stcg(mine + j * 32, v[j]);
+    __threadfence();
+    __syncwarp();
+    uint32_t* arrived = O.arrived + T.item * ORTHO_EPI_WARPS + e;
+    uint32_t before = 0;
+    if (lane == 0) before = atomicAdd(arrived, 1u);
+    if (__shfl_sync(0xffffffffu, before, 0) != (uint32_t)T.split - 1u) return false;
+    __threadfence();
+    if (lane == 0) *arrived = 0u;
+#pragma unroll
+    for (int j = 0; j < 128; ++j)
+        if (j < 64 * groups) v[j] = __ldcg(first + j * 32);
+    for (int p = 1; p < T.split; ++p) {
+        const float* part = first + p * next;
+#pragma unroll
+        for (int j = 0; j < 128; ++j)
+            if (j < 64 * groups) v[j] += __ldcg(part + j * 32);
+    }
+    return true;
+}
+
 // An epilogue warp, one phase: a quarter of the rows, one or (tiles wider than 128) two groups of 64
 // columns of each tile.
-template <bool PRECISE, bool PAIR>
+template <bool PRECISE, bool PAIR, bool SPLIT>
 __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int rank, int e,
                                            uint32_t& acc) {
     const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, part = e >> 2;
-    const int64_t tiles = kind == OR_UPDATE ? O.upds : O.syms;
+    const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
     const int bn = kind == OR_UPDATE ? O.bn_upd : O.bn_sym;
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
     const int chunk = PRECISE && !(kind == OR_SQUARE && O.c == 0.0f) ? 1 : 1 << 20;
@@ -971,9 +1022,9 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
     const uint32_t taddr0 = S.tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(group0 * 64);
     bool ok = true;
     for (int64_t t = PAIR ? blockIdx.x >> 1 : blockIdx.x; ok && t < tiles; t += PAIR ? gridDim.x >> 1 : gridDim.x) {
-        const OrthoTile T = or_tile<PAIR>(O, kind, t, rank);
+        const OrthoTile T = or_tile<PAIR, SPLIT>(O, kind, t, rank);
         const int groups = min(bn > 128 ? 2 : 1, (T.width >> 6) - group0);
-        const int chunks = (or_kblocks(O, kind, T) - 1) / chunk + 1;
+        const int chunks = (T.kblocks - 1) / chunk + 1;
         float v[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) v[j] = 0.0f;
@@ -1002,6 +1053,8 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
         else m = O.one.m, n = O.one.n;
         const int row = T.i * 128 + quad * 32 + lane;
         const int last_cb = or_b64(kind == OR_UPDATE ? n : m);  // a pair's tile may reach past the matrix
+        // A split sum: every part to the workspace; the warp that comes last adds them in order and goes on
+        if (SPLIT && ok && T.split > 1 && groups > 0 && !or_join(O, T, e, quad, group0, groups, lane, v)) continue;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const int cb = (T.c0 >> 6) + group0 + g;
@@ -1023,7 +1076,7 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
 // matrices, each role running through the phases on its own.  PAIR: launched in clusters of two blocks, which
 // work on tiles of 256 rows together (a block's own row block, half of the columns' operand each, the first
 // block issuing), a third fewer bytes to fetch per product.
-template <bool PRECISE, bool PAIR>
+template <bool PRECISE, bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const __grid_constant__ OrthoArgs O) {
     // the first kilobyte holds the barriers; the ring after it starts on the 1024 bytes of a swizzle atom
     extern __shared__ __align__(1024) unsigned char or_raw[];
@@ -1088,20 +1141,20 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
         for (int p = 0; p < phases; ++p) {
             if (or_elect()) {
                 if (PAIR && rank) or_relay<PRECISE>(O, S, p % 3, pipe);
-                else or_issue<PRECISE, PAIR>(O, S, ring, p % 3, pipe, acc);
+                else or_issue<PRECISE, PAIR, SPLIT>(O, S, ring, p % 3, pipe, acc);
             }
             __syncwarp();
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     } else if (warp <= ORTHO_PRODUCERS) {
         for (int p = 0; p < phases; ++p) {
-            if (or_elect()) or_produce<PRECISE, PAIR>(O, S, ring, p % 3, p / 3, rank, warp - 1, pipe);
+            if (or_elect()) or_produce<PRECISE, PAIR, SPLIT>(O, S, ring, p % 3, p / 3, rank, warp - 1, pipe);
             __syncwarp();
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     } else {
         for (int p = 0; p < phases; ++p) {
-            or_collect<PRECISE, PAIR>(O, S, ring, p % 3, p / 3, rank, warp - 1 - ORTHO_PRODUCERS, acc);
+            or_collect<PRECISE, PAIR, SPLIT>(O, S, ring, p % 3, p / 3, rank, warp - 1 - ORTHO_PRODUCERS, acc);
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     }
@@ -1535,35 +1588,57 @@ static OrthoDesc or_make(int64_t rows, int64_t cols) {
 // 256 x 16,384, for tiles of 128 x 64, x 128, x 192 and x 256 by one block and of 256 x 256 by a pair, and
 // OR_MIRROR more where a tile's mirror image is written too.  Wide tiles fetch less per multiply-add, narrow
 // ones spread a few small matrices over more SMs; small matrices have SMs to spare for both triangles.
+//
+// A Gram matrix has few tiles, and each sums over the whole long side: where few matrices have long ones,
+// several blocks (not pairs) sum parts of it, and the last of them adds the parts (OR_JOIN, and OR_PART per part and
+// group of 64 columns of a warp: loads of few registers each, one L2 latency after the other).  The kernel that can do this takes 4 % longer where
+// it has nothing to split, so a split has to save a tenth of the estimate.  Five steps of 256 x 16,384 take
+// 373 us (whole sums 935), of 256 x 2,048 208 (226), of 200 x 5,000 253 (376).
 static const int OR_SHAPES = 5;
 static const int OR_WIDTHS[OR_SHAPES] = {64, 128, 192, 256, 256};
 static const double OR_BLOCK[OR_SHAPES] = {0.64, 0.88, 1.1, 1.27, 1.18}, OR_END[OR_SHAPES] = {2.6, 3.2, 4.2, 4.5, 4.5};
-static const double OR_MIRROR = 2.5;
+static const double OR_MIRROR = 2.5, OR_JOIN = 3.0, OR_PART = 2.0;
+static const int OR_SPLIT = 16, OR_SPLIT_BLOCKS = 4;  // most parts, fewest k-blocks of one
 
 struct OrthoShape {
     int bn_sym, bn_upd, pair, mirror;
+    double target;  // of a Gram matrix's item, from which its parts follow; 0: whole
 };
+static double or_cost(int kind, int m, int n, int w, int mirror, int split) {
+    const double end = OR_END[w] + (kind != OR_UPDATE && mirror && m > (w == 4 ? 256 : 128) ? OR_MIRROR : 0.0);
+    const double sum = or_b64(kind == OR_GRAM ? n : m) * OR_BLOCK[w];
+    return end + (split > 1 ? (sum / split) * 1.04 + OR_JOIN + OR_PART * (w < 2 ? 1 : 2) * split : sum);
+}
+// parts of a Gram matrix's sums: the fewest that bring an item's time down to `target`, or its least time's
+static int or_split(int m, int n, int w, int mirror, double target) {
+    int best = 1, most = or_b64(n) / OR_SPLIT_BLOCKS;
+    double least = or_cost(OR_GRAM, m, n, w, mirror, 1);
+    if (target <= 0.0) return 1;
+    for (int split = 2; least > target && split <= OR_SPLIT && split <= most; ++split) {
+        const double t = or_cost(OR_GRAM, m, n, w, mirror, split);
+        if (t < least) least = t, best = split;
+    }
+    return best;
+}
 // `count` matrices of list, or of one size
 static OrthoShape or_choose(const OrthoDesc* list, int64_t count, bool same) {
     const int sms = sm_count() < 1024 ? sm_count() : 1024;
-    OrthoShape best = {64, 64, 0, 1};
+    OrthoShape best = {64, 64, 0, 1, 0.0};
     double least = -1.0, load[1024];
-    for (int pair = 0; pair < 2; ++pair) {
-        const int blocks = pair ? sms / 2 : sms, w0 = pair ? 4 : 0, w1 = pair ? 5 : 4;
-        // the busiest block's time of a kind of product: 0 the Gram matrix and its polynomial, 1 the update
-        auto busiest = [&](int kind, int w, int mirror) {
-            auto cost = [&](int m, int n) {
-                return kind ? or_b64(m) * OR_BLOCK[w] + OR_END[w]
-                            : (or_b64(n) + or_b64(m)) * OR_BLOCK[w] + 2 * (OR_END[w] + (mirror && m > (pair ? 256 : 128) ? OR_MIRROR : 0.0));
-            };
-            auto tiles = [&](int m, int n) { return kind ? or_upds(m, n, OR_WIDTHS[w], pair) : or_syms(m, OR_WIDTHS[w], pair, mirror); };
-            if (same) return (double)((count * tiles(list[0].m, list[0].n) + blocks - 1) / blocks) * cost(list[0].m, list[0].n);
+    for (int pass = 0; pass < 3; ++pass) {  // single blocks, pairs, single blocks that split sums
+        const int pair = pass == 1, blocks = pair ? sms / 2 : sms, w0 = pair ? 4 : 0, w1 = pair ? 5 : 4;
+        // the busiest block's time of a kind of product
+        auto busiest = [&](int kind, int w, int mirror, double target) {
             double top = 0.0;
             int at = 0;
             for (int b = 0; b < blocks; ++b) load[b] = 0.0;
-            for (int64_t i = 0; i < count; ++i) {
-                const double c = cost(list[i].m, list[i].n);
-                for (int64_t t = tiles(list[i].m, list[i].n); t > 0; --t) {
+            for (int64_t i = 0; i < (same ? 1 : count); ++i) {
+                const int m = list[i].m, n = list[i].n, split = kind == OR_GRAM ? or_split(m, n, w, mirror, target) : 1;
+                const double c = or_cost(kind, m, n, w, mirror, split);
+                const int64_t tiles =
+                    split * (kind == OR_UPDATE ? or_upds(m, n, OR_WIDTHS[w], pair) : or_syms(m, OR_WIDTHS[w], pair, mirror));
+                if (same) return (double)((count * tiles + blocks - 1) / blocks) * c;
+                for (int64_t t = tiles; t > 0; --t) {
                     load[at] += c;
                     if (load[at] > top) top = load[at];
                     if (++at == blocks) at = 0;
@@ -1572,19 +1647,31 @@ static OrthoShape or_choose(const OrthoDesc* list, int64_t count, bool same) {
             return top;
         };
         double sym = -1.0, upd = -1.0;
-        OrthoShape shape = {0, 0, pair, 1};
+        OrthoShape shape = {0, 0, pair, 1, 0.0};
         for (int w = w0; w < w1; ++w) {
             for (int mirror = 0; mirror < 2; ++mirror) {
-                const double t = busiest(0, w, mirror);
-                if (sym < 0.0 || t < sym) sym = t, shape.bn_sym = OR_WIDTHS[w], shape.mirror = mirror;
+                const double square = busiest(OR_SQUARE, w, mirror, 0.0), whole = busiest(OR_GRAM, w, mirror, 0.0);
+                // a split's items: a half of the busiest block's time at whole sums, a quarter and so on
+                for (int i = pass == 2 ? 1 : 0; i < (pass == 2 ? 5 : 1); ++i) {
+                    const double target = i ? whole / (1 << i) : 0.0, t = square + (i ? busiest(OR_GRAM, w, mirror, target) : whole);
+                    if (sym < 0.0 || t < sym) sym = t, shape.bn_sym = OR_WIDTHS[w], shape.mirror = mirror, shape.target = target;
+                }
             }
-            const double t = busiest(1, w, 0);
+            const double t = busiest(OR_UPDATE, w, 0, 0.0);
             if (upd < 0.0 || t < upd) upd = t, shape.bn_upd = OR_WIDTHS[w];
         }
-        if (least < 0.0 || sym + upd < least) least = sym + upd, best = shape;
+        if (least < 0.0 || sym + upd < (pass == 2 ? 0.9 : 1.0) * least) least = sym + upd, best = shape;
     }
     return best;
 }
+static int or_split_of(int m, int n, const OrthoShape& s) {
+    int w = 0;
+    while (OR_WIDTHS[w] != s.bn_sym) ++w;
+    return or_split(m, n, w, s.mirror, s.target);
+}
+// bytes of the parts and arrival counters of `items` split items
+static int64_t or_parts_bytes(int64_t items, const OrthoShape& s) { return items * 128 * s.bn_sym * 4; }
+static int64_t or_arrived_bytes(int64_t items) { return items * ORTHO_EPI_WARPS * 4; }
 
 static int64_t or_up(int64_t v) { return (v + 1023) / 1024 * 1024; }
 
@@ -1623,28 +1710,32 @@ static int or_teams(const OrthoArgs& O, int cluster, cudaStream_t s) {
 }
 
 // conversion, then the products
-static int or_products(const OrthoArgs& O, cudaStream_t s) {
-    const void* const kernels[4] = {(const void*)orthogonalize_kernel<false, false>, (const void*)orthogonalize_kernel<true, false>,
-                                    (const void*)orthogonalize_kernel<false, true>, (const void*)orthogonalize_kernel<true, true>};
+static int or_products(const OrthoArgs& O, int64_t arrived_bytes, cudaStream_t s) {
+    const void* const kernels[6] = {
+        (const void*)orthogonalize_kernel<false, false, false>, (const void*)orthogonalize_kernel<true, false, false>,
+        (const void*)orthogonalize_kernel<false, true, false>,  (const void*)orthogonalize_kernel<true, true, false>,
+        (const void*)orthogonalize_kernel<false, false, true>,  (const void*)orthogonalize_kernel<true, false, true>};
     static int configured[64] = {0};
     int dev = 0, rc = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 6; ++i) {
             rc = cuda_status(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
                              "orthogonalize: shared memory size");
             if (rc) return rc;
         }
         if (dev >= 0 && dev < 64) configured[dev] = 1;
     }
-    rc = cuda_status(cudaMemsetAsync(O.barrier, 0, 4, s), "orthogonalize: barrier");
+    // the barrier's word and, behind it, the split sums' arrivals
+    rc = cuda_status(cudaMemsetAsync(O.barrier, 0, (size_t)(256 + arrived_bytes), s), "orthogonalize: barrier");
     if (rc) return rc;
     PBG_REQUIRE(O.convs < (1ll << 31), "orthogonalize: too many tiles for one launch");
     orthogonalize_convert_kernel<<<(unsigned)O.convs, ORTHO_FLAT, 0, s>>>(O);
     rc = launch_status("orthogonalize: conversion");
     if (rc) return rc;
     // one block per SM, all of them running at once
-    const int64_t tiles = O.syms > O.upds ? O.syms : O.upds;
+    int64_t tiles = O.syms > O.upds ? O.syms : O.upds;
+    if (O.grams > tiles) tiles = O.grams;
     const int64_t most = O.pair ? sm_count() / 2 * 2 : sm_count();
     const int64_t want = O.pair ? 2 * tiles : tiles;
     cudaLaunchConfig_t config = {};
@@ -1661,7 +1752,7 @@ static int or_products(const OrthoArgs& O, cudaStream_t s) {
     config.attrs = attribute;
     config.numAttrs = O.pair ? 2 : 1;
     void* args[] = {const_cast<OrthoArgs*>(&O)};
-    return cuda_status(cudaLaunchKernelExC(&config, kernels[(O.pair ? 2 : 0) + (O.precise ? 1 : 0)], args),
+    return cuda_status(cudaLaunchKernelExC(&config, kernels[(O.pair ? 2 : O.grams > O.syms ? 4 : 0) + (O.precise ? 1 : 0)], args),
                        "orthogonalize: cooperative launch");
 }
 
@@ -1705,6 +1796,25 @@ static int64_t or_at_once(int64_t batch, int m, int n) {
     return k < batch ? k : batch;
 }
 
+// a stack of matrices of one size: how many a launch takes, its tiles' shape, and the workspace
+struct OrthoUniform {
+    int64_t at_once, sums, parts, tiles, bytes;
+    OrthoShape shape;
+    int split;
+};
+static OrthoUniform or_uniform(int64_t batch, const OrthoDesc& d) {
+    OrthoUniform U;
+    U.at_once = or_at_once(batch, d.m, d.n);
+    U.shape = or_choose(&d, U.at_once, true);
+    U.split = or_split_of(d.m, d.n, U.shape);
+    const int64_t items = U.split > 1 ? U.at_once * U.split * or_syms(d.m, U.shape.bn_sym, U.shape.pair, U.shape.mirror) : 0;
+    U.sums = or_up(256 + or_arrived_bytes(items));
+    U.parts = U.sums + or_up(U.at_once * or_spans((int64_t)d.m * d.n) * 8);
+    U.tiles = U.parts + or_up(or_parts_bytes(items, U.shape));
+    U.bytes = U.tiles + U.at_once * or_tiles_bytes(d.m, d.n);
+    return U;
+}
+
 }  // namespace pbg
 
 using namespace pbg;
@@ -1715,8 +1825,7 @@ int64_t pbg_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols) {
     if (batch <= 0 || rows <= 0 || cols <= 0 || rows > 65536 || cols > 65536) return 0;
     const OrthoDesc d = or_make(rows, cols);
     if (d.team) return 1024;
-    const int64_t k = or_at_once(batch, d.m, d.n);
-    return 1024 + or_up(k * or_spans(rows * cols) * 8) + k * or_tiles_bytes(d.m, d.n);
+    return or_uniform(batch, d).bytes;
 }
 
 int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, int32_t x_type, void* out, int32_t out_type,
@@ -1731,41 +1840,45 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
     if (batch == 0 || rows == 0 || cols == 0) return 0;
     PBG_REQUIRE(x && out && workspace && error, "orthogonalize: null pointer");
     PBG_REQUIRE((uintptr_t)workspace % 256 == 0, "orthogonalize: workspace must be 256-byte aligned");
-    PBG_REQUIRE(workspace_bytes >= pbg_orthogonalize_workspace(batch, rows, cols), "orthogonalize: workspace too small");
     OrthoArgs O = {};
     O.one = or_make(rows, cols);
     const int m = O.one.m, n = O.one.n;
-    const int64_t k = or_at_once(batch, m, n);
-    unsigned char* w = static_cast<unsigned char*>(workspace);
-    O.barrier = reinterpret_cast<uint32_t*>(w);
-    O.sums = reinterpret_cast<double*>(w + 1024);
-    O.tiles = w + 1024 + or_up(k * or_spans(rows * cols) * 8);
     O.one_src = rows * cols;
-    O.one_ws = or_tiles_bytes(m, n);
-    O.one_span = or_spans(rows * cols);
-    O.one_conv = (int64_t)or_mb(m) * or_b64(n);
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.x_type = x_type, O.out_type = out_type, O.error = error;
     O.precise = !(out_type == 1 && m >= ORTHO_SINGLE);
     if (O.one.team) {
+        PBG_REQUIRE(workspace_bytes >= 1024, "orthogonalize: workspace too small");
         O.count = batch, O.slots = batch * O.one.team;
         O.x = x, O.out = out;
         O.aligned = (uintptr_t)x % 16 == 0 && (uintptr_t)out % 16 == 0;
         return or_teams(O, O.one.team, as_stream(stream));
     }
+    const OrthoUniform U = or_uniform(batch, O.one);
+    PBG_REQUIRE(workspace_bytes >= U.bytes, "orthogonalize: workspace too small");
+    unsigned char* w = static_cast<unsigned char*>(workspace);
+    O.barrier = reinterpret_cast<uint32_t*>(w);
+    O.arrived = reinterpret_cast<uint32_t*>(w + 256);
+    O.sums = reinterpret_cast<double*>(w + U.sums);
+    O.parts = reinterpret_cast<float*>(w + U.parts);
+    O.tiles = w + U.tiles;
+    O.bn_sym = U.shape.bn_sym, O.bn_upd = U.shape.bn_upd, O.pair = U.shape.pair, O.mirror = U.shape.mirror;
+    O.one.split = U.split;
+    O.one_ws = or_tiles_bytes(m, n);
+    O.one_span = or_spans(rows * cols);
+    O.one_conv = (int64_t)or_mb(m) * or_b64(n);
+    O.one_sym = or_syms(m, O.bn_sym, O.pair, O.mirror), O.one_upd = or_upds(m, n, O.bn_upd, O.pair);
+    O.one_gram = O.one_sym * U.split;
     const int64_t xs = x_type == 0 ? 4 : 2, os = out_type == 0 ? 4 : 2;
-    for (int64_t at = 0; at < batch; at += k) {
-        O.count = batch - at < k ? batch - at : k;
-        const OrthoShape shape = or_choose(&O.one, O.count, true);
-        O.bn_sym = shape.bn_sym, O.bn_upd = shape.bn_upd, O.pair = shape.pair, O.mirror = shape.mirror;
-        O.one_sym = or_syms(m, O.bn_sym, O.pair, O.mirror), O.one_upd = or_upds(m, n, O.bn_upd, O.pair);
+    for (int64_t at = 0; at < batch; at += U.at_once) {
+        O.count = batch - at < U.at_once ? batch - at : U.at_once;
         O.spans = O.count * O.one_span, O.convs = O.count * O.one_conv;
-        O.syms = O.count * O.one_sym, O.upds = O.count * O.one_upd;
+        O.grams = O.count * O.one_gram, O.syms = O.count * O.one_sym, O.upds = O.count * O.one_upd;
         O.x = static_cast<const unsigned char*>(x) + at * rows * cols * xs;
         O.out = static_cast<unsigned char*>(out) + at * rows * cols * os;
         O.aligned = (uintptr_t)O.x % 16 == 0 && (uintptr_t)O.out % 16 == 0;
         rc = or_squares(O, as_stream(stream));
-        if (!rc) rc = or_products(O, as_stream(stream));
+        if (!rc) rc = or_products(O, U.split > 1 ? or_arrived_bytes(O.grams) : 0, as_stream(stream));
         if (rc) return rc;
     }
     return 0;
@@ -1773,7 +1886,7 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
 
 int64_t pbg_muon_descriptor_bytes(void) { return (int64_t)sizeof(OrthoDesc); }
 
-int64_t pbg_muon_plan_words(int64_t count) { return count < 0 ? 0 : 9 + 5 * count; }
+int64_t pbg_muon_plan_words(int64_t count) { return count < 0 ? 0 : 10 + 7 * count; }
 
 int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, const int64_t* cols, const float* adjust,
                   void* descriptors, int64_t* plan) {
@@ -1802,14 +1915,14 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
     }
     const OrthoShape shape = or_choose(list, general, false);
     const int bn_sym = shape.bn_sym, bn_upd = shape.bn_upd, pair = shape.pair;
-    int64_t waves = 0, most = 0;
+    int64_t waves = 0, most = 0, most_items = 0;
     int64_t* wave = plan + 8;
     OrthoDesc at = {};
     for (int64_t i = 0; i < general; ++i) {
         const int m = list[i].m, n = list[i].n;
         const int64_t bytes = or_tiles_bytes(m, n);
         if (i == 0 || at.ws + bytes > ORTHO_BUDGET) {  // the next launch
-            if (i) wave += 5;
+            if (i) wave += 7;
             at = OrthoDesc{};
             wave[0] = i;
             ++waves;
@@ -1819,13 +1932,21 @@ int pbg_muon_plan(int64_t count, const int64_t* offset, const int64_t* rows, con
         at.conv0 += (int64_t)or_mb(m) * or_b64(n);
         at.sym0 += or_syms(m, bn_sym, pair, shape.mirror);
         at.upd0 += or_upds(m, n, bn_upd, pair);
+        const int split = or_split_of(m, n, shape);
+        const int64_t items = split * or_syms(m, bn_sym, pair, shape.mirror);
+        list[i].split = split, list[i].gram0 = at.gram0, list[i].part0 = at.part0;
+        at.gram0 += items;
+        if (split > 1) at.part0 += items;
+        if (at.part0 > most_items) most_items = at.part0;
         if (at.ws > most) most = at.ws;
         wave[1] = i + 1 - wave[0], wave[2] = at.conv0, wave[3] = at.sym0, wave[4] = at.upd0;
+        wave[5] = at.gram0, wave[6] = at.part0;
     }
-    plan[0] = 1024 + or_up(spans * 8) + most;
+    plan[0] = or_up(256 + or_arrived_bytes(most_items)) + or_up(spans * 8) + or_up(or_parts_bytes(most_items, shape)) + most;
     plan[1] = spans, plan[2] = waves, plan[3] = bn_sym, plan[4] = bn_upd;
     plan[5] = pair + 2 * shape.mirror, plan[6] = general, plan[7] = slots;
-    plan[8 + 5 * waves] = slots ? list[general].team : 0;  // the clusters' size
+    plan[8 + 7 * waves] = slots ? list[general].team : 0;  // the clusters' size
+    plan[9 + 7 * waves] = most_items;
     return 0;
 }
 
@@ -1841,9 +1962,15 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
     cudaStream_t s = as_stream(stream);
     unsigned char* w = static_cast<unsigned char*>(workspace);
     OrthoArgs O = {};
+    const int64_t waves = plan[2], most_items = plan[9 + 7 * waves];
+    const OrthoShape shape = {(int)plan[3], (int)plan[4], (int)plan[5] & 1, (int)plan[5] >> 1, 0.0};
     O.barrier = reinterpret_cast<uint32_t*>(w);
-    O.sums = reinterpret_cast<double*>(w + 1024);
-    O.tiles = w + 1024 + or_up(plan[1] * 8);
+    O.arrived = reinterpret_cast<uint32_t*>(w + 256);
+    w += or_up(256 + or_arrived_bytes(most_items));
+    O.sums = reinterpret_cast<double*>(w);
+    w += or_up(plan[1] * 8);
+    O.parts = reinterpret_cast<float*>(w);
+    O.tiles = w + or_up(or_parts_bytes(most_items, shape));
     O.bn_sym = (int)plan[3], O.bn_upd = (int)plan[4], O.pair = (int)plan[5] & 1, O.mirror = (int)plan[5] >> 1;
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.precise = 1;
@@ -1853,21 +1980,20 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
     rc = cuda_status(cudaMemsetAsync(skipped, 0, 4, s), "muon_step: status");
     if (rc) return rc;
     const OrthoDesc* list = static_cast<const OrthoDesc*>(descriptors);
-    const int64_t waves = plan[2];
     O.list = list, O.count = count, O.spans = plan[1];
     rc = or_squares(O, s);  // of all matrices: every direction is checked before anything is written
     if (rc) return rc;
     for (int64_t i = 0; i < waves; ++i) {
-        const int64_t* wave = plan + 8 + 5 * i;
+        const int64_t* wave = plan + 8 + 7 * i;
         O.list = list + wave[0], O.count = wave[1];
-        O.convs = wave[2], O.syms = wave[3], O.upds = wave[4];
-        rc = or_products(O, s);
+        O.convs = wave[2], O.syms = wave[3], O.upds = wave[4], O.grams = wave[5];
+        rc = or_products(O, or_arrived_bytes(wave[6]), s);
         if (rc) return rc;
     }
     if (plan[7]) {
         const int64_t general = plan[6];
         O.list = list + general, O.count = count - general, O.slots = plan[7];
-        return or_teams(O, (int)plan[8 + 5 * waves], s);
+        return or_teams(O, (int)plan[8 + 7 * waves], s);
     }
     return 0;
 }

@@ -239,6 +239,46 @@ def test_graph_replay_controls_and_two_optimizers():
     assert all(torch.equal(o, orthogonalize(x)) for o in outs)
 
 
+@pytest.mark.parametrize("batch,m,n", [(1, 256, 2048), (1, 129, 16391), (1, 65536, 256), (3, 200, 4097), (1, 640, 8192)])
+def test_long_sides_are_summed_in_parts(batch, m, n):
+    """Few matrices with a long side: several blocks sum each Gram tile, in an order of their own, the same every call."""
+    from pbg_b200.optim import orthogonalize, orthogonalize_error
+
+    gen = torch.Generator(device=DEV).manual_seed(m + n)
+    x = torch.stack([_matrix("low", m, n, gen) for _ in range(batch)])
+    ref = _reference(x)
+    got = orthogonalize(x)
+    half = orthogonalize(x, out_dtype=BF16)
+    for i in range(batch):
+        assert _off(got[i], ref[i]) <= FP32_BAR
+        assert _off(half[i], ref[i]) <= BAR[BF16]
+    for _ in range(3):
+        orthogonalize(x[:, :150, :150])  # other work in the same workspace
+        assert torch.equal(got, orthogonalize(x))
+    assert orthogonalize_error(DEV) == 0
+
+
+def test_transition_with_long_matrices():
+    from pbg_b200.optim import FlatMuon, orthogonalize_error
+
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    mats = [(0, 256, 8192), (2097152, 160, 160), (2122752, 7000, 192), (3466752, 64, 90)]
+    n = 3472512
+    step = FlatMuon(torch.randn(n, generator=gen, device=DEV), mats, lr=0.05, momentum=0.9)
+    twin = FlatMuon(step.master.clone(), mats, lr=0.05, momentum=0.9)
+    for _ in range(2):
+        g = torch.randn(n, generator=gen, device=DEV)
+        step.grad.copy_(g), twin.grad.copy_(g)
+        w, m = _muon_reference(step.master, step.momentum, g, mats, 0.05, 0.9, 0.0, True, "shape")
+        step.step(), twin.step()
+        for at, r, c in mats:
+            s = slice(at, at + r * c)
+            bar = 0.05 * math.sqrt(max(1.0, r / c)) * FP32_BAR * 1.3 * math.sqrt(min(r, c)) + 2.0 ** -23 * float(w[s].norm())
+            assert float((step.master[s].double() - w[s]).norm()) <= bar
+        assert torch.equal(step.master, twin.master)
+    assert orthogonalize_error(DEV) == 0
+
+
 def test_transition_refusals():
     from pbg_b200.optim import FlatMuon
 
