@@ -38,9 +38,10 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from ._native import NativeError, call, ptr, stream
+from ._native import NativeError, call, ptr, raw_stream, stream
 from .embedding import embedding, embedding_backward
 from .model import _error_word, attention, linear_ex
 
@@ -234,16 +235,28 @@ class _EmbeddingFn(torch.autograd.Function):
         return embedding(table, index, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         (index,) = ctx.saved_tensors
         return embedding_backward(dy, index, ctx.rows, ctx.scale, out_dtype=ctx.dtype), None, None
 
 
 def embedding_train(table: Tensor, index: Tensor, scale: float = 1.0) -> Tensor:
-    """``scale * table[index]`` in the table's type, differentiable in the table: its gradient is the sum
-    of the incoming rows of each index (``pbg_embedding_backward``)."""
+    """``scale * table[index]`` in the table's type, differentiable (once) in the table: its gradient is the
+    sum of the incoming rows of each index (``pbg_embedding_backward``).
 
-    return _EmbeddingFn.apply(table, index, float(scale))
+    A leaf's gradient is accumulated on the stream of the oldest graph of it that lives, so a capture must
+    not begin while a lookup of the same table made on another stream is still referenced (its output or
+    what was computed from it): such a call is refused."""
+
+    out = _EmbeddingFn.apply(table, index, float(scale))
+    if table.is_leaf and out.grad_fn is not None:
+        # the leaf's accumulation node lives as long as a graph that leads to it, and its notes with it
+        notes = out.grad_fn.next_functions[0][0].metadata
+        now = raw_stream(table.device.index)
+        if notes.setdefault("pbg_b200 stream", now) != now and torch.cuda.is_current_stream_capturing():
+            raise NativeError("embedding_train: release the graphs of this table made on another stream before capturing")
+    return out
 
 
 def q_scale_of(theta: Tensor) -> Tensor:

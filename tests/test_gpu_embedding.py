@@ -282,3 +282,37 @@ def test_refusals():
                  lambda: embedding_backward(grad.double(), index, 4)):
         with pytest.raises(NativeError):
             call()
+
+
+def test_capture_with_an_eager_graph_of_the_table():
+    """A captured backward of a leaf whose older graph lives on another stream is refused, and works once it is gone."""
+    from pbg_b200._native import NativeError
+    from pbg_b200.model_train import embedding_train
+
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    table = torch.randn(30, 64, generator=gen, device=DEV, requires_grad=True)
+    index = torch.randint(30, (500,), generator=gen, device=DEV)
+    weight = torch.randn(500, 64, generator=gen, device=DEV)
+    eager = (embedding_train(table, index) * weight).sum()
+    eager.backward()
+    want = table.grad.clone()
+    table.grad.zero_()
+    refused = False
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        try:
+            embedding_train(table, index)
+        except NativeError:
+            refused = True
+    assert refused
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (embedding_train(table, index) * weight).sum().backward()
+    table.grad.zero_()
+    for _ in range(2):
+        graph.replay()
+    assert torch.equal(table.grad, want + want)
+    # twice differentiable it is not
+    g = torch.autograd.grad((embedding_train(table, index) * weight).square().sum(), table, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
