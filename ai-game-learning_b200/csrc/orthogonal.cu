@@ -8,9 +8,15 @@
 // orthogonalises each matrix's momentum and adds it to the matrix.
 //
 // A step is three products per matrix: A = X X^T, B = a I + b A + c A A (both symmetric: only the tiles
-// on and above the diagonal are computed, the others mirrored), X' = B X, run on the tensor cores
-// (tcgen05, fp32 accumulation in tensor memory) over all matrices of the call at once, a persistent CTA
-// per SM.
+// on and above the diagonal are computed, the others mirrored, where there are more tiles than SMs), X' = B X,
+// run on the tensor cores (tcgen05, fp32 accumulation in tensor memory) over all matrices of the call at once:
+// one cooperative launch, a block per SM, or a pair of them on tiles of 256 x 256, with a grid barrier (1.3 us)
+// between the 3 * steps products.  A matrix whose short side is at most 128 stays, with everything that is
+// made of it, in the shared memory of a team of 1 to 8 blocks (orthogonalize_team_kernel).
+//
+// What bounds it.  4,096 x 4,096: the tensor cores, 1.43 PFLOP/s of fp16 products in three passes (fp32,
+// 3.13 ms), power-capped.  14 of 256 x 1,024 (218 us): 15 products of a few microseconds each behind one
+// another, so each one's first copies, last stores and the barrier.
 //
 // Precision.  16-bit operands alone are not enough: an error in X in the direction of a small singular
 // value grows by a = 3.4 each step, so X is carried as a pair of fp16 numbers hi + lo of 2^14 X (22
@@ -1715,16 +1721,30 @@ static int or_products(const OrthoArgs& O, int64_t arrived_bytes, cudaStream_t s
         (const void*)orthogonalize_kernel<false, false, false>, (const void*)orthogonalize_kernel<true, false, false>,
         (const void*)orthogonalize_kernel<false, true, false>,  (const void*)orthogonalize_kernel<true, true, false>,
         (const void*)orthogonalize_kernel<false, false, true>,  (const void*)orthogonalize_kernel<true, false, true>};
-    static int configured[64] = {0};
+    static int pairs_at_once[64] = {0};  // pairs of blocks that the device runs at once, from the first call on
     int dev = 0, rc = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
+    rc = cuda_status(cudaGetDevice(&dev), "orthogonalize: device");
+    if (rc) return rc;
+    PBG_REQUIRE(dev < 64, "orthogonalize: at most 64 devices");
+    if (!pairs_at_once[dev]) {
         for (int i = 0; i < 6; ++i) {
             rc = cuda_status(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
                              "orthogonalize: shared memory size");
             if (rc) return rc;
         }
-        if (dev >= 0 && dev < 64) configured[dev] = 1;
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3((unsigned)sm_count() / 2 * 2), config.blockDim = dim3(ORTHO_THREADS);
+        config.dynamicSmemBytes = ORTHO_SMEM;
+        cudaLaunchAttribute cluster[1];
+        cluster[0].id = cudaLaunchAttributeClusterDimension;
+        cluster[0].val.clusterDim.x = 2;
+        cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+        config.attrs = cluster, config.numAttrs = 1;
+        int pairs = 0;
+        rc = cuda_status(cudaOccupancyMaxActiveClusters(&pairs, kernels[3], &config), "orthogonalize: pairs of blocks");
+        if (rc) return rc;
+        PBG_REQUIRE(pairs >= 1, "orthogonalize: the device runs no pair of blocks");
+        pairs_at_once[dev] = pairs;
     }
     // the barrier's word and, behind it, the split sums' arrivals
     rc = cuda_status(cudaMemsetAsync(O.barrier, 0, (size_t)(256 + arrived_bytes), s), "orthogonalize: barrier");
@@ -1736,7 +1756,7 @@ static int or_products(const OrthoArgs& O, int64_t arrived_bytes, cudaStream_t s
     // one block per SM, all of them running at once
     int64_t tiles = O.syms > O.upds ? O.syms : O.upds;
     if (O.grams > tiles) tiles = O.grams;
-    const int64_t most = O.pair ? sm_count() / 2 * 2 : sm_count();
+    const int64_t most = O.pair ? std::min(sm_count() / 2, pairs_at_once[dev]) * 2 : sm_count();
     const int64_t want = O.pair ? 2 * tiles : tiles;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(want < most ? want : most));
