@@ -13,6 +13,7 @@
 //   - few table rows (EMB_TABLE): every warp keeps the whole table's sums for its columns in shared memory
 //     and adds its share of the tokens' rows in order; then the warps' and the blocks' tables are added in
 //     order.  81,920 x 128 bf16 into 13 rows: 15.5 us (sorted 37); 1,000,003 x 128 into 4 rows: 94 us (125).
+//   - small tables of narrow rows (emb_narrow_plan): ranges of rows x 16 columns in a block's shared memory.
 //   - else sorted tokens, one cooperative kernel:
 //     1. a stable radix sort of (index, position) pairs: least significant digit first, at most 9 bits a
 //        pass (the least number of passes, bits shared evenly).  Each sorting block owns a contiguous range
@@ -452,7 +453,9 @@ __device__ __forceinline__ uint32_t emb_last_key(const EmbGradArgs& E, const uin
 }
 
 // parts of the run that starts in `share` and goes on past its end; 0 where there is none.  The lanes of a
-// worker (in step) look at the first keys of as many shares after it at once.
+// worker (in step) look at the first keys of as many shares after it at once, in strides that grow while all of
+// them belong to the run and shrink again where it ends: of 83,414 x 8 tokens' rows, Zipf-distributed over 1,331,
+// the longest run crosses hundreds of shares; looked at one group after another they took half of the 84 us.
 __device__ __forceinline__ int64_t emb_run_parts(const EmbGradArgs& E, const uint32_t* key, int64_t share, int lane, int lanes,
                                                  uint32_t group_mask) {
     const int64_t begin = share * E.share, end = begin + E.share;
@@ -460,14 +463,18 @@ __device__ __forceinline__ int64_t emb_run_parts(const EmbGradArgs& E, const uin
     const uint32_t run = __ldcg(key + end - 1), next = __ldcg(key + end);
     const uint32_t before = begin > 0 ? __ldcg(key + begin - 1) : 0xffffffffu;
     if (run >= (uint32_t)E.rows || next != run || before == run) return 0;
-    int64_t parts = 1;
-    while (true) {
-        const int64_t at = (share + parts + lane) * E.share;
+    int64_t last = 1, stride = 1;
+    bool up = true;
+    while (up || stride > 1) {
+        if (!up) stride /= lanes;
+        const int64_t at = (share + last + (lane + 1) * stride) * E.share;
         const uint32_t on = __ballot_sync(group_mask, at < E.tokens && __ldcg(key + at) == run) & group_mask;
         const int more = __popc(on);  // sorted keys: the shares that the run reaches come first
-        parts += more;
-        if (more < lanes) return parts;
+        last += more * stride;
+        if (up && more == lanes) stride *= lanes;
+        else up = false;
     }
+    return last + 1;
 }
 
 // parts [i0, i1) of the run that starts in `share`: part 0 is that share's tail, part i the head of the
@@ -711,7 +718,8 @@ __device__ __forceinline__ void emb_add_matches(const EmbGradArgs& E, uint32_t m
     }
 }
 
-// a warp per table row (in turn), all indices in its lanes
+// a warp per table row (in turn) and, where few rows leave warps idle, stretch of its columns (gridDim.y); all
+// indices in its lanes
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) embedding_backward_warp_kernel(EmbGradArgs E) {
     const int lane = threadIdx.x & 31;
@@ -727,7 +735,7 @@ __global__ void __launch_bounds__(256) embedding_backward_warp_kernel(EmbGradArg
             any |= match[k];
         }
         if (!any && E.accumulate) continue;
-        for (int64_t c = (int64_t)lane * VEC; c - lane * VEC < E.width; c += 32 * VEC) {
+        for (int64_t c = ((int64_t)blockIdx.y * 32 + lane) * VEC; c - lane * VEC < E.width; c += (int64_t)gridDim.y * 32 * VEC) {
             const bool in = c < E.width;
             float sum[VEC];
 #pragma unroll
@@ -836,6 +844,21 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_table_kerne
     }
 }
 
+// few blocks' tables in order: a column a thread
+constexpr int EMB_FOLD_FEW = 32;
+__global__ void __launch_bounds__(256) embedding_backward_fold_few_kernel(EmbGradArgs E, int blocks) {
+    const int64_t total = E.rows * E.width, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= total) return;
+    float sum = 0.0f;
+    for (int b = 0; b < blocks; b += 8) {
+        float x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] = b + u < blocks ? __ldcg(E.part_sums + (int64_t)(b + u) * total + at) : 0.0f;
+        sum += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    }
+    if (sum != 0.0f || !E.accumulate) emb_finish<1>(E, (uint32_t)(at / E.width), at % E.width, &sum);
+}
+
 // the blocks' tables in order: 32 columns and 16 stretches of the blocks a block
 __global__ void __launch_bounds__(EMB_THREADS) embedding_backward_fold_kernel(EmbGradArgs E, int blocks) {
     __shared__ float part[EMB_WARPS][32];
@@ -855,8 +878,202 @@ __global__ void __launch_bounds__(EMB_THREADS) embedding_backward_fold_kernel(Em
     __syncthreads();
     if (warp == 0 && at < total) {
         for (int w = 1; w < EMB_WARPS; ++w) sum += part[w][lane];
-        emb_finish<1>(E, (uint32_t)(at / E.width), at % E.width, &sum);
+        if (sum != 0.0f || !E.accumulate) emb_finish<1>(E, (uint32_t)(at / E.width), at % E.width, &sum);
     }
+}
+
+// ---------------------------------------------------------------- narrow rows
+
+// A block keeps the fp32 sums of a range of table rows and up to 16 columns in shared memory; each of its warps
+// owns the rows of one residue class of them, so that every row has one writer.  grid (shares of the tokens,
+// row ranges, column tiles).
+constexpr int EMB_NARROW_COLS = 16;           // a token's row in a lane's registers
+constexpr int EMB_NARROW_FLOATS = 22 * 1024;  // of sums: two blocks fit an SM
+constexpr int EMB_NARROW_CHUNK = 2048;        // tokens looked through at a time
+constexpr int EMB_NARROW_QUEUE = 96;          // of a warp: two batches of 32 are added at once, 32 more may come
+constexpr int EMB_NARROW_SHARE = 1024;        // tokens of a share at least
+constexpr int EMB_NARROW_BIG = 6;             // lanes of a batch on one row, from which they add across lanes
+constexpr int EMB_NARROW_ROWS = 1024;         // of the table at least
+constexpr int64_t EMB_NARROW_LOOKS = 720000;  // blocks that divide the table x tokens, at most
+constexpr int EMB_NARROW_SMEM = 4 * (EMB_NARROW_FLOATS + EMB_NARROW_CHUNK + 2 * EMB_WARPS * EMB_NARROW_QUEUE);
+
+struct EmbNarrow {
+    int cols, stride;   // of a column tile, and of a row's sums in shared memory: odd, for the banks
+    int64_t rows;       // of a range
+    int64_t ranges, tiles, shares, share;
+};
+
+// one token a lane (row: its row in the range, or -1) added to the warp's rows, in the order of the lanes
+__device__ __forceinline__ void emb_narrow_add(float* table, int cols, int stride, int row, const float* v, int lane) {
+    const uint32_t same = __match_any_sync(0xffffffffu, row);
+    bool has = row >= 0;
+    // rows that many lanes have: summed across the lanes, in an order that the lanes alone determine
+    for (uint32_t big; (big = __ballot_sync(0xffffffffu, has && __popc(same) >= EMB_NARROW_BIG)) != 0u;) {
+        const int leader = __ffs(big) - 1;
+        const uint32_t members = __shfl_sync(0xffffffffu, same, leader);
+        const int r = __shfl_sync(0xffffffffu, row, leader);
+        const bool in = (members >> lane) & 1u;
+        // halves of the columns change lanes, then quarters and so on: a column per pair of lanes is left
+        float x[EMB_NARROW_COLS];
+#pragma unroll
+        for (int c = 0; c < EMB_NARROW_COLS; ++c) x[c] = in && c < cols ? v[c] : 0.0f;
+#pragma unroll
+        for (int d = 16; d > 1; d >>= 1) {
+            const bool upper = lane & d;
+#pragma unroll
+            for (int c = 0; c < d / 2; ++c) {
+                const float give = upper ? x[c] : x[c + d / 2], keep = upper ? x[c + d / 2] : x[c];
+                x[c] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+            }
+        }
+        x[0] += __shfl_xor_sync(0xffffffffu, x[0], 1);
+        if (!(lane & 1) && lane / 2 < cols) table[r * stride + lane / 2] += x[0];
+        if (in) has = false;
+        __syncwarp();
+    }
+    const int turn = __popc(same & ((1u << lane) - 1u));
+    for (int k = 0; __any_sync(0xffffffffu, has); ++k) {
+        if (has && turn == k) {
+            float* to = table + row * stride;
+#pragma unroll
+            for (int c = 0; c < EMB_NARROW_COLS; c += 8) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? to[c + i] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (c + i < cols) to[c + i] = x[i] + v[c + i];
+            }
+            has = false;
+        }
+        __syncwarp();
+    }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_narrow_kernel(EmbGradArgs E, EmbNarrow N) {
+    extern __shared__ __align__(16) float emb_tables[];
+    float* table = emb_tables;
+    uint32_t* list = reinterpret_cast<uint32_t*>(table + EMB_NARROW_FLOATS);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t* queue_row = list + EMB_NARROW_CHUNK + warp * 2 * EMB_NARROW_QUEUE;
+    uint32_t* queue_at = queue_row + EMB_NARROW_QUEUE;
+    __shared__ uint32_t found[EMB_WARPS];
+    const int64_t row0 = (int64_t)blockIdx.y * N.rows, c0 = (int64_t)blockIdx.z * N.cols;
+    const int rows = (int)(E.rows - row0 < N.rows ? E.rows - row0 : N.rows);
+    const int cols = (int)(E.width - c0 < N.cols ? E.width - c0 : N.cols);
+    const int64_t lo = (int64_t)blockIdx.x * N.share, hi = lo + N.share < E.tokens ? lo + N.share : E.tokens;
+    const T* grad = static_cast<const T*>(E.grad) + lo * E.ldg + c0;
+    const int stride = N.stride;
+    for (int i = threadIdx.x; i < rows * stride; i += EMB_THREADS) table[i] = 0.0f;
+    int queued = 0;
+    // the queue's first n (up to 64) tokens, both batches' rows in flight at once
+    auto add = [&](int n) {
+        float v[2][EMB_NARROW_COLS];
+        int row[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const int i = b * 32 + lane;
+            row[b] = i < n ? (int)queue_row[i] : -1;
+            const T* p = grad + (i < n ? (int64_t)queue_at[i] : 0) * E.ldg;
+#pragma unroll
+            for (int c = 0; c < EMB_NARROW_COLS; c += VEC) {
+                if (row[b] >= 0 && c < cols) emb_load<T, VEC>(p + c, v[b] + c);
+            }
+        }
+        emb_narrow_add(table, cols, stride, row[0], v[0], lane);
+        if (n > 32) emb_narrow_add(table, cols, stride, row[1], v[1], lane);
+    };
+    constexpr int K = EMB_NARROW_CHUNK / EMB_THREADS;
+    for (int64_t t0 = lo; t0 < hi; t0 += EMB_NARROW_CHUNK) {
+        // the chunk's tokens of this range, in order: (row, place in the chunk); each warp looks at a stretch
+        uint32_t key[K], in[K], count = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const int64_t t = t0 + warp * (32 * K) + k * 32 + lane;
+            key[k] = t < hi ? emb_key(E, t) : 0xffffffffu;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            const bool mine = key[k] < (uint32_t)E.rows && (int64_t)key[k] >= row0 && (int64_t)key[k] < row0 + rows;
+            in[k] = __ballot_sync(0xffffffffu, mine);
+            count += __popc(in[k]);
+        }
+        __syncthreads();  // the list and the counts are free (and the table is cleared)
+        if (lane == 0) found[warp] = count;
+        __syncthreads();
+        uint32_t at = 0, total = 0;
+        for (int w = 0; w < EMB_WARPS; ++w) {
+            if (w < warp) at += found[w];
+            total += found[w];
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if ((in[k] >> lane) & 1u)
+                list[at + __popc(in[k] & ((1u << lane) - 1u))] =
+                    (uint32_t)((int64_t)key[k] - row0) * EMB_NARROW_CHUNK + warp * (32 * K) + k * 32 + lane;
+            at += __popc(in[k]);
+        }
+        __syncthreads();
+        // each warp: its rows' tokens to its queue
+        for (uint32_t i0 = 0; i0 < total; i0 += 32) {
+            const uint32_t entry = i0 + lane < total ? list[i0 + lane] : 0u;
+            const uint32_t row = entry / EMB_NARROW_CHUNK;
+            const bool mine = i0 + lane < total && (row & (EMB_WARPS - 1)) == (uint32_t)warp;
+            const uint32_t who = __ballot_sync(0xffffffffu, mine);
+            if (mine) {
+                const int q = queued + __popc(who & ((1u << lane) - 1u));
+                queue_row[q] = row;
+                queue_at[q] = (uint32_t)(t0 - lo) + entry % EMB_NARROW_CHUNK;
+            }
+            queued += __popc(who);
+            __syncwarp();
+            if (queued >= 64) {
+                add(64);
+                queued -= 64;
+                const uint32_t r = lane < queued ? queue_row[64 + lane] : 0u, a = lane < queued ? queue_at[64 + lane] : 0u;
+                __syncwarp();
+                if (lane < queued) queue_row[lane] = r, queue_at[lane] = a;
+                __syncwarp();
+            }
+        }
+    }
+    if (queued > 0) add(queued);
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * cols; i += EMB_THREADS) {
+        const int64_t r = row0 + i / cols, c = c0 + i % cols;
+        float sum = table[i / cols * stride + i % cols];
+        if (N.shares > 1) E.part_sums[((int64_t)blockIdx.x * E.rows + r) * E.width + c] = sum;
+        else if (sum != 0.0f || !E.accumulate) emb_finish<1>(E, (uint32_t)r, c, &sum);
+    }
+}
+
+// Whether rows are taken so, and their split.  Every block looks at its share's indices, so blocks x tokens
+// bounds it; few rows leave a warp's rows to batches of one row.  Measured, sorted against this way: 9,000
+// tokens into 30,000 x 16 35 and 15 us, 30,000 into 4,000 x 32 35 and 21 us, 300,000 into 4,000 x 8 54 and 41
+// us; but 100,000 into 4,000 x 32 (800,000 looks) 37 and 50 us, 30,000 into 500 x 16 26 and 41 us.
+static bool emb_narrow_plan(int64_t tokens, int64_t rows, int64_t width, int grid_max, EmbNarrow& N) {
+    N.cols = (int)(width < EMB_NARROW_COLS ? width : EMB_NARROW_COLS);
+    N.stride = N.cols | 1;
+    N.tiles = (width + N.cols - 1) / N.cols;
+    N.rows = EMB_NARROW_FLOATS / N.stride;
+    N.ranges = (rows + N.rows - 1) / N.rows;
+    N.rows = (rows + N.ranges - 1) / N.ranges;  // ranges of equal sizes
+    const int64_t blocks = N.ranges * N.tiles;
+    if (rows < EMB_NARROW_ROWS || blocks > EMB_NARROW_LOOKS / tokens) return false;
+    int64_t most = grid_max / blocks;
+    if (most > tokens / EMB_NARROW_SHARE) most = tokens / EMB_NARROW_SHARE;
+    // shares by estimated microseconds: chunks looked through, then the shares' sums written and read
+    double least = 0.0;
+    for (int64_t shares = 1; shares == 1 || shares <= most; ++shares) {
+        const int64_t share = (tokens + shares - 1) / shares, waves = (blocks * shares + grid_max - 1) / grid_max;
+        const double looks = 4.0 + 3.0 * ((share + EMB_NARROW_CHUNK - 1) / EMB_NARROW_CHUNK);
+        const double fold = shares > 1 ? 3.0 + (double)shares * rows * width * 8 / 4e6 : 0.0;
+        const double t = waves * looks + fold;
+        if (shares == 1 || t < least) least = t, N.shares = shares, N.share = share;
+    }
+    N.shares = (tokens + N.share - 1) / N.share;
+    return true;
 }
 
 // ---------------------------------------------------------------- host
@@ -884,6 +1101,14 @@ static void (*emb_forward_kernel(int vec, bool one))(EmbArgs) {
 }
 
 enum { EMB_SORT = 0, EMB_WARP = 1, EMB_BLOCK = 2, EMB_TABLE = 3 };
+template <typename T>
+static void (*emb_narrow_kernel(int vec))(EmbGradArgs, EmbNarrow) {
+    if constexpr (sizeof(T) == 2) {
+        if (vec == 8) return embedding_backward_narrow_kernel<T, 8>;
+    }
+    return vec == 4 ? embedding_backward_narrow_kernel<T, 4> : vec == 2 ? embedding_backward_narrow_kernel<T, 2>
+                                                                        : embedding_backward_narrow_kernel<T, 1>;
+}
 template <typename T, int VEC>
 static void (*emb_backward_of(int path))(EmbGradArgs) {
     if (path == EMB_WARP) return embedding_backward_warp_kernel<T, VEC>;
@@ -969,7 +1194,10 @@ static EmbLayout emb_layout(int64_t tokens, int64_t width, int grid_max) {
     const int64_t sums = (by_tokens < by_threads ? by_tokens : by_threads) * 2;
     // a table of sums per block, grid_max / (column tiles of at most 128 columns) blocks or one
     const int64_t tables = EMB_TABLE_ROWS * ((int64_t)grid_max * 128 + width);
-    L.parts = at, at += up((sums > tables ? sums : tables) * 4);
+    // and a block's sums of narrow rows for at most grid_max blocks, where the tokens go to several shares
+    const int64_t narrow = tokens >= 2 * EMB_NARROW_SHARE ? grid_max * (int64_t)EMB_NARROW_FLOATS : 0;
+    const int64_t most = sums > tables ? sums : tables;
+    L.parts = at, at += up((most > narrow ? most : narrow) * 4);
     L.bytes = at;
     return L;
 }
@@ -1062,7 +1290,8 @@ int pbg_embedding_backward(int64_t tokens, int64_t rows, int64_t width, const vo
     const int64_t column_tiles = (width + 32 * vec - 1) / (32 * vec);
     if (tokens <= EMB_SCAN_WARP) {
         const int64_t need = (rows + 7) / 8, most = (int64_t)sm_count() * 8;
-        of(vec, EMB_WARP)<<<(unsigned)(need < most ? need : most), 256, 0, s>>>(E);
+        const int64_t x = need < most ? need : most, y = most / x < column_tiles ? most / x : column_tiles;
+        of(vec, EMB_WARP)<<<dim3((unsigned)x, (unsigned)y), 256, 0, s>>>(E);
         return launch_status("embedding_backward");
     }
     // a block per row and column tile: up to a few of them per SM at once
@@ -1100,6 +1329,29 @@ int pbg_embedding_backward(int64_t tokens, int64_t rows, int64_t width, const vo
             embedding_backward_fold_kernel<<<(unsigned)((rows * width + 31) / 32), EMB_THREADS, 0, s>>>(E, (int)blocks);
             return launch_status("embedding_backward: fold");
         }
+    }
+    EmbNarrow N;
+    if (emb_narrow_plan(tokens, rows, width, grid_max, N)) {
+        auto narrow = grad_type == EMB_F32 ? emb_narrow_kernel<float>(vec)
+                      : grad_type == EMB_BF16 ? emb_narrow_kernel<__nv_bfloat16>(vec) : emb_narrow_kernel<__half>(vec);
+        static int configured[64][3][4] = {};
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const int vi = vec == 8 ? 3 : vec == 4 ? 2 : vec - 1;
+        if (dev < 0 || dev >= 64 || !configured[dev][grad_type][vi]) {
+            const int rc = cuda_status(cudaFuncSetAttribute(narrow, cudaFuncAttributeMaxDynamicSharedMemorySize, EMB_NARROW_SMEM),
+                                       "embedding_backward: shared memory size");
+            if (rc) return rc;
+            if (dev >= 0 && dev < 64) configured[dev][grad_type][vi] = 1;
+        }
+        narrow<<<dim3((unsigned)N.shares, (unsigned)N.ranges, (unsigned)N.tiles), EMB_THREADS, EMB_NARROW_SMEM, s>>>(E, N);
+        const int rc = launch_status("embedding_backward");
+        if (rc || N.shares == 1) return rc;
+        if (N.shares <= EMB_FOLD_FEW)
+            embedding_backward_fold_few_kernel<<<(unsigned)((rows * width + 255) / 256), 256, 0, s>>>(E, (int)N.shares);
+        else
+            embedding_backward_fold_kernel<<<(unsigned)((rows * width + 31) / 32), EMB_THREADS, 0, s>>>(E, (int)N.shares);
+        return launch_status("embedding_backward: fold");
     }
     auto kernel = of(vec, EMB_SORT);
     if (grid == 1) {

@@ -88,6 +88,32 @@ CASES = [
     (9000, 40, 4102, BF16, F32, "zipf"),      # 65 column tiles of a kept table, odd pairs
     (5000, 1, 130, F16, BF16, "one"),
     (20011, 21, 100, BF16, F32, "half"),
+    # rows in ranges of 22,528 sums, columns by 16, tokens in shares of 1,024 or more
+    (300, 1408, 16, F32, F32, "zipf"),        # one range of rows, one share
+    (2047, 1409, 16, F16, F16, "uniform"),    # two ranges; the last size of one share
+    (2048, 1409, 16, BF16, F32, "half"),      # two shares
+    (2049, 22529, 1, F32, F32, "zipf"),
+    (150001, 363, 1, BF16, BF16, "uniform"),
+    (97299, 3549, 8, BF16, BF16, "zipf"),
+    (60001, 1, 15, F32, F32, "one"),          # one warp's row
+    (30000, 17, 17, F32, BF16, "zipf"),       # a column tile of one column
+    (19180, 329, 57, BF16, F32, "uniform"),
+    (40000, 120730, 13, BF16, F32, "zipf"),
+    (5000, 2, 24, F16, F32, "half"),
+    (5000, 2000, 57, F32, BF16, "half"),      # four column tiles, the last of nine columns
+    (300000, 4000, 7, BF16, F32, "zipf"),
+    (30000, 1024, 16, F32, F32, "one"),
+    # few rows of many columns
+    (169, 4, 1752, F16, F16, "uniform"),
+    (256, 1, 9000, F32, F32, "one"),
+    (3, 700, 5000, BF16, F32, "uniform"),
+    # sorted tokens
+    (1500, 200003, 700, BF16, F32, "half"),   # in one block
+    (300007, 3000, 300, BF16, F32, "half"),
+    (400000, 90001, 8, F32, F32, "zipf"),
+    (1000000, 700000, 4, F16, F32, "uniform"),
+    (70000, 3000, 1000, F32, F32, "one"),
+    (70001, 400, 1500, BF16, BF16, "zipf"),
 ]
 
 
