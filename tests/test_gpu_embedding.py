@@ -67,7 +67,7 @@ CASES = [
     (5000, 511, 65, F32, F32, "zipf"),        # 9 key bits: one pass
     (5000, 512, 66, BF16, BF16, "zipf"),      # 10 key bits: two passes, 4-byte vectors
     (20000, 70001, 36, BF16, F32, "zipf"),    # 17 bits; 8-byte vectors
-    (3000, 300000, 8, F32, F32, "uniform"),   # 19 bits: three passes; the table zeroed first
+    (3000, 300000, 8, F32, F32, "uniform"),   # 120 ranges of rows
     (65537, 1000, 100, F32, F32, "half"),
     (81920, 13, 128, F32, F32, "uniform"),
     (150001, 4, 17, F16, F32, "uniform"),
@@ -81,7 +81,7 @@ CASES = [
     (200, 100003, 12, F16, F32, "half"),
     (4096, 1000, 64, BF16, F32, "half"),      # the last size that is not sorted
     (4096, 3, 2000, F32, F16, "one"),
-    (1000, 5000, 64, F32, F32, "zipf"),       # few tokens, but rows for the sort
+    (1000, 5000, 64, F32, F32, "zipf"),       # few tokens, but too many rows for a block each
     (5000, 52, 32, F32, F32, "uniform"),      # the largest table that is kept whole, the smallest width
     (5000, 53, 32, F32, F32, "uniform"),
     (5000, 52, 31, F32, F32, "uniform"),
@@ -111,7 +111,7 @@ CASES = [
     (1500, 200003, 700, BF16, F32, "half"),   # in one block
     (300007, 3000, 300, BF16, F32, "half"),
     (400000, 90001, 8, F32, F32, "zipf"),
-    (1000000, 700000, 4, F16, F32, "uniform"),
+    (1000000, 700000, 4, F16, F32, "uniform"),  # 20 bits: three passes
     (70000, 3000, 1000, F32, F32, "one"),
     (70001, 400, 1500, BF16, BF16, "zipf"),
 ]
