@@ -201,15 +201,24 @@ __device__ __forceinline__ void or_commit(uint32_t bar) {
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// Arrival at the pair's first block's barrier.  Relaxed: the arriving thread has written nothing that the
-// other block reads (it has seen its own block's copies land, or taken its accumulators' columns), and a
-// release at cluster scope here costs as long as a k-block's products.
+// Arrival at the pair's first block's barrier.  RELEASE: what the arriving thread has seen (its own block's copies
+// landing in shared memory) is ordered before what the first block does after its wait.  Relaxed is for
+// accumulators' columns that have been read: tcgen05.wait::ld and tcgen05.fence::before_thread_sync before the
+// arrival, and fence::after_thread_sync after the wait, order tensor-memory accesses across a relaxed arrival.
+template <bool RELEASE>
 __device__ __forceinline__ void or_arrive_first(uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .b32 a;\n\t"
-        "mapa.shared::cluster.u32 a, %0, 0;\n\t"
-        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
-        : "memory");
+    if constexpr (RELEASE)
+        asm volatile(
+            "{\n\t.reg .b32 a;\n\t"
+            "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+            "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .b32 a;\n\t"
+            "mapa.shared::cluster.u32 a, %0, 0;\n\t"
+            "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar)
+            : "memory");
 }
 // a wait for arrivals of the other block too
 __device__ __forceinline__ bool or_try_wait_cluster(uint32_t bar, uint32_t parity) {
@@ -971,7 +980,7 @@ __device__ __forceinline__ void or_relay(const OrthoArgs& O, OrthoShared& S, int
                 break;
             }
             pipe ^= 1u << s;
-            or_arrive_first(peer0 + 8 * s);
+            or_arrive_first<true>(peer0 + 8 * s);
             if (++s == G.stages) s = 0;
         }
     }
@@ -1050,7 +1059,7 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
             or_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if (PAIR) or_arrive_first(acc_empty0 + 8 * b);
+                if (PAIR) or_arrive_first<false>(acc_empty0 + 8 * b);
                 else or_arrive(acc_empty0 + 8 * b);
             }
         }
