@@ -20,14 +20,12 @@
 //
 // Precision.  16-bit operands alone are not enough: an error in X in the direction of a small singular
 // value grows by a = 3.4 each step, so X is carried as a pair of fp16 numbers hi + lo of 2^14 X (22
-// significant bits; every |x| <= sigma_max <= 2 keeps hi in range).  With fp32 output, and in the
-// optimizer's transition, A and B are pairs too (2^13 A, 2^12 B) and each product takes three passes,
-// hi hi + hi lo + lo hi, leaving errors of about 2^-22: at or below what fp32 operands give.  With bf16
-// output of matrices whose short side is at least ORTHO_SINGLE the symmetric matrices are single fp16
-// numbers (error 2^-12 that does not grow: about 8e-4 of the result's norm, where bf16 rounding alone is
-// 1.7e-3): one pass for A and B, two for X'.  The tensor cores truncate as they accumulate, a bias that
-// grows with the length of the sum (sums of 256 terms in three passes left 1.4e-5 of the result at
-// 256 x 1024), so with pairs a sum is taken from tensor memory every 64 terms, the small products first,
+// significant bits; every |x| <= sigma_max <= 2 keeps hi in range).  A and B are pairs too (2^13 A, 2^12 B)
+// and each product takes three passes, hi hi + hi lo + lo hi, leaving errors of about 2^-22.  (Single fp16
+// numbers for A and B where the output is bf16 took 1.85 ms at 4,096 x 4,096, but added up to as much error as
+// the output's own rounding: 1.6e-3 of a noise matrix of 4,096 x 512.)  The tensor cores truncate as they
+// accumulate, a bias that grows with the length of the sum (sums of 256 terms in three passes left 1.4e-5 of
+// the result at 256 x 1024), so a sum is taken from tensor memory every 64 terms, the small products first,
 // and added up in fp32 registers.
 //
 // Layout.  X, A and B live in the workspace as 128 x 64 tiles of 16 KB, hi then lo, already in the
@@ -90,7 +88,7 @@ struct OrthoArgs {
     int bn_sym, bn_upd;  // output tile widths
     int pair;            // output tiles of 256 rows, by two blocks each
     int mirror;          // of A and B only what is on and above the diagonal is computed
-    int steps, precise;  // precise: A and B as pairs
+    int steps;
     float a, b, c;
     double eps;
     // orthogonalize
@@ -568,11 +566,11 @@ __device__ __forceinline__ OrthoPlace or_place(const OrthoArgs& O, const OrthoDe
 // A thread's 64 finished values of one row as a row of a 128 x 64 tile, hi then lo, by way of the warp's
 // staging block of 32 rows (rows of 128 bytes are contiguous in the tile, so each part is one bulk copy); lo
 // has a block of its own where the warp of the other column part has no columns (`spare`).
-__device__ __forceinline__ void or_store_rows(uint32_t blk, uint32_t spare, unsigned char* dst, int lane, float* v, int parts) {
+__device__ __forceinline__ void or_store_rows(uint32_t blk, uint32_t spare, unsigned char* dst, int lane, float* v) {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
 #pragma unroll 1
-    for (int low = 0; low < parts; ++low) {
+    for (int low = 0; low < 2; ++low) {
         const uint32_t at = low && spare ? spare : blk;
         if (low && !spare) {
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -719,7 +717,6 @@ __device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int
 }
 
 // what an epilogue warp does with its 32 rows x 64 columns (rows row - lane ..., column block cb of 64)
-template <bool PRECISE>
 __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step, int which, int i, int row, int cb,
                                           uint32_t blk, uint32_t spare, int lane, float* v) {
     const OrthoPlace L = or_place(O, or_get(O, which), step);
@@ -728,7 +725,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
 #pragma unroll
         for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
         unsigned char* tile = L.x_next + i * L.x_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
-        or_store_rows(blk, spare, tile, lane, v, 2);
+        or_store_rows(blk, spare, tile, lane, v);
         return;
     }
     if (O.mirror && (cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
@@ -739,7 +736,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
 #pragma unroll
     for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == cb * 64 + j ? diagonal : 0.0f);
     unsigned char* tile = dst + i * L.a_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
-    or_store_rows(blk, spare, tile, lane, v, PRECISE ? 2 : 1);
+    or_store_rows(blk, spare, tile, lane, v);
     if (O.mirror && cb * 64 >= (i + 1) * 128) {
         // the mirrored place of (row, cb * 64 + j): row block cb / 2, column block row / 64, row (cb & 1) * 64 + j
         // of that tile; lanes are neighbours
@@ -753,7 +750,7 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
                 __half hi, lo;
                 or_split(v[8 * q + j], hi, lo);
                 *reinterpret_cast<__half*>(at + q * 1024) = hi;
-                if (PRECISE) *reinterpret_cast<__half*>(at + q * 1024 + 16384) = lo;
+                *reinterpret_cast<__half*>(at + q * 1024 + 16384) = lo;
             }
         }
     }
@@ -786,20 +783,17 @@ __device__ __forceinline__ bool or_phase_end(const OrthoArgs& O, OrthoShared& S,
     return *reinterpret_cast<volatile int*>(&S.ok) != 0;
 }
 
-// The operand stages of a kind of product: the row operand's tile (hi, or hi and lo), then up to three (of a
-// pair, two: half of the columns) 64-wide pieces of the other operand, hi parts and lo parts.
+// The operand stages of a kind of product: the row operand's tile, hi and lo, then up to four (of a pair, two:
+// half of the columns) 64-wide pieces of the other operand, hi parts and lo parts.
 struct OrthoStage {
-    int pa, pb, stages;
-    uint32_t a_bytes, b_part, bytes;
+    int stages;
+    uint32_t b_part, bytes;
 };
-template <bool PRECISE, bool PAIR>
-__device__ __forceinline__ OrthoStage or_stage(int kind, int bn) {
+template <bool PAIR>
+__device__ __forceinline__ OrthoStage or_stage(int bn) {
     OrthoStage G;
-    G.pa = PRECISE ? 2 : 1;
-    G.pb = PRECISE || kind == OR_UPDATE ? 2 : 1;
-    G.a_bytes = G.pa * 16384u;
     G.b_part = (uint32_t)(PAIR ? bn / 2 : bn) * 128u;
-    G.bytes = G.a_bytes + G.pb * G.b_part;
+    G.bytes = ORTHO_TILE + 2 * G.b_part;
     G.stages = min(ORTHO_STAGES, (int)(ORTHO_RING / G.bytes));
     return G;
 }
@@ -808,14 +802,14 @@ __device__ __forceinline__ OrthoStage or_stage(int kind, int bn) {
 // products take less time than an accumulator's way to the registers), else two.
 __device__ __forceinline__ uint32_t or_buffers(const OrthoArgs& O) { return max(O.bn_sym, O.bn_upd) <= 128 ? 2u : 1u; }
 
-// A producer warp's elected lane, one phase.  A stage is copy 0, the row operand, and copies 1 .. 6, a 64-row
-// or 64-column piece of the other operand each, hi and lo; the producer warps take them in turn.  `pipe`:
+// A producer warp's elected lane, one phase.  A stage is copy 0, the row operand, and copies 1 .. 8 at most, a
+// 64-row or 64-column piece of the other operand each, hi or lo; the producer warps take them in turn.  `pipe`:
 // parity of each stage's next use, a bit a stage, kept from phase to phase.
-template <bool PRECISE, bool PAIR, bool SPLIT>
+template <bool PAIR, bool SPLIT>
 __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int rank,
                                            int producer, uint32_t& pipe) {
     const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
-    const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const OrthoStage G = or_stage<PAIR>(kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
     bool ok = true;
     int s = 0;
@@ -836,11 +830,11 @@ __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, u
             if (copy == 0) {
                 src[q] = kind == OR_GRAM ? L.x + T.i * L.x_row : kind == OR_SQUARE ? L.a + T.i * L.a_row : L.b + T.i * L.a_row;
                 if (kind == OR_SQUARE && O.c == 0.0f) src[q] += (int64_t)(T.c0 >> 6) * ORTHO_TILE;
-                dst[q] = 0, bytes[q] = G.a_bytes;
+                dst[q] = 0, bytes[q] = ORTHO_TILE;
             } else {
-                const int piece = (copy - 1) >> (G.pb - 1), part = (copy - 1) & (G.pb - 1);
+                const int piece = (copy - 1) >> 1, part = (copy - 1) & 1;
                 const int cb = (T.c0 >> 6) + (PAIR ? rank * pieces : 0) + piece;
-                dst[q] = G.a_bytes + part * G.b_part + piece * 8192u;
+                dst[q] = ORTHO_TILE + part * G.b_part + piece * 8192u;
                 bytes[q] = piece < pieces ? 8192u : 0u;
                 if (kind == OR_UPDATE) src[q] = L.x + (int64_t)cb * ORTHO_TILE + part * 16384;  // 64 k-rows of column block cb
                 else src[q] = (kind == OR_GRAM ? L.x + (cb >> 1) * L.x_row : L.a + (cb >> 1) * L.a_row) + (cb & 1) * 8192 + part * 16384;
@@ -879,16 +873,16 @@ __device__ __forceinline__ void or_produce(const OrthoArgs& O, OrthoShared& S, u
 }
 
 // The issuing warp's elected lane (of a pair's first block), one phase.  `acc` counts accumulators used.
-template <bool PRECISE, bool PAIR, bool SPLIT>
+template <bool PAIR, bool SPLIT>
 __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, uint32_t& pipe,
                                          uint32_t& acc) {
     const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
-    const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const OrthoStage G = or_stage<PAIR>(kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), empty0 = or_smem(&S.empty[0]);
     const uint32_t peer0 = or_smem(&S.peer[0]);
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
     const bool linear = kind == OR_SQUARE && O.c == 0.0f;
-    const int chunk = PRECISE && !linear ? 1 : 1 << 20;
+    const int chunk = linear ? 1 << 20 : 1;
     const int mn = kind == OR_UPDATE;
     const uint32_t b_step = mn ? 2048u >> 4 : 32u >> 4, lbo = mn ? 8192u : 16u;
     const uint32_t eye = or_desc(ring + ORTHO_RING + ORTHO_STAGING, 16), eye_idesc = or_idesc<PAIR>(16, 0);
@@ -918,27 +912,22 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
                 pipe ^= 1u << s;
                 or_fence_after();
                 const uint32_t a = or_desc(ring + s * G.bytes, 16), al = a + (16384u >> 4);
-                const uint32_t bh = or_desc(ring + s * G.bytes + G.a_bytes, lbo), bl = bh + (G.b_part >> 4);
+                const uint32_t bh = or_desc(ring + s * G.bytes + ORTHO_TILE, lbo), bl = bh + (G.b_part >> 4);
                 if (linear) {
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) {
                         const uint32_t dd = d + (uint32_t)kb * 64u + ks * 16;
-                        if (PRECISE) or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 0u);
-                        or_mma<PAIR>(dd, a + ks * 2, eye, eye_idesc, PRECISE);
+                        or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 0u);
+                        or_mma<PAIR>(dd, a + ks * 2, eye, eye_idesc, 1u);
                     }
                 } else {
                     // the small products first: they are added to a small sum
-                    uint32_t more = kb > k0;
-                    if (PRECISE) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma<PAIR>(d, al + ks * 2, bh + ks * b_step, idesc, more);
-                    }
-                    if (G.pb == 2) {
+                    for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(d, al + ks * 2, bh + ks * b_step, idesc, ks > 0);
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma<PAIR>(d, a + ks * 2, bl + ks * b_step, idesc, more);
-                    }
+                    for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(d, a + ks * 2, bl + ks * b_step, idesc, 1u);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks, more = 1u) or_mma<PAIR>(d, a + ks * 2, bh + ks * b_step, idesc, more);
+                    for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(d, a + ks * 2, bh + ks * b_step, idesc, 1u);
                     if (kb >= eye0 && kb < eye1) {
                         // c A A + b A = c (A A + A (b / c) I): this k-block's columns once more, 16 at a time,
                         // against a scaled identity
@@ -947,7 +936,7 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
                             const uint32_t dd = d + (uint32_t)(kb - eye0) * 64u + ks * 16;
                             or_mma<PAIR>(dd, a + ks * 2, eye, eye_idesc, 1u);
                             or_mma<PAIR>(dd, a + ks * 2, eye + 2, eye_idesc, 1u);
-                            if (PRECISE) or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 1u);
+                            or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 1u);
                         }
                     }
                 }
@@ -964,11 +953,10 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
 }
 
 // The same warp of a pair's second block: tells the first when a stage's copies have landed here.
-template <bool PRECISE>
 __device__ __forceinline__ void or_relay(const OrthoArgs& O, OrthoShared& S, int kind, uint32_t& pipe) {
     constexpr bool PAIR = true, SPLIT = false;
     const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
-    const OrthoStage G = or_stage<PRECISE, PAIR>(kind, kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
+    const OrthoStage G = or_stage<PAIR>(kind == OR_UPDATE ? O.bn_upd : O.bn_sym);
     const uint32_t full0 = or_smem(&S.full[0]), peer0 = or_smem(&S.peer[0]);
     bool ok = true;
     int s = 0;
@@ -1022,14 +1010,14 @@ __device__ __forceinline__ bool or_join(const OrthoArgs& O, const OrthoTile& T, 
 
 // An epilogue warp, one phase: a quarter of the rows, one or (tiles wider than 128) two groups of 64
 // columns of each tile.
-template <bool PRECISE, bool PAIR, bool SPLIT>
+template <bool PAIR, bool SPLIT>
 __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, uint32_t ring, int kind, int step, int rank, int e,
                                            uint32_t& acc) {
     const int lane = threadIdx.x & 31, quad = (threadIdx.x >> 5) & 3, part = e >> 2;
     const int64_t tiles = SPLIT && kind == OR_GRAM ? O.grams : kind != OR_UPDATE ? O.syms : O.upds;
     const int bn = kind == OR_UPDATE ? O.bn_upd : O.bn_sym;
     const uint32_t acc_full0 = or_smem(&S.acc_full[0]), acc_empty0 = or_smem(&S.acc_empty[0]);
-    const int chunk = PRECISE && !(kind == OR_SQUARE && O.c == 0.0f) ? 1 : 1 << 20;
+    const int chunk = kind == OR_SQUARE && O.c == 0.0f ? 1 << 20 : 1;
     const uint32_t shift = or_buffers(O), buffers = 1u << shift;
     const int group0 = bn > 128 ? 2 * part : part;
     const uint32_t blk = ring + ORTHO_RING + (uint32_t)e * ORTHO_BLOCK;
@@ -1075,7 +1063,7 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
             const int cb = (T.c0 >> 6) + group0 + g;
             if (!ok || g >= groups || (PAIR && (cb >= last_cb || T.i >= or_mb(m)))) continue;
             if (kind == OR_UPDATE && step == O.steps - 1) or_finish_out(O, T.which, row, cb, blk, lane, v + 64 * g);
-            else or_finish<PRECISE>(O, kind, step, T.which, T.i, row, cb, blk, spare, lane, v + 64 * g);
+            else or_finish(O, kind, step, T.which, T.i, row, cb, blk, spare, lane, v + 64 * g);
         }
     }
     if (!ok) {
@@ -1091,7 +1079,7 @@ __device__ __forceinline__ void or_collect(const OrthoArgs& O, OrthoShared& S, u
 // matrices, each role running through the phases on its own.  PAIR: launched in clusters of two blocks, which
 // work on tiles of 256 rows together (a block's own row block, half of the columns' operand each, the first
 // block issuing), a third fewer bytes to fetch per product.
-template <bool PRECISE, bool PAIR, bool SPLIT>
+template <bool PAIR, bool SPLIT>
 __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const __grid_constant__ OrthoArgs O) {
     // the first kilobyte holds the barriers; the ring after it starts on the 1024 bytes of a swizzle atom
     extern __shared__ __align__(1024) unsigned char or_raw[];
@@ -1155,21 +1143,21 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
     if (warp == 0) {
         for (int p = 0; p < phases; ++p) {
             if (or_elect()) {
-                if (PAIR && rank) or_relay<PRECISE>(O, S, p % 3, pipe);
-                else or_issue<PRECISE, PAIR, SPLIT>(O, S, ring, p % 3, pipe, acc);
+                if (PAIR && rank) or_relay(O, S, p % 3, pipe);
+                else or_issue<PAIR, SPLIT>(O, S, ring, p % 3, pipe, acc);
             }
             __syncwarp();
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     } else if (warp <= ORTHO_PRODUCERS) {
         for (int p = 0; p < phases; ++p) {
-            if (or_elect()) or_produce<PRECISE, PAIR, SPLIT>(O, S, ring, p % 3, p / 3, rank, warp - 1, pipe);
+            if (or_elect()) or_produce<PAIR, SPLIT>(O, S, ring, p % 3, p / 3, rank, warp - 1, pipe);
             __syncwarp();
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     } else {
         for (int p = 0; p < phases; ++p) {
-            or_collect<PRECISE, PAIR, SPLIT>(O, S, ring, p % 3, p / 3, rank, warp - 1 - ORTHO_PRODUCERS, acc);
+            or_collect<PAIR, SPLIT>(O, S, ring, p % 3, p / 3, rank, warp - 1 - ORTHO_PRODUCERS, acc);
             if (p + 1 < phases && !or_phase_end(O, S, p + 1)) break;
         }
     }
@@ -1568,7 +1556,6 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
 // ------------------------------------------------------------ host
 
 constexpr int64_t ORTHO_BUDGET = 1ll << 30;  // bytes of tiles that one launch works in, where a matrix alone does not need more
-constexpr int ORTHO_SINGLE = 512;
 
 // blocks of a matrix's team, 0 where it takes the general path
 static int or_team(int m, int n) {
@@ -1726,17 +1713,15 @@ static int or_teams(const OrthoArgs& O, int cluster, cudaStream_t s) {
 
 // conversion, then the products
 static int or_products(const OrthoArgs& O, int64_t arrived_bytes, cudaStream_t s) {
-    const void* const kernels[6] = {
-        (const void*)orthogonalize_kernel<false, false, false>, (const void*)orthogonalize_kernel<true, false, false>,
-        (const void*)orthogonalize_kernel<false, true, false>,  (const void*)orthogonalize_kernel<true, true, false>,
-        (const void*)orthogonalize_kernel<false, false, true>,  (const void*)orthogonalize_kernel<true, false, true>};
+    const void* const kernels[3] = {(const void*)orthogonalize_kernel<false, false>, (const void*)orthogonalize_kernel<true, false>,
+                                    (const void*)orthogonalize_kernel<false, true>};
     static int pairs_at_once[64] = {0};  // pairs of blocks that the device runs at once, from the first call on
     int dev = 0, rc = 0;
     rc = cuda_status(cudaGetDevice(&dev), "orthogonalize: device");
     if (rc) return rc;
     PBG_REQUIRE(dev < 64, "orthogonalize: at most 64 devices");
     if (!pairs_at_once[dev]) {
-        for (int i = 0; i < 6; ++i) {
+        for (int i = 0; i < 3; ++i) {
             rc = cuda_status(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, ORTHO_SMEM),
                              "orthogonalize: shared memory size");
             if (rc) return rc;
@@ -1750,7 +1735,7 @@ static int or_products(const OrthoArgs& O, int64_t arrived_bytes, cudaStream_t s
         cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
         config.attrs = cluster, config.numAttrs = 1;
         int pairs = 0;
-        rc = cuda_status(cudaOccupancyMaxActiveClusters(&pairs, kernels[3], &config), "orthogonalize: pairs of blocks");
+        rc = cuda_status(cudaOccupancyMaxActiveClusters(&pairs, kernels[1], &config), "orthogonalize: pairs of blocks");
         if (rc) return rc;
         PBG_REQUIRE(pairs >= 1, "orthogonalize: the device runs no pair of blocks");
         pairs_at_once[dev] = pairs;
@@ -1781,7 +1766,7 @@ static int or_products(const OrthoArgs& O, int64_t arrived_bytes, cudaStream_t s
     config.attrs = attribute;
     config.numAttrs = O.pair ? 2 : 1;
     void* args[] = {const_cast<OrthoArgs*>(&O)};
-    return cuda_status(cudaLaunchKernelExC(&config, kernels[(O.pair ? 2 : O.grams > O.syms ? 4 : 0) + (O.precise ? 1 : 0)], args),
+    return cuda_status(cudaLaunchKernelExC(&config, kernels[O.pair ? 1 : O.grams > O.syms ? 2 : 0], args),
                        "orthogonalize: cooperative launch");
 }
 
@@ -1875,7 +1860,6 @@ int pbg_orthogonalize(int64_t batch, int64_t rows, int64_t cols, const void* x, 
     O.one_src = rows * cols;
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
     O.x_type = x_type, O.out_type = out_type, O.error = error;
-    O.precise = !(out_type == 1 && m >= ORTHO_SINGLE);
     if (O.one.team) {
         PBG_REQUIRE(workspace_bytes >= 1024, "orthogonalize: workspace too small");
         O.count = batch, O.slots = batch * O.one.team;
@@ -2002,7 +1986,6 @@ int pbg_muon_step(int64_t count, const void* descriptors, const int64_t* plan, f
     O.tiles = w + or_up(or_parts_bytes(most_items, shape));
     O.bn_sym = (int)plan[3], O.bn_upd = (int)plan[4], O.pair = (int)plan[5] & 1, O.mirror = (int)plan[5] >> 1;
     O.steps = steps, O.a = a, O.b = b, O.c = c, O.eps = eps;
-    O.precise = 1;
     O.grad = grad, O.momentum = momentum, O.master = master, O.controls = controls;
     O.nesterov = nesterov, O.bad = skipped, O.error = error;
     O.aligned = (uintptr_t)grad % 16 == 0 && (uintptr_t)momentum % 16 == 0 && (uintptr_t)master % 16 == 0;

@@ -84,9 +84,8 @@ def orthogonalize(x: Tensor, *, steps: int = 5, coefficients: tuple[float, float
     steps: ``X / (|X|_F + epsilon)``, then ``X <- a X + (b G + c G^2) X`` with ``G = X X^T`` on the short side.
 
     The output has ``x``'s shape and ``out_dtype`` (``x``'s by default), or goes to ``out`` (contiguous; it
-    may be ``x`` itself).  fp32 and fp16 outputs carry fp32 accuracy; bf16 outputs of matrices whose short
-    side is 512 or more are computed to about half of their rounding.  A matrix of zeros gives zeros, one
-    with a NaN or an infinity gives NaN."""
+    may be ``x`` itself).  Products carry fp32 accuracy whatever the types; the result is rounded
+    once.  A matrix of zeros gives zeros, one with a NaN or an infinity gives NaN."""
 
     if x.ndim < 2 or x.dtype not in _TYPES:
         raise NativeError("orthogonalize takes float32, bfloat16 or float16 matrices [..., rows, cols]")

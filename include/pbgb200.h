@@ -448,9 +448,8 @@ int pbg_adam_step(int64_t n, float *master, float *grad, float *first, float *se
 
 /* Orthogonalises `batch` contiguous matrices [rows, cols]: X / (|X|_F + eps), then `steps` times
  * X <- a X + (b G + c G^2) X with G = X X^T on the short side; out contiguous like x.  Types 0 fp32, 1 bf16,
- * 2 fp16.  fp32 accuracy inside (fp16 pairs on the tensor cores), but for bf16 output of matrices whose
- * short side is 512 or more (errors of about half the output's rounding).  Coefficients that would let a
- * singular value grow past 2 are refused; sides up to 65,536.  workspace: 256-byte aligned device memory
+ * 2 fp16.  fp32 accuracy inside (fp16 pairs on the tensor cores), one rounding to the output's type.
+ * Coefficients that would let a singular value grow past 2 are refused; sides up to 65,536.  workspace: 256-byte aligned device memory
  * of pbg_orthogonalize_workspace bytes, any contents, one per call in flight.  error (device uint32,
  * sticky): non-zero when a bounded wait gave up. */
 int64_t pbg_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);

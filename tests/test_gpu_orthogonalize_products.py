@@ -25,3 +25,17 @@ def test_pairs_of_blocks_give_the_same_bits(m, n, dtype):
         assert bool(other.isfinite().all())
         assert torch.equal(got, orthogonalize(x))
     assert orthogonalize_error(DEV) == 0
+
+
+@pytest.mark.parametrize("m,n,kind", [(4096, 512, "noise"), (1024, 640, "noise"), (1536, 2048, "noise"), (513, 700, "steep"),
+                                      (520, 8000, "noise"), (4096, 4096, "low")])
+def test_bf16_outputs_are_fp32_results_rounded_once(m, n, kind):
+    """The error is the rounding's own, and what fp32 accuracy may add: FP32_BAR of the result; the rounding of
+    so slightly other values is another sample of the same million roundings and more, taken as 1 % apart."""
+    from pbg_b200.optim import orthogonalize, orthogonalize_error
+
+    x = _matrix(kind, m, n, torch.Generator(device=DEV).manual_seed(m + 3 * n)).bfloat16()
+    ref = _reference(x)
+    assert _off(orthogonalize(x), ref) <= 1.01 * _off(ref.bfloat16(), ref) + FP32_BAR
+    assert _off(orthogonalize(x, out_dtype=F16), ref) <= BAR[F16]
+    assert orthogonalize_error(DEV) == 0
