@@ -51,18 +51,20 @@ constexpr int ORTHO_THREADS = 32 * (1 + ORTHO_PRODUCERS + ORTHO_EPI_WARPS);  // 
 constexpr int ORTHO_RING = 192 * 1024;  // operand stages
 constexpr int ORTHO_STAGES = 8;         // at most
 constexpr int ORTHO_BLOCK = 4096;       // an epilogue warp's staging block
-constexpr int ORTHO_EYE = 2048;         // 16 rows of 128 bytes: (b / c) 2^13 I in fp16 (2^13 I where c is 0), hi, and lo 32 bytes on
+constexpr int ORTHO_EYE = 2048;         // 16 rows of 128 bytes: (b / c) 2^13 I (2^13 I where c is 0) as three fp16 numbers, 32 bytes apart
 constexpr int ORTHO_STAGING = ORTHO_EPI_WARPS * ORTHO_BLOCK;
 constexpr int ORTHO_SMEM = 1024 + ORTHO_RING + ORTHO_STAGING + ORTHO_EYE;
 constexpr int ORTHO_FLAT = 256;         // threads of the kernels around the products
 constexpr int ORTHO_SPAN = ORTHO_FLAT * 16;  // elements whose squares one block sums
 constexpr int ORTHO_TILE = 32768;       // bytes of a 128 x 64 tile, hi and lo
 constexpr uint32_t ORTHO_WAIT_TRIES = 1u << 24;
-// What truncation takes from the sums on average, given back where they are scaled: from the update's
-// 2^-22 of the result; the polynomial's, where the positive square loses against the negative multiple of A,
-// come out 2^-22 too large.  Measured: 2.0e-6 of the result instead of 3.3e-6 at 256 x 1,024, 1.8e-6 instead
-// of 3.1e-6 at 384 x 128 (fp32 operands: 2.1e-6 and 1.6e-6).
-constexpr float ORTHO_UPDATE_BACK = 1.0f + 0x1p-22f, ORTHO_SQUARE_BACK = 1.0f - 0x1p-22f;
+// What the tensor cores take, on average, from sums whose large terms are positive (X X^T and A A), given back
+// where the sums are scaled: each 16 terms truncate the running sum, so by 64 terms a Gram matrix comes out about
+// 4 x 2^-24 of itself too small, by 16 or 32 terms 2 to 3 (measured on 1 to 1,536 rows of 7 to 4,096 columns).
+// Five steps of 26 sizes and three spectra are then off by 0.02e-6 to 3.1e-6 of the result, 0.77 times what fp32
+// products are on (geometric) average and 1.7 at most (33 x 2,000 of noise); with nothing given back by up to 3.6e-6.
+constexpr float ORTHO_BACK_LONG = 1.0f + 0x1p-22f, ORTHO_BACK_SHORT = 1.0f + 0x1p-23f;
+__device__ __forceinline__ float or_back(int terms) { return terms > 32 ? ORTHO_BACK_LONG : ORTHO_BACK_SHORT; }
 constexpr float ORTHO_SX = 16384.0f, ORTHO_SA = 8192.0f, ORTHO_SB = 4096.0f;
 
 struct OrthoDesc {
@@ -629,7 +631,7 @@ __device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int
         k.shrink = 1.0f - k.lr * O.controls[2];
         k.lr *= d.adjust;
     }
-    const float scale = ORTHO_UPDATE_BACK / (ORTHO_SB * ORTHO_SX);
+    const float scale = 1.0f / (ORTHO_SB * ORTHO_SX);
     const bool vector = d.n % 4 == 0 && d.src % 4 == 0 && O.aligned;
     if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
@@ -716,6 +718,11 @@ __device__ __forceinline__ void or_finish_out(const OrthoArgs& O, int which, int
     }
 }
 
+// A launch of the products has one scaled identity: a list's few matrices of at most 32 rows take the others'.
+__device__ __forceinline__ float or_square_back(const OrthoArgs& O) { return O.list ? ORTHO_BACK_LONG : or_back(O.one.m); }
+// What the square's sum A A + A (b / factor) I is multiplied by; where there is no square, b.
+__device__ __forceinline__ float or_square_factor(const OrthoArgs& O, float back) { return O.c != 0.0f ? O.c * back : O.b; }
+
 // what an epilogue warp does with its 32 rows x 64 columns (rows row - lane ..., column block cb of 64)
 __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step, int which, int i, int row, int cb,
                                           uint32_t blk, uint32_t spare, int lane, float* v) {
@@ -723,15 +730,15 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
     const int r0 = row - lane;
     if (kind == OR_UPDATE) {
 #pragma unroll
-        for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
+        for (int j = 0; j < 64; ++j) v[j] *= 1.0f / ORTHO_SB;
         unsigned char* tile = L.x_next + i * L.x_row + (int64_t)cb * ORTHO_TILE + (r0 & 127) * 128;
         or_store_rows(blk, spare, tile, lane, v);
         return;
     }
     if (O.mirror && (cb >> 1) < i) return;  // below the diagonal (a pair's second row block): mirrored from above
     unsigned char* dst = kind == OR_GRAM ? L.a : L.b;
-    const float factor = kind == OR_GRAM ? ORTHO_SA / (ORTHO_SX * ORTHO_SX)
-                                         : (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA) * ORTHO_SQUARE_BACK);
+    const float factor = kind == OR_GRAM ? ORTHO_BACK_LONG * (ORTHO_SA / (ORTHO_SX * ORTHO_SX))
+                                         : or_square_factor(O, or_square_back(O)) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA));
     const float diagonal = kind == OR_GRAM ? 0.0f : O.a * ORTHO_SB;
 #pragma unroll
     for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == cb * 64 + j ? diagonal : 0.0f);
@@ -754,6 +761,37 @@ __device__ __forceinline__ void or_finish(const OrthoArgs& O, int kind, int step
             }
         }
     }
+}
+
+// The scaled identity that b A is taken against, from its row `first` on, by 128 threads: 16 rows x 8 chunks of
+// 16 bytes, swizzled; chunks 0-1 hold the value's first part (columns 0-15), 2-3 and 4-5 what the parts before
+// leave.  Three parts hold the value to 33 bits.  (Two left b off by 1.0e-7 of itself, the same way in every
+// step: matrices of 3 x 500 came out 2.1e-6 off, where fp32 products are 7e-7.)
+__device__ __forceinline__ void or_identity(const OrthoArgs& O, unsigned char* eye, int t, int first, float back) {
+    const int r = t >> 3, chunk = t & 7;
+    const double value = O.c != 0.0f ? (double)O.b / (double)or_square_factor(O, back) * ORTHO_SA : ORTHO_SA;
+    __half part[3];
+    double left = value;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        part[i] = __double2half(left);
+        left -= (double)__half2float(part[i]);
+    }
+    const __half zero = __float2half_rn(0.0f), mine = chunk < 2 ? part[0] : chunk < 4 ? part[1] : chunk < 6 ? part[2] : zero;
+    __align__(16) __half h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = (chunk & 1) * 8 + e == r + first ? mine : zero;
+    *reinterpret_cast<uint4*>(eye + r * 128 + ((chunk ^ (r & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
+}
+
+// c A A + b A = c (A A + A (b / c) I): 16 columns of A (hi and lo) against the scaled identity, added at d; the
+// products that are small beside the sum go before its large ones, whose size decides what truncation takes
+template <bool PAIR>
+__device__ __forceinline__ void or_identity_small(uint32_t d, uint32_t a, uint32_t al, uint32_t eye, uint32_t idesc) {
+    or_mma<PAIR>(d, a, eye + 4, idesc, 1u);
+    or_mma<PAIR>(d, al, eye + 2, idesc, 1u);
+    or_mma<PAIR>(d, a, eye + 2, idesc, 1u);
+    or_mma<PAIR>(d, al, eye, idesc, 1u);
 }
 
 struct OrthoShared {
@@ -926,18 +964,17 @@ __device__ __forceinline__ void or_issue(const OrthoArgs& O, OrthoShared& S, uin
                     for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(d, al + ks * 2, bh + ks * b_step, idesc, ks > 0);
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(d, a + ks * 2, bl + ks * b_step, idesc, 1u);
+                    const bool diagonal = kb >= eye0 && kb < eye1;  // this k-block's columns once more, 16 at a time
+                    const uint32_t dd = d + (uint32_t)(kb - eye0) * 64u;
+                    if (diagonal) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks) or_identity_small<PAIR>(dd + ks * 16, a + ks * 2, al + ks * 2, eye, eye_idesc);
+                    }
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(d, a + ks * 2, bh + ks * b_step, idesc, 1u);
-                    if (kb >= eye0 && kb < eye1) {
-                        // c A A + b A = c (A A + A (b / c) I): this k-block's columns once more, 16 at a time,
-                        // against a scaled identity
+                    if (diagonal) {
 #pragma unroll
-                        for (int ks = 0; ks < 4; ++ks) {
-                            const uint32_t dd = d + (uint32_t)(kb - eye0) * 64u + ks * 16;
-                            or_mma<PAIR>(dd, a + ks * 2, eye, eye_idesc, 1u);
-                            or_mma<PAIR>(dd, a + ks * 2, eye + 2, eye_idesc, 1u);
-                            or_mma<PAIR>(dd, al + ks * 2, eye, eye_idesc, 1u);
-                        }
+                        for (int ks = 0; ks < 4; ++ks) or_mma<PAIR>(dd + ks * 16, a + ks * 2, eye, eye_idesc, 1u);
                     }
                 }
                 or_commit<PAIR>(empty0 + 8 * s);
@@ -1108,19 +1145,7 @@ __global__ void __launch_bounds__(ORTHO_THREADS, 1) orthogonalize_kernel(const _
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x >= 128 && threadIdx.x < 256) {
-        // 16 rows x 8 chunks of 16 bytes, swizzled: chunks 0-1 hold hi (columns 0-15), chunks 2-3 lo; of a pair
-        // each block has eight of the identity's rows
-        const int r = (threadIdx.x - 128) >> 3, chunk = (threadIdx.x - 128) & 7;
-        const float value = O.c != 0.0f ? O.b / O.c * ORTHO_SA : ORTHO_SA;
-        __align__(16) __half h[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            __half hi, lo;
-            or_split((chunk & 1) * 8 + e == r + 8 * rank ? value : 0.0f, hi, lo);
-            h[e] = chunk < 2 ? hi : chunk < 4 ? lo : __float2half_rn(0.0f);
-        }
-        unsigned char* at = or_raw + 1024 + ORTHO_RING + ORTHO_STAGING + r * 128 + ((chunk ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(h);
+        or_identity(O, or_raw + 1024 + ORTHO_RING + ORTHO_STAGING, threadIdx.x - 128, 8 * rank, or_square_back(O));  // of a pair each block has eight of its rows
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 0) {
@@ -1290,16 +1315,7 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (threadIdx.x >= 128 && threadIdx.x < 256) {
-        const int r = (threadIdx.x - 128) >> 3, chunk = (threadIdx.x - 128) & 7;
-        const float value = O.c != 0.0f ? O.b / O.c * ORTHO_SA : ORTHO_SA;
-        __align__(16) __half h[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            __half hi, lo;
-            or_split((chunk & 1) * 8 + e == r ? value : 0.0f, hi, lo);
-            h[e] = chunk < 2 ? hi : chunk < 4 ? lo : __float2half_rn(0.0f);
-        }
-        *reinterpret_cast<uint4*>(or_raw + (eye_at - or_smem(or_raw)) + r * 128 + ((chunk ^ (r & 7)) << 4)) = *reinterpret_cast<uint4*>(h);
+        or_identity(O, or_raw + (eye_at - or_smem(or_raw)), threadIdx.x - 128, 0, or_back(d.m));
     }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(or_smem(&S.tmem)), "r"(512u)
@@ -1412,21 +1428,27 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
                         const uint32_t a = or_desc(at, 16), al = a + (16384u >> 4);
                         const uint32_t bh = kind == OR_UPDATE ? or_desc(xs + (uint32_t)kb * 8192u, ORTHO_TILE) : a;
                         const uint32_t bl = bh + (16384u >> 4), b_step = kind == OR_UPDATE ? 2048u >> 4 : 2u;
-                        if (!linear) {
+                        const uint32_t dc = dd + (uint32_t)kb * 64u;
+                        if (linear) {
+#pragma unroll
+                            for (int ks = 0; ks < 4; ++ks) {
+                                or_mma<false>(dc + ks * 16, al + ks * 2, eye, eye_idesc, 0u);
+                                or_mma<false>(dc + ks * 16, a + ks * 2, eye, eye_idesc, 1u);
+                            }
+                        } else {
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks) or_mma<false>(dd, al + ks * 2, bh + ks * b_step, idesc, ks > 0);
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks) or_mma<false>(dd, a + ks * 2, bl + ks * b_step, idesc, 1u);
+                            if (kind == OR_SQUARE) {
+#pragma unroll
+                                for (int ks = 0; ks < 4; ++ks) or_identity_small<false>(dc + ks * 16, a + ks * 2, al + ks * 2, eye, eye_idesc);
+                            }
 #pragma unroll
                             for (int ks = 0; ks < 4; ++ks) or_mma<false>(dd, a + ks * 2, bh + ks * b_step, idesc, 1u);
-                        }
-                        if (kind == OR_SQUARE) {
+                            if (kind == OR_SQUARE) {
 #pragma unroll
-                            for (int ks = 0; ks < 4; ++ks) {
-                                const uint32_t dc = dd + (uint32_t)kb * 64u + ks * 16;
-                                or_mma<false>(dc, al + ks * 2, eye, eye_idesc, !linear);
-                                or_mma<false>(dc, a + ks * 2, eye, eye_idesc, 1u);
-                                if (!linear) or_mma<false>(dc, a + ks * 2, eye + 2, eye_idesc, 1u);
+                                for (int ks = 0; ks < 4; ++ks) or_mma<false>(dc + ks * 16, a + ks * 2, eye, eye_idesc, 1u);
                             }
                         }
                         if (!linear || kb == kblocks - 1) {
@@ -1462,7 +1484,7 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
                 }
                 if (kind == OR_GRAM) {
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) v[j] *= ORTHO_SA / (ORTHO_SX * ORTHO_SX);
+                    for (int j = 0; j < 64; ++j) v[j] *= or_back(d.n) * (ORTHO_SA / (ORTHO_SX * ORTHO_SX));
                     if (team == 1) {
                         if (mine) or_keep_rows(as + part * ORTHO_TILE, row, v);
                     } else if (part < m64) {
@@ -1477,7 +1499,7 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
                                          : "memory");
                     }
                 } else if (kind == OR_SQUARE) {
-                    const float factor = (O.c != 0.0f ? O.c : O.b) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA) * ORTHO_SQUARE_BACK), diagonal = O.a * ORTHO_SB;
+                    const float factor = or_square_factor(O, or_back(d.m)) * (ORTHO_SB / (ORTHO_SA * ORTHO_SA)), diagonal = O.a * ORTHO_SB;
                     if (mine) {
 #pragma unroll
                         for (int j = 0; j < 64; ++j) v[j] = fmaf(v[j], factor, row == part * 64 + j ? diagonal : 0.0f);
@@ -1486,7 +1508,7 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
                 } else if (mine && ok) {
                     if (step + 1 < O.steps) {
 #pragma unroll
-                        for (int j = 0; j < 64; ++j) v[j] *= ORTHO_UPDATE_BACK / ORTHO_SB;
+                        for (int j = 0; j < 64; ++j) v[j] *= 1.0f / ORTHO_SB;
                         or_keep_rows(xs + part * ORTHO_TILE, row, v);
                     } else {
                         or_finish_out(O, which, row, first + part, sums + (uint32_t)e * ORTHO_BLOCK, lane, v);

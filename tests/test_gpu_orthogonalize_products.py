@@ -39,3 +39,34 @@ def test_bf16_outputs_are_fp32_results_rounded_once(m, n, kind):
     assert _off(orthogonalize(x), ref) <= 1.01 * _off(ref.bfloat16(), ref) + FP32_BAR
     assert _off(orthogonalize(x, out_dtype=F16), ref) <= BAR[F16]
     assert orthogonalize_error(DEV) == 0
+
+
+def _fp32_products(x):
+    x = x.float()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    x = x / (torch.linalg.matrix_norm(x.double()).float() + 1e-7)
+    for _ in range(5):
+        g = x @ x.mT
+        x = 3.4445 * x + (-4.7750 * g + 2.0315 * (g @ g)) @ x
+    return x.mT if tall else x
+
+
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 7), (1, 300), (3, 2), (3, 500), (9, 64), (64, 64), (65, 130), (128, 384), (1, 4096),
+                                 (5000, 3), (20, 3000), (129, 257), (256, 1024), (200, 5000), (1024, 640)])
+def test_errors_are_those_of_fp32_products(m, n):
+    """Pairs of fp16 numbers hold 22 bits, operands 2^-23 off where fp32's are 2^-24: twice the error of fp32 products
+    at most, on average over matrices (a single small one may by chance come out exact in fp32)."""
+    from pbg_b200.optim import orthogonalize
+
+    allowed = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        ours = theirs = 0.0
+        for seed in range(24 if m * n < 5000 else 6):
+            x = _matrix("low" if seed % 3 == 2 else "noise", m, n, torch.Generator(device=DEV).manual_seed(1000 + seed))
+            ref = _reference(x)
+            ours, theirs = ours + _off(orthogonalize(x), ref), theirs + _off(_fp32_products(x), ref)
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = allowed
+    assert ours <= 2.0 * theirs
