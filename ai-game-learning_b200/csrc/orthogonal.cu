@@ -351,6 +351,13 @@ __device__ __forceinline__ double or_block_sum(double v) {
     return sum;
 }
 
+// what a matrix of that sum of squares is multiplied by: 2^14 over its norm and epsilon (a matrix of zeros stays
+// zeros where epsilon is 0 too)
+__device__ __forceinline__ double or_wide(const OrthoArgs& O, double squares) {
+    const double norm = sqrt(squares) + O.eps;
+    return norm == 0.0 ? 0.0 : (double)ORTHO_SX / norm;
+}
+
 // eight consecutive elements i .. i + 7, zeros from `live` on
 __device__ __forceinline__ void or_load8(const void* p, int type, int64_t i, bool vector, int live, float* v) {
     if (vector && live >= 8) {
@@ -428,7 +435,7 @@ __global__ void __launch_bounds__(ORTHO_FLAT) orthogonalize_convert_kernel(const
     double sum = 0.0;
     const int64_t spans = ((int64_t)d.m * d.n + ORTHO_SPAN - 1) / ORTHO_SPAN;
     for (int64_t i = threadIdx.x; i < spans; i += ORTHO_FLAT) sum += O.sums[d.span0 + i];
-    const double wide = (double)ORTHO_SX / (sqrt(or_block_sum(sum)) + O.eps);
+    const double wide = or_wide(O, or_block_sum(sum));
     const float scale = (float)wide;
     const bool plain = scale < 1.0e30f;  // beyond it belongs to a direction of (sub)normal smallness: in fp64 then
     unsigned char* tile = O.tiles + d.ws + ((int64_t)ti * or_pitch_x(d.n) + tj) * ORTHO_TILE;
@@ -1358,7 +1365,7 @@ __global__ void __launch_bounds__(ORTHO_TEAM_THREADS, 1) orthogonalize_team_kern
         const int64_t spans = ((int64_t)d.m * d.n + ORTHO_SPAN - 1) / ORTHO_SPAN;
         for (int64_t r = 0; r < spans; ++r) total += __ldg(O.sums + d.span0 + r);
     }
-    const double wide = (double)ORTHO_SX / (sqrt(total) + O.eps);
+    const double wide = or_wide(O, total);
     const float scale = (float)wide;
     const bool plain = scale < 1.0e30f;
 #pragma unroll 2

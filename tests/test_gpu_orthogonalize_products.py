@@ -70,3 +70,24 @@ def test_errors_are_those_of_fp32_products(m, n):
     finally:
         torch.backends.cuda.matmul.allow_tf32 = allowed
     assert ours <= 2.0 * theirs
+
+
+@pytest.mark.parametrize("m,n", [(1, 5), (64, 200), (128, 1600), (200, 300), (1536, 2048)])
+def test_zeros_without_an_epsilon(m, n):
+    """A matrix of zeros gives zeros, and moves its master by the decay alone, where epsilon is 0 too."""
+    from pbg_b200.optim import FlatMuon, orthogonalize
+
+    x = torch.zeros(2, m, n, device=DEV)
+    x[1].normal_(generator=torch.Generator(device=DEV).manual_seed(m))
+    got = orthogonalize(x, epsilon=0.0)
+    assert bool((got[0] == 0).all())
+    assert _off(got[1], _reference(x[1], eps=0.0)) <= FP32_BAR
+    x[0, 0, 1] = float("nan")
+    assert bool(orthogonalize(x[0], epsilon=0.0).isnan().all())
+    master = torch.randn(2 * m * n, generator=torch.Generator(device=DEV).manual_seed(n), device=DEV)
+    step = FlatMuon(master, [(0, m, n), (m * n, m, n)], epsilon=0.0, lr=0.5, decay=0.5)
+    before = master.clone()
+    step.grad[m * n:].copy_(x[1].flatten())
+    step.step()
+    assert int(step.skipped) == 0 and bool(master.isfinite().all())
+    assert torch.equal(master[:m * n], 0.75 * before[:m * n]) and not torch.equal(master[m * n:], 0.75 * before[m * n:])
