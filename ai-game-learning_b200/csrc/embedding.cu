@@ -38,6 +38,7 @@
 namespace pbg {
 
 enum { EMB_F32 = 0, EMB_BF16 = 1, EMB_F16 = 2 };
+constexpr uint32_t EMB_BAD_INDEX = 1, EMB_GAVE_UP = 2;  // bits of the error word
 constexpr int EMB_THREADS = 512;
 constexpr int EMB_WARPS = EMB_THREADS / 32;
 constexpr int EMB_BINS = 512;        // 9-bit digits
@@ -114,6 +115,11 @@ __device__ __forceinline__ int64_t emb_index(const void* index, int wide, int64_
     return wide ? __ldg(static_cast<const long long*>(index) + t) : (int64_t)__ldg(static_cast<const int*>(index) + t);
 }
 
+// an index outside the table: its bit is set once, so that many such indices do not queue up at one word
+__device__ __forceinline__ void emb_bad_index(uint32_t* error) {
+    if (!(*reinterpret_cast<volatile uint32_t*>(error) & EMB_BAD_INDEX)) atomicOr(error, EMB_BAD_INDEX);
+}
+
 // ---------------------------------------------------------------- forward
 
 struct EmbArgs {
@@ -145,10 +151,11 @@ __global__ void __launch_bounds__(256) embedding_kernel(EmbArgs E) {
     const int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> E.log_lanes;
     const int64_t step = ((int64_t)gridDim.x * 256) >> E.log_lanes;
     const T* table = static_cast<const T*>(E.table);
+    bool bad = false;
     for (int64_t t = first; t < E.tokens; t += step) {
         const int64_t i = emb_index(E.index, E.index64, t);
         const bool live = i >= 0 && i < E.rows;
-        if (!live && lane == 0) *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
+        bad |= !live;
         const T* src = table + (live ? i : 0) * E.ldt;
         for (int64_t c0 = (int64_t)lane * VEC; c0 < E.width; c0 += (int64_t)lanes * VEC * 4) {
             EmbVec<T, VEC> x[4];
@@ -164,6 +171,7 @@ __global__ void __launch_bounds__(256) embedding_kernel(EmbArgs E) {
             }
         }
     }
+    if (bad && lane == 0) emb_bad_index(E.error);
 }
 
 // Rows of at most a vector per lane: eight rows a group in flight, indices first.
@@ -174,6 +182,7 @@ __global__ void __launch_bounds__(256) embedding_rows_kernel(EmbArgs E) {
     const int64_t c = (int64_t)lane * VEC;
     const bool in = c < E.width;
     const T* table = static_cast<const T*>(E.table);
+    bool bad = false;
     for (int64_t t0 = (int64_t)blockIdx.x * groups * 8; t0 < E.tokens; t0 += (int64_t)gridDim.x * groups * 8) {
         int64_t i[8];
         EmbVec<T, VEC> x[8];
@@ -186,7 +195,7 @@ __global__ void __launch_bounds__(256) embedding_rows_kernel(EmbArgs E) {
         for (int u = 0; u < 8; ++u) {
             const int64_t t = t0 + u * groups + group;
             if (i[u] < 0 || i[u] >= E.rows) {
-                if (t < E.tokens) *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
+                bad |= t < E.tokens;
                 i[u] = -1;
             } else if (in && t < E.tokens) {
                 x[u] = *reinterpret_cast<const EmbVec<T, VEC>*>(table + i[u] * E.ldt + c);
@@ -198,6 +207,7 @@ __global__ void __launch_bounds__(256) embedding_rows_kernel(EmbArgs E) {
             if (in && t < E.tokens) emb_scaled<T, VEC>(E, t * E.width + c, i[u] >= 0, x[u]);
         }
     }
+    if (bad && lane == 0) emb_bad_index(E.error);
 }
 
 // ---------------------------------------------------------------- backward
@@ -231,7 +241,7 @@ struct EmbGradArgs {
 };
 
 // Arrivals of `blocks` blocks counted in one word (E.barrier[0]: the whole grid, [1]: the sorting
-// blocks); the kernel is launched cooperatively, so every block runs.  A wait that runs out records 2 in
+// blocks); the kernel is launched cooperatively, so every block runs.  A wait that runs out sets its bit of
 // the error word and lets its block go on to the end of the kernel without touching the output.
 __device__ __forceinline__ bool emb_sync(const EmbGradArgs& E, int word, uint32_t blocks, uint32_t& target) {
     if (blocks == 1) {
@@ -250,7 +260,7 @@ __device__ __forceinline__ bool emb_sync(const EmbGradArgs& E, int word, uint32_
             ++i;
         }
         const int ok = (int32_t)(seen - target) >= 0;
-        if (!ok) atomicExch(E.error, 2u);
+        if (!ok) atomicOr(E.error, EMB_GAVE_UP);
         __threadfence();
         ok_s = ok;
     }
@@ -263,7 +273,7 @@ __device__ __forceinline__ bool emb_sync(const EmbGradArgs& E, int word, uint32_
 __device__ __forceinline__ uint32_t emb_key(const EmbGradArgs& E, int64_t t) {
     const int64_t i = emb_index(E.index, E.index64, t);
     if (i < 0 || i >= E.rows) {
-        *reinterpret_cast<volatile uint32_t*>(E.error) = 1u;
+        emb_bad_index(E.error);
         return (uint32_t)E.rows;
     }
     return i == E.padding ? (uint32_t)E.rows : (uint32_t)i;

@@ -35,8 +35,8 @@ def _error_word(device: torch.device) -> Tensor:
 
 
 def index_error(device=None) -> int:
-    """The device's sticky error word: 0 none, 1 an index outside a table, 2 a grid barrier that gave up
-    (the gradient of that call is incomplete); synchronises."""
+    """The device's sticky error word: 0 none, bit 0 an index outside a table, bit 1 a grid barrier that gave
+    up (the gradient of that call is incomplete); synchronises."""
 
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     if device.index is None:

@@ -418,7 +418,7 @@ int pbg_ppo_categorical_backward_noalloc(int64_t N, int32_t A, int32_t dtype, co
 /* Embedding rows by index (pbg/games/poker/model/preflop.py:206-233, the networks' tables):
  * out[t, :] = scale * table[index[t], :], out [tokens, width] contiguous.  Types 0 fp32, 1 bf16, 2 fp16;
  * index int32 or int64 (index64); table row stride ldt elements.  An index outside [0, rows) gives a row
- * of zeros and sets error (device uint32, sticky) to 1. */
+ * of zeros and sets bit 0 of error (device uint32, sticky). */
 int pbg_embedding(int64_t tokens, int64_t rows, int64_t width, const void *index, int32_t index64, const void *table,
                   int32_t table_type, int64_t ldt, float scale, void *out, int32_t out_type, uint32_t *error,
                   void *stream);
@@ -426,7 +426,7 @@ int pbg_embedding(int64_t tokens, int64_t rows, int64_t width, const void *index
  * rows without tokens zero (accumulate: untouched).  fp32 sums in an order that sizes alone determine,
  * rounded once.  padding: an index whose tokens give no gradient, or -1.  workspace: 256-byte aligned
  * device memory of pbg_embedding_backward_workspace(tokens, width) bytes, any contents, one per call in
- * flight.  error: 1 an index outside the table (no gradient), 2 a grid barrier gave up.  At most
+ * flight.  error: bit 0 an index outside the table (no gradient), bit 1 a grid barrier gave up.  At most
  * 2^31 - 1 tokens and rows. */
 int64_t pbg_embedding_backward_workspace(int64_t tokens, int64_t width);
 int pbg_embedding_backward(int64_t tokens, int64_t rows, int64_t width, const void *grad, int32_t grad_type, int64_t ldg,

@@ -1,0 +1,31 @@
+"""What the embedding and orthogonalisation kernels report of failures, and who reads it."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+
+
+@pytest.mark.parametrize("tokens,rows,width", [(3, 50, 24), (40000, 50, 24), (3000, 50, 40), (9000, 50, 40), (9000, 2000, 16),
+                                               (9000, 500, 40)])
+def test_errors_are_bits_that_stay(tokens, rows, width):
+    """An index outside the table does not wipe out an earlier barrier's failure."""
+    from pbg_b200 import embedding as E
+
+    gen = torch.Generator(device=DEV).manual_seed(tokens)
+    table = torch.randn(rows, width, generator=gen, device=DEV)
+    index = torch.randint(0, rows, (tokens,), generator=gen, device=DEV)
+    index[1] = rows
+    grad = torch.randn(tokens, width, generator=gen, device=DEV)
+    try:
+        for call in (lambda: E.embedding(table, index), lambda: E.embedding_backward(grad, index, rows)):
+            E._error_word(DEV).fill_(2)
+            call()
+            assert E.index_error(DEV) == 3
+            E._error_word(DEV).zero_()
+            call()
+            assert E.index_error(DEV) == 1
+    finally:
+        E._error_word(DEV).zero_()
