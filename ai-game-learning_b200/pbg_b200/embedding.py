@@ -9,8 +9,8 @@ floating-point atomics: the same inputs give the same bits in every run.
 ``pbg_b200.model_train.embedding_train`` is the two as one autograd function.
 
 An index outside the table gives a row of zeros and no gradient, and sets the
-device's sticky error word, which ``index_error`` reads (no launch waits for
-it).  Calls run on the current stream of their tensors' device and can be
+device's sticky error word, which ``index_error`` reads and
+``checks.raise_input_errors`` reports (no launch waits for it).  Calls run on the current stream of their tensors' device and can be
 captured into graphs once one call has been made on the device.
 """
 
@@ -19,10 +19,13 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
+from . import checks
 from ._native import NativeError, entry, lib, raw_stream
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ERROR: dict[int, Tensor] = {}
+checks.watch(_ERROR, {1: "an embedding index is outside its table",
+                      2: "a wait inside an embedding gradient gave up: the gradient is incomplete"})
 
 
 def _error_word(device: torch.device) -> Tensor:

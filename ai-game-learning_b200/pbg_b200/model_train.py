@@ -335,7 +335,11 @@ class ModelLearnerStep:
     ``muon``: options of ``FlatMuon`` (a dict, may be empty): the hidden matrices (``is_hidden_matrix``)
     then take its transition and AdamW keeps the tables, vectors and head rows; ``grad`` is the whole
     flat gradient either way.  Each transition guards its own part against gradients that are not finite.
-    ``sorted_embeddings``: the tables' gradients by sorted tokens instead of one-hot products."""
+    ``sorted_embeddings``: the tables' gradients by sorted tokens instead of one-hot products.
+
+    A step waits for nothing on the host: ``checks.raise_input_errors`` reports, whenever it is called, what
+    its kernels found wrong since the last call (inputs out of range, an index outside a table, a wait that
+    gave up), ``adam.report`` and ``muon.skipped`` what the last transition did."""
 
     def __init__(self, model, *, lr: float = 3e-4, beta1: float = 0.9, beta2: float = 0.999, epsilon: float = 1e-8,
                  weight_decay: float = 0.0, grad_clip: float = 1.0, muon: dict | None = None,

@@ -19,6 +19,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
+from . import checks
 from ._native import NativeError, call, entry, lib, ptr, raw_stream, stream
 
 CONTROL_NAMES = ("lr", "beta1", "beta2", "epsilon", "decay", "clip", "scale", "growth", "backoff", "interval")
@@ -57,6 +58,7 @@ class FlatAdam:
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ERROR: dict[int, Tensor] = {}
+checks.watch(_ERROR, {0x7FFFFFFF: "a wait inside an orthogonalisation gave up: its outputs, or masters and momenta, are incomplete"})
 
 
 def _error_word(device: torch.device) -> Tensor:

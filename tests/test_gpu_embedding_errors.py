@@ -29,3 +29,23 @@ def test_errors_are_bits_that_stay(tokens, rows, width):
             assert E.index_error(DEV) == 1
     finally:
         E._error_word(DEV).zero_()
+
+
+def test_the_learner_steps_checks_report_them():
+    """What a one-hot lookup refused, an index outside the table, and a wait that gave up reach the caller."""
+    from pbg_b200 import checks, optim
+    from pbg_b200.model_train import embedding_train
+
+    table = torch.randn(9, 16, device=DEV, requires_grad=True)
+    checks.input_errors(DEV)
+    embedding_train(table, torch.tensor([0, 8, 3], device=DEV)).sum().backward()
+    optim.orthogonalize(torch.ones(3, 4, device=DEV))
+    assert checks.input_errors(DEV) == []
+    embedding_train(table, torch.tensor([0, 9, 3], device=DEV))
+    with pytest.raises(ValueError, match="outside its table"):
+        checks.raise_input_errors(DEV)
+    checks.raise_input_errors(DEV)
+    optim._error_word(DEV).fill_(4)
+    with pytest.raises(ValueError, match="gave up"):
+        checks.raise_input_errors(torch.device("cuda"))
+    assert optim.orthogonalize_error(DEV) == 0
