@@ -334,7 +334,7 @@ class ModelLearnerStep:
 
     ``muon``: options of ``FlatMuon`` (a dict, may be empty): the hidden matrices (``is_hidden_matrix``)
     then take its transition and AdamW keeps the tables, vectors and head rows; ``grad`` is the whole
-    flat gradient either way.  Each transition guards its own part against gradients that are not finite.
+    flat gradient either way.  A gradient that is not finite anywhere stops both transitions.
     ``sorted_embeddings``: the tables' gradients by sorted tokens instead of one-hot products.
 
     A step waits for nothing on the host: ``checks.raise_input_errors`` reports, whenever it is called, what
@@ -380,9 +380,20 @@ class ModelLearnerStep:
             results.append(result)
         return results
 
+    def transition(self) -> None:
+        """One transition of the flat master from ``self.grad`` (summed over the ranks where there are several),
+        all of it or nothing: a gradient that is not finite leaves masters and moments as they were and is cleared."""
+
+        if self.muon is None:
+            self.adam.step()
+            return
+        # each optimizer's own guard sees what stops the other as a NaN in its part's first element
+        self.adam.grad[:1].add_(self.grad[: self.flat.split].sum(dtype=torch.float64) * 0.0)
+        report = self.adam.step()
+        self.grad[:1].add_(report[:1].reciprocal() * 0.0)  # report[0]: 1 where the transition was applied, else 0
+        self.muon.step()
+
     def __call__(self, batches: list) -> list:
         results = self.gradient(batches)
-        if self.muon is not None:
-            self.muon.step()
-        self.adam.step()
+        self.transition()
         return results
