@@ -316,9 +316,11 @@ _FIELDS = ("type_logits", "omega", "mu", "s", "iota")
 
 def is_hidden_matrix(name: str, shape: tuple) -> bool:
     """Whether a parameter is one that an orthogonalised update suits: a weight matrix of a map with more
-    than one row and column; not a table (embeddings, tokens), a vector or a scalar's affine map."""
+    than one row and column; not a table (embeddings, tokens), a vector, a scalar's affine map or the rows that
+    a head's outputs are (``*_head.*affine``)."""
 
-    return len(shape) == 2 and min(shape) > 1 and name.endswith(".weight") and "embedding" not in name
+    head_rows = "_head." in name and name.endswith("affine.weight")
+    return len(shape) == 2 and min(shape) > 1 and name.endswith(".weight") and "embedding" not in name and not head_rows
 
 
 class ModelLearnerStep:
