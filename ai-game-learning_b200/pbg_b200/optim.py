@@ -66,7 +66,9 @@ def _error_word(device: torch.device) -> Tensor:
     if word is None:
         if torch.cuda.is_current_stream_capturing():
             raise NativeError("make one call on this device before capturing one into a graph")
-        word = _ERROR[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        word = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()  # once: calls on other streams use it too
+        _ERROR[device.index] = word
     return word
 
 

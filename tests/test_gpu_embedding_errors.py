@@ -49,3 +49,20 @@ def test_the_learner_steps_checks_report_them():
     with pytest.raises(ValueError, match="gave up"):
         checks.raise_input_errors(torch.device("cuda"))
     assert optim.orthogonalize_error(DEV) == 0
+
+
+def test_the_first_call_on_a_busy_stream_keeps_other_streams_errors(monkeypatch):
+    """The error word is clear before any call on another stream can set it."""
+    from pbg_b200 import embedding as E
+
+    table = torch.randn(9, 16, device=DEV)
+    good, bad = torch.tensor([0, 8, 3], device=DEV), torch.tensor([0, 9, 3], device=DEV)
+    torch.cuda.synchronize()
+    monkeypatch.setattr(E, "_ERROR", {})
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about a tenth of a second
+        E.embedding(table, good)
+    E.embedding(table, bad)
+    torch.cuda.synchronize()
+    assert E.index_error(DEV) == 1
