@@ -254,8 +254,10 @@ def embedding_train(table: Tensor, index: Tensor, scale: float = 1.0) -> Tensor:
         # the leaf's accumulation node lives as long as a graph that leads to it, and its notes with it
         notes = out.grad_fn.next_functions[0][0].metadata
         now = raw_stream(table.device.index)
-        if notes.setdefault("pbg_b200 stream", now) != now and torch.cuda.is_current_stream_capturing():
-            raise NativeError("embedding_train: release the graphs of this table made on another stream before capturing")
+        if notes.setdefault("pbg_b200 stream", now) != now:
+            with torch.cuda.device(table.device):  # the capture that matters is of the table's device
+                if torch.cuda.is_current_stream_capturing():
+                    raise NativeError("embedding_train: release the graphs of this table made on another stream before capturing")
     return out
 
 
