@@ -69,3 +69,19 @@ def test_without_muon_the_transition_is_adamw(gold):
     twin.gradient(batches)
     twin.adam.step()
     assert torch.equal(step.adam.grad, twin.adam.grad) and torch.equal(step.flat.master, twin.flat.master)
+
+
+def test_adamw_takes_the_rest_of_the_gradient(gold):
+    """A first AdamW step against float64 of the gradient that it was given: about 16 fp32 roundings of the
+    direction (of size 1, times lr) and two of the master."""
+    lr, decay, clip = 3e-4, 0.1, 1.0
+    step, batches = _step(gold, sorted_embeddings=True, muon={}, lr=lr, weight_decay=decay, grad_clip=clip)
+    step.gradient(batches)
+    split = step.flat.split
+    before, g = step.flat.master[split:].double(), step.grad[split:].double()
+    step.transition()
+    g = g * min(1.0, clip / float(g.norm()))
+    want = before * (1 - lr * decay) - lr * g / (g.abs() + 1e-8)
+    bar = lr * 32 * 2.0 ** -24 + 2.0 ** -23 * before.abs()
+    assert bool(((step.flat.master[split:].double() - want).abs() <= bar).all())
+    assert float((want - before).abs().max()) > 0.9 * lr and int((g != 0).sum()) > g.numel() // 4

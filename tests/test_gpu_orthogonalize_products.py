@@ -91,3 +91,65 @@ def test_zeros_without_an_epsilon(m, n):
     step.step()
     assert int(step.skipped) == 0 and bool(master.isfinite().all())
     assert torch.equal(master[:m * n], 0.75 * before[:m * n]) and not torch.equal(master[m * n:], 0.75 * before[m * n:])
+
+
+@pytest.mark.parametrize("m,n", [(200, 300), (192, 192), (256, 8192), (1536, 2048), (300, 170)])
+@pytest.mark.parametrize("steps,k", [(1, (3.4445, -4.7750, 2.0315)), (4, (3.4445, -4.7750, 2.0315)), (12, (1.5, -0.5, 0.0)),
+                                     (10, (1.875, -1.25, 0.375)), (6, (2.0, -1.5, 0.5)), (3, (1.0, 0.0, 0.0)),
+                                     (2, (0.5, 0.25, 0.125))])
+def test_polynomials_and_step_counts(m, n, steps, k):
+    """Single blocks, an odd number of 64-wide blocks, split sums and pairs, with and without a square."""
+    from pbg_b200.optim import orthogonalize, orthogonalize_error
+
+    x = _matrix("low", m, n, torch.Generator(device=DEV).manual_seed(m + n))
+    ref = _reference(x, steps, 0.5, k)
+    for dtype in (F32, BF16):
+        got = orthogonalize(x, steps=steps, coefficients=k, epsilon=0.5, out_dtype=dtype)
+        assert _off(got, ref) <= BAR[dtype]
+    assert orthogonalize_error(DEV) == 0
+
+
+def test_a_batch_of_more_tiles_than_one_launch_works_in():
+    """18 matrices of 2,048 x 2,048: 69 MB of tiles each, 15 a launch within 1 GB."""
+    from pbg_b200.optim import orthogonalize, orthogonalize_error
+
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(18, 2048, 2048, generator=gen, device=DEV)
+    got = orthogonalize(x)
+    for i in (0, 14, 15, 17):
+        assert _off(got[i], _reference(x[i])) <= FP32_BAR
+    for i in (3, 16):
+        assert _off(got[i], orthogonalize(x[i]).double()) <= 2 * FP32_BAR  # another tile shape may serve one matrix
+    assert torch.equal(got, orthogonalize(x)) and orthogonalize_error(DEV) == 0
+
+
+def test_a_transition_of_more_tiles_than_one_launch_works_in():
+    """Launches of their own for what passes 1 GB, one matrix with split sums, and teams, in one list."""
+    from pbg_b200.optim import FlatMuon, orthogonalize_error
+
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    sizes = [(2048, 2048)] * 17 + [(256, 8192), (100, 300), (300, 64), (130, 131)]
+    mats, at = [], 0
+    for r, c in sizes:
+        mats.append((at, r, c))
+        at += (r * c + 3) // 4 * 4
+    step = FlatMuon(torch.randn(at, generator=gen, device=DEV), mats, lr=0.05, momentum=0.9, decay=0.1)
+    assert int(step._plan[2]) >= 2
+    twin = FlatMuon(step.master.clone(), mats, lr=0.05, momentum=0.9, decay=0.1)
+    for _ in range(2):
+        step.grad.normal_(generator=gen)
+        twin.grad.copy_(step.grad)
+        before, old = step.master.clone(), step.momentum.clone()
+        step.step(), twin.step()
+        assert int(step.skipped) == 0 and torch.equal(step.master, twin.master)
+        for i in (0, 13, 14, 15, 16, 17, 18, 19, 20):
+            o, r, c = mats[i]
+            s = slice(o, o + r * c)
+            w, m, g = before[s].double(), old[s].double(), step.grad[s].double()
+            m = 0.9 * m + 0.1 * g
+            f = 0.05 * max(1.0, r / c) ** 0.5
+            want = w * (1 - 0.05 * 0.1) - f * _reference((0.9 * m + 0.1 * g).view(r, c)).reshape(-1)
+            bar = f * FP32_BAR * 1.3 * min(r, c) ** 0.5 + 2.0 ** -23 * float(want.norm())
+            assert float((step.master[s].double() - want).norm()) <= bar, i
+            assert float((step.momentum[s].double() - m).norm()) <= 2.0 ** -22 * float(m.norm() + g.norm())
+    assert orthogonalize_error(DEV) == 0
