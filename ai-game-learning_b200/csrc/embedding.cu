@@ -6,13 +6,14 @@
 // Both are bound by HBM: the forward reads each looked-up row and writes each output row once, the
 // backward reads each incoming row once and writes each table row once.
 //
-// The backward has no floating-point atomics, so the result is the same in every run.  By size (measured
-// times are at 1965 MHz):
+// The backward has no floating-point atomics, so the result is the same in every run on the same data, strides
+// and alignment (which decide the vector width, and with it the order of the sums) and the same device.  By size
+// (times of the device at 1965 MHz; a call takes 13 to 17 us at least, most of it on the host):
 //   - few tokens (EMB_SCAN): no sort.  A warp (up to 256 tokens) or a block per table row looks through all
 //     indices, 32 at a time, and adds the rows that match.  512 tokens into 169 x 32: 2.7 us (sorted 15.5).
 //   - few table rows (EMB_TABLE): every warp keeps the whole table's sums for its columns in shared memory
 //     and adds its share of the tokens' rows in order; then the warps' and the blocks' tables are added in
-//     order.  81,920 x 128 bf16 into 13 rows: 15.5 us (sorted 37); 1,000,003 x 128 into 4 rows: 94 us (125).
+//     order.  81,920 x 128 fp32 into 13 rows: 15.3 us (sorted 37); 1,000,003 x 128 bf16 into 4 rows: 94 us (125).
 //   - small tables of narrow rows (emb_narrow_plan): ranges of rows x 16 columns in a block's shared memory.
 //   - else sorted tokens, one cooperative kernel:
 //     1. a stable radix sort of (index, position) pairs: least significant digit first, at most 9 bits a
@@ -699,7 +700,11 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_kernel(EmbG
 
 // ---------------------------------------------------------------- few tokens
 
-constexpr int EMB_SCAN_TOKENS = 4096;  // at most
+// A block per row (of up to eight an SM) looks through up to this many tokens.  Measured, this way and what else
+// would be taken: 4,096 tokens into 40 x 32 6.4 and 8.5 us, into 300 x 128 7.8 and 25, into 1,184 x 16 13 and 75,
+// but into 4 x 32 12.5 and 7.4; 16,384 into 40 x 32 18 and 8.7, into 1,184 x 128 39 and 45; 4,096 into 2,400 x 512
+// (9,600 blocks) 84 and 45 us.
+constexpr int EMB_SCAN_TOKENS = 4096;
 constexpr int EMB_SCAN_WARP = 256;     // up to here a warp per table row
 
 // the rows of the tokens in `match` (bits of tokens t0 ..), added in order, eight in flight
@@ -854,7 +859,9 @@ __global__ void __launch_bounds__(EMB_THREADS, 2) embedding_backward_table_kerne
     }
 }
 
-// few blocks' tables in order: a column a thread
+// few blocks' tables in order: a column a thread.  Measured, with this fold and with the next: 9,000 tokens into
+// 30,000 x 16 (5 tables) 14.4 and 44 us, 50,000 into 8,000 x 8 (25) 17.6 and 20.7, 100,000 into 10,000 x 2 (49)
+// 20.7 and 18.5, 500,000 into 1,024 x 1 (245) 48 and 33 us; where few sums leave both a few us, they are alike.
 constexpr int EMB_FOLD_FEW = 32;
 __global__ void __launch_bounds__(256) embedding_backward_fold_few_kernel(EmbGradArgs E, int blocks) {
     const int64_t total = E.rows * E.width, at = (int64_t)blockIdx.x * 256 + threadIdx.x;

@@ -14,8 +14,8 @@
 // between the 3 * steps products.  A matrix whose short side is at most 128 stays, with everything that is
 // made of it, in the shared memory of a team of 1 to 8 blocks (orthogonalize_team_kernel).
 //
-// What bounds it.  4,096 x 4,096: the tensor cores, 1.43 PFLOP/s of fp16 products in three passes (fp32,
-// 3.13 ms), power-capped.  14 of 256 x 1,024 (218 us): 15 products of a few microseconds each behind one
+// What bounds it.  4,096 x 4,096: the tensor cores, 1.29 PFLOP/s of fp16 products in three passes (3.30 ms; call
+// after call the power cap makes it 3.9 ms).  14 of 256 x 1,024 (218 us): 15 products of a few microseconds each behind one
 // another, so each one's first copies, last stores and the barrier.
 //
 // Precision.  16-bit operands alone are not enough: an error in X in the direction of a small singular

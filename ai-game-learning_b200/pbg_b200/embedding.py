@@ -5,7 +5,8 @@ types, seats, streets, actions, positions, classes, ranks and suits;
 pbg/games/poker/model/preflop.py:206-233, shared.py:36-72).  ``embedding``
 looks rows up and scales them in one pass; ``embedding_backward`` sums the
 incoming rows of each index after sorting the tokens by index, without
-floating-point atomics: the same inputs give the same bits in every run.
+floating-point atomics: the same inputs, laid out and aligned alike, give the
+same bits in every run on a device.
 ``pbg_b200.model_train.embedding_train`` is the two as one autograd function.
 
 An index outside the table gives a row of zeros and no gradient, and sets the
@@ -74,7 +75,8 @@ def embedding(table: Tensor, index: Tensor, scale: float = 1.0, *, out_dtype: to
               out: Tensor | None = None) -> Tensor:
     """``scale * table[index]``: fp32, bf16 or fp16 rows ``[rows, width]`` (columns contiguous, any row
     stride), ``index`` int64 or int32 of any shape; the product is taken in fp32 and rounded once to
-    ``out_dtype`` (the table's by default) or to ``out``'s type (contiguous ``[*index.shape, width]``)."""
+    ``out_dtype`` (the table's by default) or to ``out``'s type (contiguous ``[*index.shape, width]``).
+    The result is not part of an autograd graph: ``model_train.embedding_train`` is the differentiable lookup."""
 
     if table.ndim != 2 or table.dtype not in TYPES:
         raise NativeError("embedding: the table must be a float32, bfloat16 or float16 matrix")

@@ -338,7 +338,8 @@ class ModelLearnerStep:
 
     ``muon``: options of ``FlatMuon`` (a dict, may be empty): the hidden matrices (``is_hidden_matrix``)
     then take its transition and AdamW keeps the tables, vectors and head rows; ``grad`` is the whole
-    flat gradient either way.  A gradient that is not finite anywhere stops both transitions.
+    flat gradient either way (``adam.grad`` is AdamW's part of it then, and ``grad_clip`` that part's norm).
+    A gradient that is not finite anywhere stops both transitions.
     ``sorted_embeddings``: the tables' gradients by sorted tokens instead of one-hot products.
 
     A step waits for nothing on the host: ``checks.raise_input_errors`` reports, whenever it is called, what

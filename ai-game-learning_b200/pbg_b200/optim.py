@@ -6,8 +6,8 @@ so one fused kernel sequence updates the whole model.
 
 ``orthogonalize`` brings every singular value of a matrix to about one by
 Newton-Schulz products; ``FlatMuon`` is the transition that updates the
-matrices of a flat master by their orthogonalised momentum, all of them in one
-launch.
+matrices of a flat master by their orthogonalised momentum, all of them
+together.
 """
 
 from __future__ import annotations
@@ -89,7 +89,8 @@ def orthogonalize(x: Tensor, *, steps: int = 5, coefficients: tuple[float, float
 
     The output has ``x``'s shape and ``out_dtype`` (``x``'s by default), or goes to ``out`` (contiguous; it
     may be ``x`` itself).  Products carry fp32 accuracy whatever the types; the result is rounded
-    once.  A matrix of zeros gives zeros, one with a NaN or an infinity gives NaN."""
+    once.  A matrix of zeros gives zeros, one with a NaN or an infinity gives NaN.  The result is not part
+    of an autograd graph, whatever ``x`` is."""
 
     if x.ndim < 2 or x.dtype not in _TYPES:
         raise NativeError("orthogonalize takes float32, bfloat16 or float16 matrices [..., rows, cols]")
@@ -148,8 +149,9 @@ class FlatMuon:
 
     with ``s = sqrt(max(1, rows / cols))`` (``adjust="shape"``) or ``0.2 sqrt(max(rows, cols))``
     (``"rms"``: updates as large as AdamW's usual ones).  ``controls`` (device fp32: lr, momentum, decay,
-    scale) may be rewritten between steps, also under a captured graph.  All matrices go through one
-    launch (several where their tiles would pass 1 GB).  A direction that is not finite leaves masters
+    scale) may be rewritten between steps, also under a captured graph.  A step launches the squares of
+    all directions, then the conversion and the products of all matrices whose short side is over 128 (of as
+    many at a time as 1 GB of tiles holds), then all others' teams.  A direction that is not finite leaves masters
     and momenta untouched, clears the matrices' gradients and sets ``skipped`` to 1 for that step."""
 
     def __init__(self, master: Tensor, matrices, *, lr=0.02, momentum=0.95, decay=0.0, scale=1.0, nesterov=True,

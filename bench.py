@@ -748,8 +748,8 @@ def learner_scaling_cfg2(args, device, world, rank, pre_rows=1024, post_rows=256
     def one():
         step.gradient(batches)
         if world > 1:
-            dist.all_reduce(step.adam.grad)
-        step.adam.step()
+            dist.all_reduce(step.grad)
+        step.transition()
 
     for _ in range(max(3, args.warmup)):
         one()

@@ -423,8 +423,8 @@ int pbg_embedding(int64_t tokens, int64_t rows, int64_t width, const void *index
                   int32_t table_type, int64_t ldt, float scale, void *out, int32_t out_type, uint32_t *error,
                   void *stream);
 /* Its gradient: out[v, :] = (accumulate: out[v, :] +) scale * sum of grad[t, :] over t with index[t] == v,
- * rows without tokens zero (accumulate: untouched).  fp32 sums in an order that sizes alone determine,
- * rounded once.  padding: an index whose tokens give no gradient, or -1.  workspace: 256-byte aligned
+ * rows without tokens zero (accumulate: untouched).  fp32 sums in an order that sizes, strides, alignment, indices and the
+ * device determine, rounded once.  padding: an index whose tokens give no gradient, or -1.  workspace: 256-byte aligned
  * device memory of pbg_embedding_backward_workspace(tokens, width) bytes, any contents, one per call in
  * flight.  error: bit 0 an index outside the table (no gradient), bit 1 a grid barrier gave up.  At most
  * 2^31 - 1 tokens and rows. */
